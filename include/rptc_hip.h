@@ -32,11 +32,16 @@ extern "C" {
 #define RPTC_AS_WRITTEN 0
 #define RPTC_CONTINUOUS 1
 
+/* element types of the ops that take more than fp16 */
+#define RPTC_F16 0
+#define RPTC_BF16 1
+#define RPTC_F32 2
+
 #define RPTC_OK 0
 #define RPTC_ENULL (-1)      /* a required pointer is NULL */
 #define RPTC_ESHAPE (-2)     /* a size breaks the op's shape rule */
 #define RPTC_EALIGN (-3)     /* a pointer is not 16-byte aligned */
-#define RPTC_EMODE (-4)      /* carry_mode is not one of the two modes */
+#define RPTC_EMODE (-4)      /* carry_mode is not one of the two modes, or dtype none the op takes */
 #define RPTC_ELIMIT (-5)     /* a size exceeds what the kernel's LDS staging can hold */
 #define RPTC_EDEVICE (-6)    /* the current device is not gfx950 */
 #define RPTC_EALIAS (-7)     /* an output buffer aliases an input the op still reads */
@@ -388,6 +393,35 @@ int rptc_lite_viterbi(const float *samples, const float *importance, int64_t imp
 /* Bytes of scratch rptc_lite_viterbi needs (back pointers of every step, and the path costs where they are not held
  * in registers); 0 for parameters it does not take.  No counterpart in the reference, which lets jax allocate. */
 int64_t rptc_lite_viterbi_scratch_bytes(int L, int R, int64_t rows, int64_t steps);
+
+/*
+ * Attention of whole prompts: packed sequences of different lengths, grouped heads, fp16 or bf16 (dtype), fp32 inside.  No
+ * counterpart in the reference (it generates with transformers, quantize_hf.py:229-236).  Sequence s has the query
+ * rows [q_start[s], q_start[s+1]) and the key rows [k_start[s], k_start[s] + k_len[s]); with causal != 0 query i of Lq sees
+ * the keys j <= i + Lk - Lq (the last query sees all: a chunk at the end of a context), else all Lk.
+ *   out[i] = softmax(scale * q[i] . K^T) V,  lse[i] = log sum exp(scale * q[i] . K^T)  (lse float [total_q][heads], may be NULL)
+ * A query that sees no key gets out = 0, lse = -inf.  What a query does not see does not reach it, not-a-number included.
+ * Rows of q outside every sequence, and sequences whose rows lie outside q or k (checked on the device), are left unwritten.
+ *   q [total_q][heads][hd], k, v [total_k][kv_heads][hd], out as q, by token and head strides in elements (multiples of
+ *   8, tokens at most 2^23 apart; a key cache [kv_heads][positions][hd] has k_token = hd, k_head = positions * hd); head h reads
+ *   key head h / (heads / kv_heads); hd in {32, 64, 128, 256}; out must not overlap q, k or v
+ *   q_start int32 [seqs + 1], k_start, k_len int32 [seqs], device memory.  q_start NULL: one sequence of all query rows.
+ *   k_start and k_len NULL (both or neither): the keys lie as the queries do (total_k == total_q), or, without q_start, are
+ *   all key rows.  max_k an upper bound of k_len (total_k will do:
+ *   it only decides how far the keys of a call with few rows are split)
+ *   workspace  rptc_attn_prompt_workspace_bytes(...) bytes of device memory, 16-byte aligned (0: may be NULL); no
+ *              initialisation, calls that may overlap need one each.  At most 2^24 query rows, 1024 heads, 2^20 sequences.
+ */
+typedef struct rptc_prompt_strides {
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+} rptc_prompt_strides;
+int64_t rptc_attn_prompt_workspace_bytes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t max_k, int64_t heads,
+                                         int64_t kv_heads, int64_t hd);
+int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint16_t *v, uint16_t *out, float *lse,
+                     const int32_t *q_start, const int32_t *k_start, const int32_t *k_len, int64_t seqs, int64_t total_q,
+                     int64_t total_k, int64_t max_k, int64_t heads, int64_t kv_heads, int64_t hd,
+                     const rptc_prompt_strides *strides, float scale, int causal, int dtype, void *workspace,
+                     int64_t workspace_bytes, void *stream, float *ms);
 
 #ifdef __cplusplus
 }

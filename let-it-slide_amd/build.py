@@ -45,6 +45,7 @@ def asm_blocks_left_waiting(assembly):
     that issues LDS reads or global loads waits for them before it ends.  The data of such a request lands in its
     register some time after the instruction; the compiler does not know that, and between two `asm` statements it is
     free to copy or reuse that register, so a request and its wait must never sit in different statements.
+    (A load straight into LDS, `... lds`, writes no register: its data may arrive behind the block.)
     Returns [(line number, instruction)] for every request that its own block does not wait for (empty = good)."""
     bad = []
     lgkm, vm, in_asm = [], [], False
@@ -58,7 +59,7 @@ def asm_blocks_left_waiting(assembly):
         elif in_asm:
             if re.match(r"ds_(read|bpermute|permute)", t):
                 lgkm.append((no, t))
-            elif re.match(r"(global|buffer|flat)_load", t):
+            elif re.match(r"(global|buffer|flat)_load", t) and not re.search(r"\blds\b", t):
                 vm.append((no, t))
             elif t.startswith("s_waitcnt"):
                 k = re.search(r"lgkmcnt\((\d+)\)", t)

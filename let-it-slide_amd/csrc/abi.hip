@@ -15,6 +15,7 @@ int prepare_matmul(int device);
 int prepare_hadamard();
 int prepare_decode_glue(int device);
 int prepare_viterbi();
+int prepare_attn_prompt();
 void matmul_counters(int device, uint32_t **counters, int *count);
 void matvec_t_counters(int device, uint32_t **counters, int *count);
 void attn_counters(int device, uint32_t **counters, int *count);
@@ -50,6 +51,7 @@ int device_info(DeviceInfo **out)
         if ((rc = prepare_hadamard())) return rc;
         if ((rc = prepare_decode_glue(dev))) return rc;
         if ((rc = prepare_viterbi())) return rc;
+        if ((rc = prepare_attn_prompt())) return rc;
         g_ready[dev] = true;
     }
     *out = &g_devices[dev];
@@ -114,7 +116,7 @@ extern "C" const char *rptc_status_string(int status)
     case RPTC_ENULL: return "a required pointer is NULL";
     case RPTC_ESHAPE: return "a size breaks the op's shape rule";
     case RPTC_EALIGN: return "a pointer is not 16-byte aligned";
-    case RPTC_EMODE: return "carry_mode must be RPTC_AS_WRITTEN (0) or RPTC_CONTINUOUS (1)";
+    case RPTC_EMODE: return "carry_mode must be RPTC_AS_WRITTEN (0) or RPTC_CONTINUOUS (1); dtype one the op takes";
     case RPTC_ELIMIT: return "a size exceeds what the kernel supports";
     case RPTC_EDEVICE: return "the current device is not a gfx950 GPU";
     case RPTC_EALIAS: return "an output buffer aliases an input the op still reads";

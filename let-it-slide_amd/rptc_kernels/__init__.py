@@ -66,6 +66,11 @@ class ChainPlan(ctypes.Structure):
     _fields_ = [("opaque", ctypes.c_uint64 * 10)]
 
 
+class PromptStrides(ctypes.Structure):
+    """rptc_prompt_strides of include/rptc_hip.h (elements)."""
+    _fields_ = [(n, _I64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "out_token", "out_head")]
+
+
 _MATVEC_ARGS = [_VP, _VP, _VP, _VP, _I64, _I64, _INT, _VP, _FP]
 _SIGNATURES = {
     "rptc_version": ([], _INT),
@@ -109,6 +114,8 @@ _SIGNATURES = {
     "rptc_decompress_matvec_hadamard": ([_VP, _VP, _VP, _VP, _VP, _I64, _I64, _I64, _INT, _INT, _VP, _FP], _INT),
     "rptc_decompress_matvec_rmsnorm": ([_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64, ctypes.c_float, _INT, _INT,
                                         _VP, _FP], _INT),
+    "rptc_attn_prompt_workspace_bytes": ([_I64] * 7, _I64),
+    "rptc_attn_prompt": ([_VP] * 8 + [_I64] * 7 + [ctypes.POINTER(PromptStrides), ctypes.c_float, _INT, _INT, _VP, _I64, _VP, _FP], _INT),
     "rptc_decompress_matvec_affine": ([_VP] * 8 + [_I64, _I64, _INT, _INT, _VP, _FP], _INT),
     "rptc_decompress_matvec_silu_affine": ([_VP] * 8 + [_I64, _I64, _INT, _INT, _VP, _FP], _INT),
     "rptc_decompress_matvec_rmsnorm_affine": ([_VP] * 11 + [_I64, _I64, ctypes.c_float, _INT, _INT, _VP, _FP], _INT),
@@ -800,3 +807,89 @@ def matvec_bits_dense(compressed, codebook, out, bits):
     _check(n % 64 == 0 and m >= 1 and n >= 64, "out.size(1) % 64 == 0")
     _check(compressed.numel() * 32 == m * n * bits, "compressed.numel() * 32 == m * n * bits")
     return _call(library().rptc_matvec_bits_dense, (compressed, codebook, out), m, n, S, bits)
+
+
+# ---------------------------------------------------------------- prompts, the 4-bit cache, scoring
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}      # RPTC_F16, RPTC_BF16, RPTC_F32
+
+
+def _check_rows(t, name, dtype):
+    # [tokens, heads, hd], any token and head strides, the head dimension contiguous
+    _check(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
+    _check(t.is_cuda, f"{name} must be a CUDA tensor")
+    _check(t.dim() == 3, f"{name}.dim() == 3 ([tokens, heads, head_dim])")
+    _check(t.dtype == dtype, f"{name} must have the type of q")
+    _check(t.stride(2) == 1, f"{name} must be contiguous along the head dimension")
+
+
+def _strides(t):
+    # the stride of a dimension of one element means nothing: any valid one will do
+    n, h, hd = t.shape
+    a, b, _ = t.stride()
+    return a if n > 1 else hd, b if h > 1 else hd
+
+
+def _check_index(t, name, dtype, count, device):
+    _check_input(t, name)
+    _check(t.dtype == dtype and t.dim() == 1, f"{name} must be a 1-D {str(dtype)[6:]} tensor")
+    _check(t.size(0) == count, f"{name}.size(0) == {count}")
+    _check(t.device == device, "all tensors must be on the same device")
+
+
+def attn_prompt(q, k, v, out, q_start=None, k_start=None, k_len=None, causal=True, scale=None, lse=None, max_k=None, timed=None):
+    """Attention of whole prompts, packed one behind the other: out[i] = softmax(scale * q[i] . K^T) V.
+
+    q, out [Tq, heads, hd], k, v [Tk, kv_heads, hd], fp16 or bf16, head h reading key head h // (heads // kv_heads); any
+    token and head strides that are multiples of 8 (views of a projection's output, a transposed cache
+    [kv_heads, positions, hd]); hd 32, 64, 128 or 256.  Sequence s has the query rows q_start[s] .. q_start[s+1] and the
+    k_len[s] key rows from k_start[s] on (int32 tensors on the device).  Without k_start / k_len the keys lie as the
+    queries do; without q_start there is one sequence.  ``causal``: query i of Lq sees the keys j <= i + Lk - Lq, so a
+    chunk's last query sees the whole context.  ``scale`` defaults to hd ** -0.5.  ``lse`` (float32 [Tq, heads], optional)
+    takes the logarithm of every row's sum.  A query that sees no key gets 0 (lse -inf); rows outside every sequence stay as
+    they are.  ``max_k``: an upper bound of k_len where the key rows are many more (a cache's positions).  Returns elapsed ms."""
+    _check(isinstance(q, torch.Tensor) and q.dtype in (torch.float16, torch.bfloat16), "q must be an fp16 or bf16 tensor")
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
+        _check_rows(t, name, q.dtype)
+        _check(t.device == q.device, "all tensors must be on the same device")
+    (tq, heads, hd), (tk, kv_heads, _) = q.shape, k.shape
+    _check(out.shape == q.shape, "out.shape == q.shape")
+    _check(v.shape == k.shape and k.size(2) == hd, "v.shape == k.shape, k.size(2) == q.size(2)")
+    _check(hd in (32, 64, 128, 256), "the head dimension must be 32, 64, 128 or 256")
+    _check(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "heads must be a multiple of kv_heads")
+    device = q.device
+    seqs = 1
+    if q_start is not None:
+        seqs = q_start.size(0) - 1
+        _check(seqs >= 1, "q_start must hold at least two entries")
+        _check_index(q_start, "q_start", torch.int32, seqs + 1, device)
+    _check((k_start is None) == (k_len is None), "k_start and k_len go together")
+    if k_start is not None:
+        _check_index(k_start, "k_start", torch.int32, seqs, device)
+        _check_index(k_len, "k_len", torch.int32, seqs, device)
+    else:
+        _check(q_start is None or tk == tq, "without k_start the keys lie as the queries do: k.size(0) == q.size(0)")
+    if lse is not None:
+        _check_input(lse, "lse")
+        _check(lse.dtype == torch.float32 and lse.shape == (tq, heads), "lse must be float32 [Tq, heads]")
+        _check(lse.device == device, "all tensors must be on the same device")
+    if tq == 0:
+        return 0.0
+    st = PromptStrides(*_strides(q), *_strides(k), *_strides(v), *_strides(out))
+    sizes = (seqs, tq, tk, tk if max_k is None else int(max_k), heads, kv_heads, hd)
+    lib = library()
+    ms = ctypes.c_float(0.0)
+    with torch.cuda.device(device):
+        need = lib.rptc_attn_prompt_workspace_bytes(*sizes)
+        if need < 0:
+            _status(int(need))
+        # from torch's allocator, so it is this call's own on the current stream and in a graph being captured
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        rc = lib.rptc_attn_prompt(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
+                                  None if q_start is None else q_start.data_ptr(), None if k_start is None else k_start.data_ptr(),
+                                  None if k_len is None else k_len.data_ptr(), *sizes, ctypes.byref(st),
+                                  hd ** -0.5 if scale is None else float(scale), 1 if causal else 0, _DTYPES[q.dtype],
+                                  None if ws is None else ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream,
+                                  ctypes.byref(ms) if (_timing if timed is None else timed) else None)
+    _status(rc)
+    return float(ms.value)
