@@ -423,6 +423,59 @@ int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint16_t *v, ui
                      const rptc_prompt_strides *strides, float scale, int causal, int dtype, void *workspace,
                      int64_t workspace_bytes, void *stream, float *ms);
 
+/*
+ * A key/value cache held in 4 bits.  No counterpart in the reference (it generates with transformers, quantize_hf.py:229-236).
+ * k_cache, v_cache: uint8 [seqs][kv_heads][max_len][rptc_kv4_row_bytes(hd)], hd in {32, 64, 128, 256}.  A row holds hd fp16
+ * values in groups of 32: m = min x, s = fp16((max x - min x) / 15), code = clamp(rint((x - m) / s), 0, 15) (0 where s = 0; the
+ * quotients in fp32), and stands for fp16(code * s + m).  A group with a value that is no finite number reads as
+ * not-a-number.  hd / 2 bytes of codes (word w: values 8w .. 8w+7, nibble t the value 8w + 2t, nibble t + 4 the value
+ * 8w + 2t + 1), then (s, m) of every group.
+ *   rptc_kv4_append       k, v fp16 [total][kv_heads][hd] by token and head strides (elements, multiples of 8): row t of sequence
+ *                         s goes to position pos[s] + t - q_start[s] of cache s.  q_start int32 [seqs + 1] (rows of
+ *                         no sequence are skipped), or NULL: total / seqs rows a sequence; pos int64 [seqs]; both device memory.
+ *                         Rows whose position lies outside [0, max_len) are not written.
+ *   rptc_kv4_read         the first `rows` positions of every sequence as fp16: k, v [seqs * rows][kv_heads][hd] by strides
+ *   rptc_kv4_rope_append  one token per sequence: qkv [seqs][(heads + 2 kv_heads) * hd] = [q | k | v]; rotates the (2i, 2i+1)
+ *                         pairs of q and k by cos/sin [max_len][hd/2] at pos[s] as rptc_rope_cache does, writes q_out
+ *                         [seqs][heads][hd] and appends k and v at pos[s].  A sequence whose position lies outside is skipped.
+ *   rptc_kv4_attn_decode  out[s][h] = softmax(scale * q[s][h] . K^T) V over positions 0..pos[s] of cache s, head h reading key head
+ *                         h / (heads / kv_heads); q fp16 [seqs][heads][hd], sequences q_token elements apart, out
+ *                         contiguous.  A sequence whose position lies outside [0, max_len) (a padded batch) is left unwritten.
+ *                         workspace: rptc_kv4_attn_decode_workspace_bytes(...) bytes, 16-byte aligned (0: may be NULL),
+ *                         no initialisation; calls that may overlap need one each.
+ * At most 65535 sequences, 1024 heads, 2^30 - 1 positions; q_out, out and the caches must not overlap the inputs.
+ */
+int64_t rptc_kv4_row_bytes(int64_t hd);
+int rptc_kv4_append(const uint16_t *k, const uint16_t *v, uint8_t *k_cache, uint8_t *v_cache, const int64_t *pos,
+                    const int32_t *q_start, int64_t seqs, int64_t total, int64_t kv_heads, int64_t hd, int64_t max_len,
+                    int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, void *stream, float *ms);
+int rptc_kv4_read(const uint8_t *k_cache, const uint8_t *v_cache, uint16_t *k, uint16_t *v, int64_t seqs, int64_t rows,
+                  int64_t kv_heads, int64_t hd, int64_t max_len, int64_t k_token, int64_t k_head, int64_t v_token,
+                  int64_t v_head, void *stream, float *ms);
+int rptc_kv4_rope_append(const uint16_t *qkv, const uint16_t *cos_t, const uint16_t *sin_t, const int64_t *pos, uint16_t *q_out,
+                         uint8_t *k_cache, uint8_t *v_cache, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t hd,
+                         int64_t max_len, void *stream);
+int64_t rptc_kv4_attn_decode_workspace_bytes(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t hd, int64_t max_len);
+int rptc_kv4_attn_decode(const uint16_t *q, const uint8_t *k_cache, const uint8_t *v_cache, const int64_t *pos, uint16_t *out,
+                         int64_t seqs, int64_t heads, int64_t kv_heads, int64_t hd, int64_t max_len, int64_t q_token, float scale,
+                         void *workspace, int64_t workspace_bytes, void *stream, float *ms);
+
+/*
+ * Log probabilities of given tokens, the entropy of every row and its most likely tokens, from logits in one pass.  The measure
+ * the reference's perplexity harness takes with framework ops (contrib/eval_ppl.py:35-39), per token.
+ *   logits        [rows][vocab], rows row_stride elements apart, fp16, bf16 or fp32 (dtype)
+ *   tokens        int64 [rows], device memory (may be NULL without logprob)
+ *   logprob       float [rows]: log softmax(logits[r])[tokens[r]], not-a-number for a token outside [0, vocab)
+ *   entropy       float [rows], nats
+ *   top_ids       int64 [rows][top], top_logprobs float [rows][top]: the `top` largest logits of a row in falling order, equal
+ *                 ones by the lowest id (a not-a-number counts as -inf); top <= 64 and <= vocab
+ * Each output may be NULL (top == 0 without the last two).  fp32 inside.  A row that holds +inf or a not-a-number, or nothing
+ * but -inf, has not-a-number for probabilities and entropy.
+ */
+int rptc_token_logprobs(const void *logits, int dtype, const int64_t *tokens, float *logprob, float *entropy, int64_t *top_ids,
+                        float *top_logprobs, int64_t rows, int64_t vocab, int64_t row_stride, int64_t top, void *stream,
+                        float *ms);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,6 +16,7 @@ int prepare_hadamard();
 int prepare_decode_glue(int device);
 int prepare_viterbi();
 int prepare_attn_prompt();
+int prepare_kv4();
 void matmul_counters(int device, uint32_t **counters, int *count);
 void matvec_t_counters(int device, uint32_t **counters, int *count);
 void attn_counters(int device, uint32_t **counters, int *count);
@@ -52,6 +53,7 @@ int device_info(DeviceInfo **out)
         if ((rc = prepare_decode_glue(dev))) return rc;
         if ((rc = prepare_viterbi())) return rc;
         if ((rc = prepare_attn_prompt())) return rc;
+        if ((rc = prepare_kv4())) return rc;
         g_ready[dev] = true;
     }
     *out = &g_devices[dev];

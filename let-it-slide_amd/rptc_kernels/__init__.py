@@ -116,6 +116,13 @@ _SIGNATURES = {
                                         _VP, _FP], _INT),
     "rptc_attn_prompt_workspace_bytes": ([_I64] * 7, _I64),
     "rptc_attn_prompt": ([_VP] * 8 + [_I64] * 7 + [ctypes.POINTER(PromptStrides), ctypes.c_float, _INT, _INT, _VP, _I64, _VP, _FP], _INT),
+    "rptc_kv4_row_bytes": ([_I64], _I64),
+    "rptc_kv4_append": ([_VP] * 6 + [_I64] * 9 + [_VP, _FP], _INT),
+    "rptc_kv4_read": ([_VP] * 4 + [_I64] * 9 + [_VP, _FP], _INT),
+    "rptc_kv4_rope_append": ([_VP] * 7 + [_I64] * 5 + [_VP], _INT),
+    "rptc_kv4_attn_decode_workspace_bytes": ([_I64] * 5, _I64),
+    "rptc_kv4_attn_decode": ([_VP] * 5 + [_I64] * 6 + [ctypes.c_float, _VP, _I64, _VP, _FP], _INT),
+    "rptc_token_logprobs": ([_VP, _INT] + [_VP] * 5 + [_I64] * 4 + [_VP, _FP], _INT),
     "rptc_decompress_matvec_affine": ([_VP] * 8 + [_I64, _I64, _INT, _INT, _VP, _FP], _INT),
     "rptc_decompress_matvec_silu_affine": ([_VP] * 8 + [_I64, _I64, _INT, _INT, _VP, _FP], _INT),
     "rptc_decompress_matvec_rmsnorm_affine": ([_VP] * 11 + [_I64, _I64, ctypes.c_float, _INT, _INT, _VP, _FP], _INT),
@@ -891,5 +898,189 @@ def attn_prompt(q, k, v, out, q_start=None, k_start=None, k_len=None, causal=Tru
                                   hd ** -0.5 if scale is None else float(scale), 1 if causal else 0, _DTYPES[q.dtype],
                                   None if ws is None else ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream,
                                   ctypes.byref(ms) if (_timing if timed is None else timed) else None)
+    _status(rc)
+    return float(ms.value)
+
+
+def kv4_row_bytes(hd):
+    """Bytes of a row (one position of one head) of the 4-bit cache: hd / 2 of codes and a scale and a minimum for every 32 values."""
+    _check(hd in (32, 64, 128, 256), "the head dimension must be 32, 64, 128 or 256")
+    return hd // 2 + hd // 8
+
+
+def kv4_cache(seqs, kv_heads, max_len, hd, device="cuda"):
+    """A pair of empty 4-bit caches (keys, values), uint8 [seqs, kv_heads, max_len, kv4_row_bytes(hd)]; zeros stand for zeros."""
+    shape = (seqs, kv_heads, max_len, kv4_row_bytes(hd))
+    return torch.zeros(shape, dtype=torch.uint8, device=device), torch.zeros(shape, dtype=torch.uint8, device=device)
+
+
+def _check_kv4(k_cache, v_cache, hd, kv_heads=None):
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _check_input(t, name)
+        _check(t.dtype == torch.uint8 and t.dim() == 4, f"{name} must be uint8 [seqs, kv_heads, positions, row bytes]")
+    _check(k_cache.shape == v_cache.shape and k_cache.device == v_cache.device, "k_cache and v_cache must be alike")
+    _check(k_cache.size(3) == kv4_row_bytes(hd), "the cache's rows must have kv4_row_bytes(head dimension) bytes")
+    _check(kv_heads is None or k_cache.size(1) == kv_heads, "the cache must have as many heads as k and v")
+
+
+def _kv4_rows(k, v, device):
+    for t, name in ((k, "k"), (v, "v")):
+        _check_rows(t, name, torch.float16)
+        _check(t.device == device, "all tensors must be on the same device")
+    _check(k.shape == v.shape, "v.shape == k.shape")
+
+
+def kv4_append(k, v, k_cache, v_cache, pos, q_start=None, timed=None):
+    """Put the rows k, v (fp16 [tokens, kv_heads, hd], strides as in ``attn_prompt``) into the 4-bit caches of
+    ``kv4_cache``: sequence s's rows q_start[s] .. q_start[s+1] go to positions pos[s], pos[s] + 1, ... of cache s (int32 and
+    int64 tensors on the device; without q_start every sequence has tokens / seqs rows).  Rows that do not fit are
+    not written.  Returns elapsed ms."""
+    _check(isinstance(k, torch.Tensor) and k.dim() == 3, "k must be [tokens, kv_heads, head_dim]")
+    total, kv_heads, hd = k.shape
+    _check_kv4(k_cache, v_cache, hd, kv_heads)
+    device = k_cache.device
+    _kv4_rows(k, v, device)
+    seqs, max_len = k_cache.size(0), k_cache.size(2)
+    _check_index(pos, "pos", torch.int64, seqs, device)
+    if q_start is not None:
+        _check_index(q_start, "q_start", torch.int32, seqs + 1, device)
+    else:
+        _check(total % seqs == 0, "without q_start the rows must divide evenly: k.size(0) % k_cache.size(0) == 0")
+    if total == 0 or max_len == 0:
+        return 0.0
+    ms = ctypes.c_float(0.0)
+    with torch.cuda.device(device):
+        rc = library().rptc_kv4_append(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pos.data_ptr(),
+                                       None if q_start is None else q_start.data_ptr(), seqs, total, kv_heads, hd, max_len,
+                                       *_strides(k), *_strides(v), torch.cuda.current_stream().cuda_stream,
+                                       ctypes.byref(ms) if (_timing if timed is None else timed) else None)
+    _status(rc)
+    return float(ms.value)
+
+
+def kv4_read(k_cache, v_cache, k, v, timed=None):
+    """The first positions of every sequence of the 4-bit caches as fp16: k, v [seqs * rows, kv_heads, hd] (strides as in
+    ``attn_prompt``) receive positions 0 .. rows-1, sequence after sequence.  Returns elapsed ms."""
+    _check(isinstance(k, torch.Tensor) and k.dim() == 3, "k must be [tokens, kv_heads, head_dim]")
+    total, kv_heads, hd = k.shape
+    _check_kv4(k_cache, v_cache, hd, kv_heads)
+    device = k_cache.device
+    _kv4_rows(k, v, device)
+    seqs, max_len = k_cache.size(0), k_cache.size(2)
+    _check(seqs >= 1 and total % seqs == 0 and total // seqs <= max_len, "k must hold the same number of rows for every sequence, at most the cache's positions")
+    if total == 0:
+        return 0.0
+    for t, name in ((k, "k"), (v, "v")):
+        _check(all(s != 0 or n == 1 for s, n in zip(t.stride(), t.shape)), f"{name} must not repeat elements")
+    ms = ctypes.c_float(0.0)
+    with torch.cuda.device(device):
+        rc = library().rptc_kv4_read(k_cache.data_ptr(), v_cache.data_ptr(), k.data_ptr(), v.data_ptr(), seqs, total // seqs, kv_heads,
+                                     hd, max_len, *_strides(k), *_strides(v), torch.cuda.current_stream().cuda_stream,
+                                     ctypes.byref(ms) if (_timing if timed is None else timed) else None)
+    _status(rc)
+    return float(ms.value)
+
+
+def kv4_rope_append(qkv, cos, sin, pos, q_out, k_cache, v_cache):
+    """One token of every sequence on its way into the 4-bit cache: rotate the (2i, 2i+1) pairs of q and k of qkv (fp16
+    [seqs, (heads + 2 kv_heads) * hd]) by cos/sin (fp16 [positions, hd/2]) at pos (int64 [seqs]), write q to q_out (fp16
+    [seqs, heads, hd]) and append k and v at pos.  A sequence whose position lies outside the cache is skipped.  Asynchronous."""
+    for t, name in ((qkv, "qkv"), (cos, "cos"), (sin, "sin"), (q_out, "q_out")):
+        _check_input(t, name)
+        _check(t.dtype == torch.float16, f"{name} must be fp16")
+    _check(q_out.dim() == 3 and qkv.dim() == 2, "q_out must be [seqs, heads, head_dim], qkv [seqs, (heads + 2 kv_heads) * head_dim]")
+    seqs, heads, hd = q_out.shape
+    _check_kv4(k_cache, v_cache, hd)
+    kv_heads, max_len, device = k_cache.size(1), k_cache.size(2), k_cache.device
+    _check(k_cache.size(0) == seqs and qkv.shape == (seqs, (heads + 2 * kv_heads) * hd), "qkv must be [seqs, (heads + 2 kv_heads) * head_dim]")
+    _check(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "heads must be a multiple of kv_heads")
+    _check(cos.shape == sin.shape and cos.dim() == 2 and cos.size(0) >= max_len and cos.size(1) == hd // 2, "cos and sin must be [positions >= the cache's, head_dim / 2]")
+    _check_index(pos, "pos", torch.int64, seqs, device)
+    _check(all(t.device == device for t in (qkv, cos, sin, q_out)), "all tensors must be on the same device")
+    if seqs == 0 or max_len == 0:
+        return
+    with torch.cuda.device(device):
+        rc = library().rptc_kv4_rope_append(qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), q_out.data_ptr(),
+                                            k_cache.data_ptr(), v_cache.data_ptr(), seqs, heads, kv_heads, hd, max_len,
+                                            torch.cuda.current_stream().cuda_stream)
+    _status(rc)
+
+
+def kv4_attn_decode(q, k_cache, v_cache, pos, out, scale=None, timed=None):
+    """Attention of one token per sequence over the 4-bit caches: out[s, h] = softmax(scale * q[s, h] . K^T) V over positions
+    0 .. pos[s] of cache s.  q, out fp16 [seqs, heads, hd] (q's sequences may be any multiple of 8 elements apart), head h
+    reading key head h // (heads // kv_heads); pos int64 [seqs] on the device.  A sequence whose pos lies outside the cache
+    (a padded batch: -1) keeps what ``out`` holds.  ``scale`` defaults to hd ** -0.5.  Returns elapsed ms."""
+    _check(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [seqs, heads, head_dim]")
+    seqs, heads, hd = q.shape
+    _check_kv4(k_cache, v_cache, hd)
+    device = k_cache.device
+    _check(q.is_cuda, "q must be a CUDA tensor")
+    _check(q.dtype == torch.float16 and q.stride(2) == 1 and (heads == 1 or q.stride(1) == hd), "q must be fp16 with contiguous heads")
+    _check_input(out, "out")
+    _check(out.dtype == torch.float16 and out.shape == q.shape, "out must be fp16 and have the shape of q")
+    _check(q.device == device and out.device == device, "all tensors must be on the same device")
+    kv_heads, max_len = k_cache.size(1), k_cache.size(2)
+    _check(k_cache.size(0) == seqs, "k_cache.size(0) == q.size(0)")
+    _check(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "heads must be a multiple of kv_heads")
+    _check_index(pos, "pos", torch.int64, seqs, device)
+    if seqs == 0 or max_len == 0:
+        return 0.0
+    lib = library()
+    ms = ctypes.c_float(0.0)
+    with torch.cuda.device(device):
+        need = lib.rptc_kv4_attn_decode_workspace_bytes(seqs, heads, kv_heads, hd, max_len)
+        if need < 0:
+            _status(int(need))
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        rc = lib.rptc_kv4_attn_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pos.data_ptr(), out.data_ptr(), seqs, heads,
+                                      kv_heads, hd, max_len, q.stride(0) if seqs > 1 else heads * hd,
+                                      hd ** -0.5 if scale is None else float(scale), None if ws is None else ws.data_ptr(), need,
+                                      torch.cuda.current_stream().cuda_stream, ctypes.byref(ms) if (_timing if timed is None else timed) else None)
+    _status(rc)
+    return float(ms.value)
+
+
+def token_logprobs(logits, tokens=None, logprob=None, entropy=None, top_ids=None, top_logprobs=None, timed=None):
+    """Log probabilities from logits (fp16, bf16 or fp32 [rows, vocab], rows any distance apart), in one pass over them.
+
+    logprob (float32 [rows]): log softmax of tokens (int64 [rows]; not-a-number for a token outside the vocabulary);
+    entropy (float32 [rows]): of every row, in nats; top_ids (int64 [rows, k]) and top_logprobs (float32 [rows, k]): the k largest
+    logits in falling order, equal ones by the lowest id, k at most 64.  Each output is optional.  A row that holds +inf or a
+    not-a-number, or nothing but -inf, gives not-a-number.  Returns elapsed ms."""
+    _check(isinstance(logits, torch.Tensor), "logits must be a torch.Tensor")
+    _check(logits.is_cuda, "logits must be a CUDA tensor")
+    _check(logits.dim() == 2 and logits.dtype in _DTYPES, "logits must be fp16, bf16 or float32 [rows, vocab]")
+    rows, vocab = logits.shape
+    _check(vocab >= 1, "the vocabulary must not be empty")
+    _check(vocab == 1 or logits.stride(1) == 1, "logits must be contiguous along the vocabulary")
+    _check(not (logprob is None and entropy is None and top_ids is None and top_logprobs is None), "at least one output is needed")
+    device = logits.device
+    if logprob is not None:
+        _check(tokens is not None, "logprob needs tokens")
+    if tokens is not None:
+        _check_index(tokens, "tokens", torch.int64, rows, device)
+    for t, name in ((logprob, "logprob"), (entropy, "entropy")):
+        if t is not None:
+            _check_index(t, name, torch.float32, rows, device)
+    top = 0
+    for t, name, dtype in ((top_ids, "top_ids", torch.int64), (top_logprobs, "top_logprobs", torch.float32)):
+        if t is not None:
+            _check_input(t, name)
+            _check(t.dtype == dtype and t.dim() == 2 and t.size(0) == rows, f"{name} must be {str(dtype)[6:]} [rows, k]")
+            _check(t.device == device, "all tensors must be on the same device")
+            _check(top in (0, t.size(1)), "top_ids and top_logprobs must have the same shape")
+            top = t.size(1)
+            _check(1 <= top <= min(64, vocab), "1 <= k <= 64, k <= vocabulary")
+    if rows == 0:
+        return 0.0
+    ms = ctypes.c_float(0.0)
+    with torch.cuda.device(device):
+        rc = library().rptc_token_logprobs(logits.data_ptr(), _DTYPES[logits.dtype], None if tokens is None else tokens.data_ptr(),
+                                           None if logprob is None else logprob.data_ptr(), None if entropy is None else entropy.data_ptr(),
+                                           None if top_ids is None else top_ids.data_ptr(),
+                                           None if top_logprobs is None else top_logprobs.data_ptr(), rows, vocab,
+                                           logits.stride(0) if rows > 1 else vocab, top, torch.cuda.current_stream().cuda_stream,
+                                           ctypes.byref(ms) if (_timing if timed is None else timed) else None)
     _status(rc)
     return float(ms.value)
