@@ -410,7 +410,8 @@ int64_t rptc_lite_viterbi_scratch_bytes(int L, int R, int64_t rows, int64_t step
  *   all key rows.  max_k an upper bound of k_len (total_k will do:
  *   it only decides how far the keys of a call with few rows are split)
  *   workspace  rptc_attn_prompt_workspace_bytes(...) bytes of device memory, 16-byte aligned (0: may be NULL); no
- *              initialisation, calls that may overlap need one each.  At most 2^24 query rows, 1024 heads, 2^20 sequences.
+ *              initialisation, calls that may overlap need one each.  At most 2^24 query rows, 1024 heads, 2^20 sequences,
+ *              (total_q / 128 + seqs) * heads below 2^23.
  */
 typedef struct rptc_prompt_strides {
     int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
@@ -443,7 +444,7 @@ int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint16_t *v, ui
  *                         contiguous.  A sequence whose position lies outside [0, max_len) (a padded batch) is left unwritten.
  *                         workspace: rptc_kv4_attn_decode_workspace_bytes(...) bytes, 16-byte aligned (0: may be NULL),
  *                         no initialisation; calls that may overlap need one each.
- * At most 65535 sequences, 1024 heads, 2^30 - 1 positions; q_out, out and the caches must not overlap the inputs.
+ * At most 65535 sequences, 1024 heads, 2^26 positions; q_out, out and the caches must not overlap the inputs.
  */
 int64_t rptc_kv4_row_bytes(int64_t hd);
 int rptc_kv4_append(const uint16_t *k, const uint16_t *v, uint8_t *k_cache, uint8_t *v_cache, const int64_t *pos,
@@ -454,7 +455,7 @@ int rptc_kv4_read(const uint8_t *k_cache, const uint8_t *v_cache, uint16_t *k, u
                   int64_t v_head, void *stream, float *ms);
 int rptc_kv4_rope_append(const uint16_t *qkv, const uint16_t *cos_t, const uint16_t *sin_t, const int64_t *pos, uint16_t *q_out,
                          uint8_t *k_cache, uint8_t *v_cache, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t hd,
-                         int64_t max_len, void *stream);
+                         int64_t max_len, void *stream, float *ms);
 int64_t rptc_kv4_attn_decode_workspace_bytes(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t hd, int64_t max_len);
 int rptc_kv4_attn_decode(const uint16_t *q, const uint8_t *k_cache, const uint8_t *v_cache, const int64_t *pos, uint16_t *out,
                          int64_t seqs, int64_t heads, int64_t kv_heads, int64_t hd, int64_t max_len, int64_t q_token, float scale,

@@ -14,7 +14,7 @@
 // layout is, up to a renumbering of the keys that V follows, the layout the second product wants P in, and every
 // factor of a row is a factor of a lane.  K and V come from memory straight into LDS (two buffers, 16 bytes a lane);
 // V^T is read with the transposing LDS read.
-#include "rptc_common.hpp"
+#include "join.hpp"
 
 namespace rptc {
 
@@ -63,7 +63,7 @@ struct PromptArgs {
     uint16_t *out;
     float *lse;                        // [total_q][heads], may be null
     const int32_t *q_start, *k_start, *k_len;
-    float *part_acc, *part_ml;         // splits > 1: [split][total_q][heads][hd] sums, [..][2] bound and sum of p
+    float *part_acc, *part_ml;         // splits > 1: [total_q][heads][split][hd] sums, [..][2] bound and sum of p
     rptc_prompt_strides st;
     int seqs, total_q, total_k, heads, kv_heads, tiles, splits, causal;
     float c;                           // scale * log2(e)
@@ -209,7 +209,7 @@ __device__ __forceinline__ void prompt_rows_plain(const PromptArgs &a, const Pro
         for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
         const int64_t at = (int64_t)row * a.heads + head;
         if (a.splits > 1) {
-            const int64_t pa = (int64_t)split * a.total_q * a.heads + at;
+            const int64_t pa = at * a.splits + split;
             for (int u = 0; u < kOut; u++)
                 if (lane + 64 * u < HD) a.part_acc[pa * HD + lane + 64 * u] = acc[u];
             if (lane == 0) {
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
     const int64_t at = (int64_t)row * a.heads + head;
     if (a.splits > 1) {
         if (row >= t.q_end) return;
-        const int64_t pa = (int64_t)split * a.total_q * a.heads + at;
+        const int64_t pa = at * a.splits + split;
         float *o = a.part_acc + pa * HD + 4 * c;
 #pragma unroll
         for (int d = 0; d < kDims; d++)
@@ -422,41 +422,24 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
     if (a.lse && c == 0 && row < t.q_end) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
 }
 
-// Joins the splits of a row: o = sum_i acc_i 2^(m_i - M) / sum_i l_i 2^(m_i - M), a wave per (row, head), in split order.
-// The rows are found as the kernel above found them (rows of no sequence have no partial results and stay as they are).
-constexpr int kMergeRows = 4;
-
+// Joins the pieces of a row, a workgroup per (row, head).  The rows are found as the kernel above found them: rows of no
+// sequence have no pieces and stay as they are.
 template <int HD, class T>
-__global__ __launch_bounds__(256) void attn_prompt_merge_kernel(const PromptArgs a)
+__global__ __launch_bounds__(kJoinThreads) void attn_prompt_merge_kernel(const PromptArgs a)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int head = blockIdx.y;
-    const int tile = blockIdx.x / (kRows / kMergeRows), part = blockIdx.x % (kRows / kMergeRows);
     PromptTile t;
-    if (!find_tile(a, tile, t)) return;
+    if (!find_tile(a, blockIdx.x / kRows, t)) return;
     int ks, lk;
     if (!find_keys(a, t, ks, lk)) return;
-    const int row = t.row0 + part * kMergeRows + wave;
+    const int row = t.row0 + blockIdx.x % kRows;
     if (row >= t.q_end) return;
-    const int64_t at = (int64_t)row * a.heads + head, step = (int64_t)a.total_q * a.heads;
-    float m = -INFINITY;
-    for (int i = 0; i < a.splits; i++) m = fmaxf(m, a.part_ml[2 * (at + i * step)]);
-    constexpr int kOut = (HD + 63) / 64;
-    float l = 0.f, acc[kOut];
-    for (int u = 0; u < kOut; u++) acc[u] = 0.f;
-    for (int i = 0; i < a.splits; i++) {
-        const int64_t pa = at + i * step;
-        const float mi = a.part_ml[2 * pa], li = a.part_ml[2 * pa + 1];
-        const float f = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - m);
-        if (li == 0.f) continue;                           // the split holds no key of the row
-        l = fmaf(li, f, l);
-        for (int u = 0; u < kOut; u++)
-            if (lane + 64 * u < HD) acc[u] = fmaf(a.part_acc[pa * HD + lane + 64 * u], f, acc[u]);
-    }
-    uint16_t *o = a.out + (int64_t)row * a.st.out_token + (int64_t)head * a.st.out_head;
-    for (int u = 0; u < kOut; u++)
-        if (lane + 64 * u < HD) o[lane + 64 * u] = (uint16_t)T::pack(l == 0.f ? 0.f : acc[u] / l, 0.f);
-    if (a.lse && lane == 0) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
+    const int64_t at = (int64_t)row * a.heads + head;
+    float M, l;
+    const float num = join_pieces(a.part_acc + at * a.splits * HD, a.part_ml + 2 * at * a.splits, a.splits, HD, M, l);
+    if (threadIdx.x < HD)
+        a.out[(int64_t)row * a.st.out_token + (int64_t)head * a.st.out_head + threadIdx.x] = (uint16_t)T::pack(l == 0.f ? 0.f : num / l, 0.f);
+    if (a.lse && threadIdx.x == 0) a.lse[at] = l == 0.f ? -INFINITY : (M + log2f(l)) * 0.693147180559945f;
 }
 
 template <int HD>
@@ -488,7 +471,7 @@ static int prompt_sizes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t 
     if (seqs < 1 || total_q < 1 || total_k < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0) return RPTC_ESHAPE;
     if (hd != 32 && hd != 64 && hd != 128 && hd != 256) return RPTC_ESHAPE;
     if (heads > 1024 || seqs > (1 << 20) || total_q > (1 << 24) || total_k >= ((int64_t)1 << 31) - 64) return RPTC_ELIMIT;
-    if ((total_q / kRows + seqs) * heads >= (int64_t)1 << 30) return RPTC_ELIMIT;
+    if ((total_q / kRows + seqs) * heads >= (int64_t)1 << 23) return RPTC_ELIMIT;      // workgroups of one launch
     return 0;
 }
 
@@ -498,7 +481,7 @@ static void launch_prompt(const PromptArgs &a, hipStream_t s)
     const int items = a.heads * a.tiles * a.splits;
     hipLaunchKernelGGL((attn_prompt_kernel<HD, T>), dim3((unsigned)((items + 7) / 8 * 8)), dim3(kPromptThreads), prompt_lds<HD>(), s, a);
     if (a.splits > 1)
-        hipLaunchKernelGGL((attn_prompt_merge_kernel<HD, T>), dim3((unsigned)(a.tiles * (kRows / kMergeRows)), (unsigned)a.heads), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((attn_prompt_merge_kernel<HD, T>), dim3((unsigned)a.tiles * kRows, (unsigned)a.heads), dim3(kJoinThreads), 0, s, a);
 }
 
 }  // namespace rptc

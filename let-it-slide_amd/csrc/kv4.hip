@@ -8,7 +8,7 @@
 // hd / 2 bytes of codes, then s and m of every group: hd / 2 + hd / 8 bytes, 80 against 256 at hd = 128.  Word w of a row
 // holds the values 8w .. 8w+7, nibble t the value 8w + 2t and nibble t + 4 the value 8w + 2t + 1: one mask of a word gives a
 // pair of neighbours in the two halves of a register.
-#include "rptc_common.hpp"
+#include "join.hpp"
 
 namespace rptc {
 
@@ -95,7 +95,7 @@ struct Kv4AppendArgs {
     uint8_t *k_cache, *v_cache;
     const int64_t *pos;
     const int32_t *q_start;                // may be null: rows_each rows a sequence
-    int64_t k_token, k_head, v_token, v_head, items, max_len;
+    int64_t k_token, k_head, v_token, v_head, max_len;
     int seqs, total, rows_each, kv_heads;
 };
 
@@ -105,14 +105,10 @@ template <int HD>
 __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4AppendArgs a)
 {
     constexpr int kWords = HD / 8;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= a.items) return;             // (whole rows: items is a multiple of kWords, 4 at least)
-    const int word = (int)(id % kWords);
-    int64_t rest = id / kWords;
-    const int token = (int)(rest % a.total);
-    rest /= a.total;
-    const int head = (int)(rest % a.kv_heads);
-    const bool is_v = rest >= a.kv_heads;
+    const int word = threadIdx.x % kWords, token = blockIdx.x * (256 / kWords) + threadIdx.x / kWords;
+    if (token >= a.total) return;          // (whole rows: the lanes of a group stay together)
+    const bool is_v = blockIdx.y >= a.kv_heads;
+    const int head = blockIdx.y - (is_v ? a.kv_heads : 0);
     int seq, start;
     if (a.q_start) {
         // the last sequence that starts at or in front of the token
@@ -154,24 +150,18 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4AppendArgs a)
 struct Kv4ReadArgs {
     const uint8_t *k_cache, *v_cache;
     uint16_t *k, *v;
-    int64_t k_token, k_head, v_token, v_head, items, max_len;
-    int rows, kv_heads, seqs;
+    int64_t k_token, k_head, v_token, v_head, max_len;
+    int rows, kv_heads;
 };
 
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4ReadArgs a)
 {
     constexpr int kWords = HD / 8;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= a.items) return;
-    const int word = (int)(id % kWords);
-    int64_t rest = id / kWords;
-    const int p = (int)(rest % a.rows);
-    rest /= a.rows;
-    const int head = (int)(rest % a.kv_heads);
-    rest /= a.kv_heads;
-    const bool is_v = rest >= a.seqs;
-    const int seq = (int)(is_v ? rest - a.seqs : rest);
+    const int word = threadIdx.x % kWords, p = blockIdx.x * (256 / kWords) + threadIdx.x / kWords;
+    if (p >= a.rows) return;
+    const bool is_v = blockIdx.y >= a.kv_heads;
+    const int head = blockIdx.y - (is_v ? a.kv_heads : 0), seq = blockIdx.z;
     const uint8_t *row = (is_v ? a.v_cache : a.k_cache) + (((int64_t)seq * a.kv_heads + head) * a.max_len + p) * kv4_row_bytes(HD);
     const uint32_t code = *reinterpret_cast<const uint32_t *>(row + 4 * word);
     const uint32_t par = *reinterpret_cast<const uint32_t *>(row + HD / 2 + word / 4 * 4);
@@ -426,28 +416,16 @@ __global__ __launch_bounds__(64 * kKv4Waves) void kv4_attn_kernel(const Kv4AttnA
     }
 }
 
-// Joins the pieces of a head, in order, a wave per (sequence, head).
-__global__ __launch_bounds__(64) void kv4_merge_kernel(const float *__restrict__ part, int64_t part_ml, const int64_t *__restrict__ pos,
-                                                       uint16_t *__restrict__ out, int heads, int hd, int splits, int64_t max_len)
+// Joins the pieces of a head, a workgroup per (sequence, head).
+__global__ __launch_bounds__(kJoinThreads) void kv4_merge_kernel(const float *__restrict__ part, int64_t part_ml, const int64_t *__restrict__ pos,
+                                                                 uint16_t *__restrict__ out, int heads, int hd, int splits, int64_t max_len)
 {
-    const int lane = threadIdx.x, head = blockIdx.x, seq = blockIdx.y;
+    const int head = blockIdx.x, seq = blockIdx.y;
     if (pos[seq] < 0 || pos[seq] >= max_len) return;
     const int64_t at = (int64_t)seq * heads + head;
-    const float *ml = part + part_ml + 2 * at * splits;
-    float M = -INFINITY;
-    for (int i = 0; i < splits; i++) M = fmaxf(M, ml[2 * i]);
-    float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
-    for (int i = 0; i < splits; i++) {
-        if (ml[2 * i + 1] == 0.f) continue;                // an empty piece
-        const float f = ml[2 * i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[2 * i] - M);
-        den = fmaf(ml[2 * i + 1], f, den);
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-            if (lane + 64 * u < hd) num[u] = fmaf(part[(at * splits + i) * hd + lane + 64 * u], f, num[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < 4; u++)
-        if (lane + 64 * u < hd) out[at * hd + lane + 64 * u] = float_to_half_bits(num[u] / den);
+    float M, den;
+    const float num = join_pieces(part + at * splits * hd, part + part_ml + 2 * at * splits, splits, hd, M, den);
+    if (threadIdx.x < hd) out[at * hd + threadIdx.x] = float_to_half_bits(num / den);
 }
 
 template <int HD>
@@ -464,7 +442,7 @@ static int kv4_sizes(int64_t seqs, int64_t kv_heads, int64_t hd, int64_t max_len
 {
     if (seqs < 1 || kv_heads < 1 || max_len < 1) return RPTC_ESHAPE;
     if (hd != 32 && hd != 64 && hd != 128 && hd != 256) return RPTC_ESHAPE;
-    if (seqs > 65535 || kv_heads > 1024 || max_len >= (int64_t)1 << 30) return RPTC_ELIMIT;
+    if (seqs > 65535 || kv_heads > 1024 || max_len > (int64_t)1 << 26) return RPTC_ELIMIT;
     return 0;
 }
 
@@ -506,22 +484,21 @@ extern "C" int rptc_kv4_append(const uint16_t *k, const uint16_t *v, uint8_t *k_
     a.k_head = k_head;
     a.v_token = v_token;
     a.v_head = v_head;
-    a.items = 2 * total * kv_heads * (hd / 8);
     a.max_len = max_len;
     a.seqs = (int)seqs;
     a.total = (int)total;
     a.rows_each = (int)(total / seqs);
     a.kv_heads = (int)kv_heads;
-    const int64_t blocks = (a.items + 255) / 256;
-    if (blocks >= (int64_t)1 << 31) return RPTC_ELIMIT;
+    const int per = 256 / (int)(hd / 8);       // rows of a workgroup
+    const dim3 grid((unsigned)((total + per - 1) / per), (unsigned)(2 * kv_heads));
     hipStream_t s = static_cast<hipStream_t>(stream);
     Timer timer;
     if ((rc = timer.begin(dev, s, ms))) return rc;
     switch (hd) {
-    case 32: hipLaunchKernelGGL(kv4_append_kernel<32>, dim3((unsigned)blocks), dim3(256), 0, s, a); break;
-    case 64: hipLaunchKernelGGL(kv4_append_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, s, a); break;
-    case 128: hipLaunchKernelGGL(kv4_append_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL(kv4_append_kernel<256>, dim3((unsigned)blocks), dim3(256), 0, s, a); break;
+    case 32: hipLaunchKernelGGL(kv4_append_kernel<32>, grid, dim3(256), 0, s, a); break;
+    case 64: hipLaunchKernelGGL(kv4_append_kernel<64>, grid, dim3(256), 0, s, a); break;
+    case 128: hipLaunchKernelGGL(kv4_append_kernel<128>, grid, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL(kv4_append_kernel<256>, grid, dim3(256), 0, s, a); break;
     }
     return timer.end();
 }
@@ -547,28 +524,26 @@ extern "C" int rptc_kv4_read(const uint8_t *k_cache, const uint8_t *v_cache, uin
     a.k_head = k_head;
     a.v_token = v_token;
     a.v_head = v_head;
-    a.items = 2 * seqs * rows * kv_heads * (hd / 8);
     a.max_len = max_len;
     a.rows = (int)rows;
     a.kv_heads = (int)kv_heads;
-    a.seqs = (int)seqs;
-    const int64_t blocks = (a.items + 255) / 256;
-    if (blocks >= (int64_t)1 << 31) return RPTC_ELIMIT;
+    const int per = 256 / (int)(hd / 8);       // rows of a workgroup
+    const dim3 grid((unsigned)((rows + per - 1) / per), (unsigned)(2 * kv_heads), (unsigned)seqs);
     hipStream_t s = static_cast<hipStream_t>(stream);
     Timer timer;
     if ((rc = timer.begin(dev, s, ms))) return rc;
     switch (hd) {
-    case 32: hipLaunchKernelGGL(kv4_read_kernel<32>, dim3((unsigned)blocks), dim3(256), 0, s, a); break;
-    case 64: hipLaunchKernelGGL(kv4_read_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, s, a); break;
-    case 128: hipLaunchKernelGGL(kv4_read_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL(kv4_read_kernel<256>, dim3((unsigned)blocks), dim3(256), 0, s, a); break;
+    case 32: hipLaunchKernelGGL(kv4_read_kernel<32>, grid, dim3(256), 0, s, a); break;
+    case 64: hipLaunchKernelGGL(kv4_read_kernel<64>, grid, dim3(256), 0, s, a); break;
+    case 128: hipLaunchKernelGGL(kv4_read_kernel<128>, grid, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL(kv4_read_kernel<256>, grid, dim3(256), 0, s, a); break;
     }
     return timer.end();
 }
 
 extern "C" int rptc_kv4_rope_append(const uint16_t *qkv, const uint16_t *cos_t, const uint16_t *sin_t, const int64_t *pos,
                                     uint16_t *q_out, uint8_t *k_cache, uint8_t *v_cache, int64_t seqs, int64_t heads, int64_t kv_heads,
-                                    int64_t hd, int64_t max_len, void *stream)
+                                    int64_t hd, int64_t max_len, void *stream, float *ms)
 {
     if (!qkv || !cos_t || !sin_t || !pos || !q_out || !k_cache || !v_cache) return RPTC_ENULL;
     int rc = kv4_sizes(seqs, kv_heads, hd, max_len);
@@ -580,10 +555,12 @@ extern "C" int rptc_kv4_rope_append(const uint16_t *qkv, const uint16_t *cos_t, 
     DeviceInfo *dev;
     if ((rc = device_info(&dev))) return rc;
     const int items = (int)((heads + 2 * kv_heads) * (hd / 8));
-    hipLaunchKernelGGL(kv4_rope_append_kernel, dim3((unsigned)((items + 255) / 256), (unsigned)seqs), dim3(256), 0,
-                       static_cast<hipStream_t>(stream), qkv, cos_t, sin_t, pos, q_out, k_cache, v_cache, (int)heads, (int)kv_heads, (int)hd,
-                       max_len, items);
-    return (int)hipGetLastError();
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    Timer timer;
+    if ((rc = timer.begin(dev, s, ms))) return rc;
+    hipLaunchKernelGGL(kv4_rope_append_kernel, dim3((unsigned)((items + 255) / 256), (unsigned)seqs), dim3(256), 0, s, qkv, cos_t, sin_t, pos,
+                       q_out, k_cache, v_cache, (int)heads, (int)kv_heads, (int)hd, max_len, items);
+    return timer.end();
 }
 
 extern "C" int64_t rptc_kv4_attn_decode_workspace_bytes(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t hd, int64_t max_len)
@@ -651,7 +628,7 @@ extern "C" int rptc_kv4_attn_decode(const uint16_t *q, const uint8_t *k_cache, c
     default: launch_kv4_attn<256>(a, (int)seqs, s); break;
     }
     if (a.splits > 1)
-        hipLaunchKernelGGL(kv4_merge_kernel, dim3((unsigned)heads, (unsigned)seqs), dim3(64), 0, s, a.part, a.part_ml, pos, out, (int)heads,
+        hipLaunchKernelGGL(kv4_merge_kernel, dim3((unsigned)heads, (unsigned)seqs), dim3(kJoinThreads), 0, s, a.part, a.part_ml, pos, out, (int)heads,
                            (int)hd, a.splits, max_len);
     return timer.end();
 }

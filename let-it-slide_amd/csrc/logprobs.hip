@@ -8,18 +8,21 @@
 // thread's own, then over the workgroup in a fixed order.  A logit of -inf has probability 0 and adds nothing; +inf or a not-a-number makes
 // the row's results not-a-number, and so does a row of -inf only, as a log-softmax does.
 //
-// The k most likely tokens need no second pass over the row: the k-th largest of 64 maxima (of 64 groups of threads) is a
-// bound that at least k logits reach; only threads whose own maximum reaches it look at their logits again, what
-// reaches it goes to a list (as value and id in one 64-bit key, so equal values order by the lowest id), and an entry's
-// rank in the list is its place.  Where more logits reach the bound than the list holds (ties by the hundred, a row with
+// The k most likely tokens need no second pass over the row: the k-th largest of 64 maxima (of the threads of a lane number) is a
+// bound that at least k logits reach.  Every thread leaves the maxima of up to eight stretches of its logits in LDS;
+// stretches that reach the bound (about as many as there are alternatives) are dealt out, one a thread, and read again; what
+// reaches the bound there goes to a list (as value and id in one 64-bit key, so equal values order by the lowest id), and an
+// entry's rank in the list is its place.  Where more logits reach the bound than the list holds (ties by the hundred, a row with
 // nearly everything masked) the workgroup looks for one maximum after the other instead.
 #include "rptc_common.hpp"
 
 namespace rptc {
 
-constexpr int kScoreThreads = 1024;
+constexpr int kScoreThreads = 512;
 constexpr int kScoreGroups = 64;
 constexpr int kScoreList = 1024;
+constexpr int kScoreUnits = 8;             // stretches of a thread's logits
+constexpr int kScoreLoads = 4;             // 16-byte loads of a thread in flight
 constexpr float kLog2E = 1.44269504088896f, kLn2 = 0.693147180559945f;
 
 struct ScoreF16 {
@@ -91,12 +94,13 @@ template <class T>
 __global__ __launch_bounds__(kScoreThreads) void token_logprobs_kernel(const ScoreArgs a)
 {
     typedef typename T::elem elem;
-    constexpr int kEach = T::kEach, kLoads = 4, kWaves = kScoreThreads / 64;
-    __shared__ float s_m[kWaves], s_l[kWaves], s_t[kWaves], s_group[kScoreGroups];
+    constexpr int kEach = T::kEach, kLoads = kScoreLoads, kWaves = kScoreThreads / 64;
+    __shared__ float s_m[kWaves], s_l[kWaves], s_t[kWaves], s_big[kScoreThreads];
     __shared__ uint64_t s_list[kScoreList];
     __shared__ uint64_t s_best[kWaves];
-    __shared__ int s_count;
-    __shared__ float s_bound;
+    __shared__ float s_unit[kScoreUnits * kScoreThreads];
+    __shared__ uint16_t s_found[kScoreList];
+    __shared__ int s_count, s_found_count;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x;
     const elem *x = static_cast<const elem *>(a.logits) + row * a.row_stride;
@@ -144,7 +148,11 @@ __global__ __launch_bounds__(kScoreThreads) void token_logprobs_kernel(const Sco
         raise(v);
         add(v, big == -INFINITY ? 0.f : big);
     }
-    for (int v0 = tid; v0 < vecs; v0 += kScoreThreads * kLoads) {
+    const int rounds = (vecs + kScoreThreads * kLoads - 1) / (kScoreThreads * kLoads);
+    const int per_unit = (rounds + kScoreUnits - 1) / kScoreUnits;        // rounds of a stretch
+    float unit_max = -INFINITY;
+    for (int r = 0, in_unit = 0, unit = tid; r < rounds; r++) {
+        const int v0 = r * kScoreThreads * kLoads + tid;
         uint4 raw[kLoads];
 #pragma unroll
         for (int u = 0; u < kLoads; u++) {
@@ -159,9 +167,16 @@ __global__ __launch_bounds__(kScoreThreads) void token_logprobs_kernel(const Sco
 #pragma unroll
             for (int i = 1; i < kEach; i++) mx = fmaxf(mx, e[i]);
             raise(mx);
+            unit_max = fmaxf(unit_max, mx);
             const float base = big == -INFINITY ? 0.f : big;
 #pragma unroll
             for (int i = 0; i < kEach; i++) add(e[i], base);
+        }
+        if (++in_unit == per_unit || r == rounds - 1) {
+            s_unit[unit] = unit_max;
+            unit += kScoreThreads;
+            unit_max = -INFINITY;
+            in_unit = 0;
         }
     }
 
@@ -175,16 +190,13 @@ __global__ __launch_bounds__(kScoreThreads) void token_logprobs_kernel(const Sco
         l += __shfl_xor(l, off, 64);
         t += __shfl_xor(t, off, 64);
     }
-    float g = big;                             // largest logit of the 16 threads of a group
-#pragma unroll
-    for (int off = 1; off < kScoreThreads / kScoreGroups; off <<= 1) g = fmaxf(g, __shfl_xor(g, off, 64));
     if (lane == 0) {
         s_m[wave] = M;
         s_l[wave] = l;
         s_t[wave] = t;
     }
-    if (tid % (kScoreThreads / kScoreGroups) == 0) s_group[tid / (kScoreThreads / kScoreGroups)] = g;
-    if (tid == 0) s_count = 0;
+    s_big[tid] = big;
+    if (tid == 0) s_count = s_found_count = 0;
     __syncthreads();
     M = s_m[0];
 #pragma unroll
@@ -208,18 +220,72 @@ __global__ __launch_bounds__(kScoreThreads) void token_logprobs_kernel(const Sco
     }
     if (a.top == 0) return;
 
-    if (wave == 0) {
-        // the top-th largest of the 64 maxima: the one with top - 1 in front of it (equal ones in lane order)
-        const float own = s_group[lane];
-        int front = 0;
-        for (int i = 0; i < 64; i++) {
-            const float o = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, own), i));
-            front += o > own || (o == own && i < lane);
+    // the top-th largest of the 64 maxima, in every wave: the one with top - 1 in front of it (equal ones in lane order)
+    float own = s_big[lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) own = fmaxf(own, s_big[w * 64 + lane]);
+    int front = 0;
+#pragma unroll
+    for (int i = 0; i < kScoreGroups; i++) {
+        const float o = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, own), i));
+        front += o > own || (o == own && i < lane);
+    }
+    const float bound = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, own), __builtin_ctzll(__ballot(front == a.top - 1))));
+    // a bound of -inf says nothing (fewer lane numbers than wanted hold a logit above it): a row no longer than the list then
+    // goes there whole, a longer one is searched below
+    const bool all = bound == -INFINITY && a.vocab <= kScoreList;
+    const bool listed = all || bound != -INFINITY;
+    auto take = [&](float v, int id) {
+        if (v >= bound || all) {
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kScoreList) s_list[at] = score_key(v, (uint32_t)id);
         }
-        if (front == a.top - 1) s_bound = own;
+    };
+    const int units = per_unit ? (rounds + per_unit - 1) / per_unit : 0;
+    if (listed && (big >= bound || all)) {
+        for (int i = tid; i < head; i += kScoreThreads) take(T::one(x[i]), i);
+        for (int i = tail + tid; i < a.vocab; i += kScoreThreads) take(T::one(x[i]), i);
+        for (int n = 0; n < units; n++)
+            if (s_unit[n * kScoreThreads + tid] >= bound || all) {
+                const int at = atomicAdd(&s_found_count, 1);
+                if (at < kScoreList) s_found[at] = (uint16_t)(n * kScoreThreads + tid);
+            }
     }
     __syncthreads();
-    const float bound = s_bound;
+    const int found = s_found_count;
+    if (found <= kScoreList)
+        for (int j = tid; j < found; j += kScoreThreads) {
+            const int n = s_found[j] / kScoreThreads, owner = s_found[j] % kScoreThreads;
+            for (int r = n * per_unit; r < min(rounds, (n + 1) * per_unit); r++) {
+                const int v0 = r * kScoreThreads * kLoads + owner;
+                uint4 raw[kLoads];
+#pragma unroll
+                for (int u = 0; u < kLoads; u++) raw[u] = xv[min(v0 + u * kScoreThreads, vecs - 1)];
+#pragma unroll
+                for (int u = 0; u < kLoads; u++) {
+                    const int v = v0 + u * kScoreThreads;
+                    if (v >= vecs) break;
+                    float e[kEach];
+                    T::unpack(raw[u], e);
+#pragma unroll
+                    for (int i = 0; i < kEach; i++) take(e[i], head + v * kEach + i);
+                }
+            }
+        }
+    __syncthreads();
+    const int count = s_count;
+    if (listed && found <= kScoreList && count <= kScoreList) {
+        for (int j = tid; j < count; j += kScoreThreads) {
+            const uint64_t key = s_list[j];
+            int rank = 0;
+            for (int i = 0; i < count; i++) rank += s_list[i] > key;
+            if (rank < a.top) {
+                if (a.top_ids) a.top_ids[row * a.top + rank] = 0xFFFFFFFFu - (uint32_t)key;
+                if (a.top_logprobs) a.top_logprobs[row * a.top + rank] = logp(score_value(key));
+            }
+        }
+        return;
+    }
     auto each = [&](auto f) {                  // the thread's logits with their ids
         for (int i = tid; i < head; i += kScoreThreads) f(T::one(x[i]), i);
         for (int i = tail + tid; i < a.vocab; i += kScoreThreads) f(T::one(x[i]), i);
@@ -230,28 +296,6 @@ __global__ __launch_bounds__(kScoreThreads) void token_logprobs_kernel(const Sco
             for (int i = 0; i < kEach; i++) f(e[i], head + v * kEach + i);
         }
     };
-    // (a bound of -inf says nothing: fewer groups than wanted hold a logit above it)
-    if (bound != -INFINITY && big >= bound)
-        each([&](float v, int id) {
-            if (v >= bound) {
-                const int at = atomicAdd(&s_count, 1);
-                if (at < kScoreList) s_list[at] = score_key(v, (uint32_t)id);
-            }
-        });
-    __syncthreads();
-    const int count = s_count;
-    if (bound != -INFINITY && count <= kScoreList) {
-        if (tid < count) {
-            const uint64_t key = s_list[tid];
-            int rank = 0;
-            for (int i = 0; i < count; i++) rank += s_list[i] > key;
-            if (rank < a.top) {
-                if (a.top_ids) a.top_ids[row * a.top + rank] = 0xFFFFFFFFu - (uint32_t)key;
-                if (a.top_logprobs) a.top_logprobs[row * a.top + rank] = logp(score_value(key));
-            }
-        }
-        return;
-    }
     // one after the other: the largest key below the last one taken
     uint64_t last = ~0ull;
     for (int r = 0; r < a.top; r++) {
@@ -293,7 +337,7 @@ extern "C" int rptc_token_logprobs(const void *logits, int dtype, const int64_t 
     if (dtype != RPTC_F16 && dtype != RPTC_BF16 && dtype != RPTC_F32) return RPTC_EMODE;
     if (rows < 1 || vocab < 1 || row_stride < 0 || top < 0 || top > vocab) return RPTC_ESHAPE;
     if ((top > 0) != (top_ids || top_logprobs)) return RPTC_ESHAPE;
-    if (rows >= (int64_t)1 << 31 || vocab >= (int64_t)1 << 30 || top > kScoreGroups) return RPTC_ELIMIT;
+    if (rows >= (int64_t)1 << 22 || vocab >= (int64_t)1 << 30 || top > kScoreGroups) return RPTC_ELIMIT;
     if (reinterpret_cast<uintptr_t>(logits) % (dtype == RPTC_F32 ? 4 : 2) != 0) return RPTC_EALIGN;
     DeviceInfo *dev;
     int rc = device_info(&dev);

@@ -119,7 +119,7 @@ _SIGNATURES = {
     "rptc_kv4_row_bytes": ([_I64], _I64),
     "rptc_kv4_append": ([_VP] * 6 + [_I64] * 9 + [_VP, _FP], _INT),
     "rptc_kv4_read": ([_VP] * 4 + [_I64] * 9 + [_VP, _FP], _INT),
-    "rptc_kv4_rope_append": ([_VP] * 7 + [_I64] * 5 + [_VP], _INT),
+    "rptc_kv4_rope_append": ([_VP] * 7 + [_I64] * 5 + [_VP, _FP], _INT),
     "rptc_kv4_attn_decode_workspace_bytes": ([_I64] * 5, _I64),
     "rptc_kv4_attn_decode": ([_VP] * 5 + [_I64] * 6 + [ctypes.c_float, _VP, _I64, _VP, _FP], _INT),
     "rptc_token_logprobs": ([_VP, _INT] + [_VP] * 5 + [_I64] * 4 + [_VP, _FP], _INT),
@@ -817,31 +817,79 @@ def matvec_bits_dense(compressed, codebook, out, bits):
 
 
 # ---------------------------------------------------------------- prompts, the 4-bit cache, scoring
+# These ops run between the launches of a decode loop, so their checks are plain comparisons whose messages are put together
+# only when one fails.
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}      # RPTC_F16, RPTC_BF16, RPTC_F32
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _check_rows(t, name, dtype):
+def _refuse(msg):
+    raise RuntimeError(msg)
+
+
+def _run_on(device, timed, fn, *args):
+    """fn(*args, stream, ms) on the device's current stream; elapsed ms (0.0 when not timed)."""
+    index = device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(device):
+            return _run_on(device, timed, fn, *args)
+    if _timing if timed is None else timed:
+        ms = ctypes.c_float(0.0)
+        rc = fn(*args, _raw_stream(index), ctypes.byref(ms))
+        if rc:
+            _status(rc)
+        return float(ms.value)
+    rc = fn(*args, _raw_stream(index), None)
+    if rc:
+        _status(rc)
+    return 0.0
+
+
+def _workspace(device, fn, *sizes):
+    """(tensor or None, bytes) for an op's workspace.  From torch's allocator, so it is this call's own on the current
+    stream and in a graph being captured."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _workspace(device, fn, *sizes)
+    need = fn(*sizes)
+    if need < 0:
+        _status(int(need))
+    return (torch.empty(need, dtype=torch.uint8, device=device), need) if need else (None, 0)
+
+
+def _rows_ok(t, name, dtype, device):
     # [tokens, heads, hd], any token and head strides, the head dimension contiguous
-    _check(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
-    _check(t.is_cuda, f"{name} must be a CUDA tensor")
-    _check(t.dim() == 3, f"{name}.dim() == 3 ([tokens, heads, head_dim])")
-    _check(t.dtype == dtype, f"{name} must have the type of q")
-    _check(t.stride(2) == 1, f"{name} must be contiguous along the head dimension")
-
-
-def _strides(t):
-    # the stride of a dimension of one element means nothing: any valid one will do
+    if not isinstance(t, torch.Tensor):
+        _refuse(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        _refuse(f"{name} must be a CUDA tensor")
+    if t.dim() != 3:
+        _refuse(f"{name}.dim() == 3 ([tokens, heads, head_dim])")
+    if t.dtype != dtype:
+        _refuse(f"{name} must be {str(dtype)[6:]}")
+    if t.device != device:
+        _refuse("all tensors must be on the same device")
+    a, b, c = t.stride()
+    if c != 1:
+        _refuse(f"{name} must be contiguous along the head dimension")
     n, h, hd = t.shape
-    a, b, _ = t.stride()
+    # the stride of a dimension of one element means nothing: any valid one will do
     return a if n > 1 else hd, b if h > 1 else hd
 
 
-def _check_index(t, name, dtype, count, device):
-    _check_input(t, name)
-    _check(t.dtype == dtype and t.dim() == 1, f"{name} must be a 1-D {str(dtype)[6:]} tensor")
-    _check(t.size(0) == count, f"{name}.size(0) == {count}")
-    _check(t.device == device, "all tensors must be on the same device")
+def _vector_ok(t, name, dtype, count, device):
+    if not isinstance(t, torch.Tensor):
+        _refuse(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        _refuse(f"{name} must be a CUDA tensor")
+    if t.dtype != dtype or t.dim() != 1 or t.size(0) != count:
+        _refuse(f"{name} must be a 1-D {str(dtype)[6:]} tensor of {count} elements")
+    if not t.is_contiguous():
+        _refuse(f"{name} must be contiguous")
+    if t.device != device:
+        _refuse("all tensors must be on the same device")
+    return t.data_ptr()
 
 
 def attn_prompt(q, k, v, out, q_start=None, k_start=None, k_len=None, causal=True, scale=None, lse=None, max_k=None, timed=None):
@@ -855,56 +903,55 @@ def attn_prompt(q, k, v, out, q_start=None, k_start=None, k_len=None, causal=Tru
     chunk's last query sees the whole context.  ``scale`` defaults to hd ** -0.5.  ``lse`` (float32 [Tq, heads], optional)
     takes the logarithm of every row's sum.  A query that sees no key gets 0 (lse -inf); rows outside every sequence stay as
     they are.  ``max_k``: an upper bound of k_len where the key rows are many more (a cache's positions).  Returns elapsed ms."""
-    _check(isinstance(q, torch.Tensor) and q.dtype in (torch.float16, torch.bfloat16), "q must be an fp16 or bf16 tensor")
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
-        _check_rows(t, name, q.dtype)
-        _check(t.device == q.device, "all tensors must be on the same device")
-    (tq, heads, hd), (tk, kv_heads, _) = q.shape, k.shape
-    _check(out.shape == q.shape, "out.shape == q.shape")
-    _check(v.shape == k.shape and k.size(2) == hd, "v.shape == k.shape, k.size(2) == q.size(2)")
-    _check(hd in (32, 64, 128, 256), "the head dimension must be 32, 64, 128 or 256")
-    _check(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "heads must be a multiple of kv_heads")
+    dtype = q.dtype if isinstance(q, torch.Tensor) else None
+    if dtype != torch.float16 and dtype != torch.bfloat16:
+        _refuse("q must be an fp16 or bf16 tensor")
     device = q.device
-    seqs = 1
+    st = PromptStrides(*_rows_ok(q, "q", dtype, device), *_rows_ok(k, "k", dtype, device), *_rows_ok(v, "v", dtype, device),
+                       *_rows_ok(out, "out", dtype, device))
+    (tq, heads, hd), (tk, kv_heads, k_hd) = q.shape, k.shape
+    if out.shape != q.shape:
+        _refuse("out.shape == q.shape")
+    if v.shape != k.shape or k_hd != hd:
+        _refuse("v.shape == k.shape, k.size(2) == q.size(2)")
+    if hd not in (32, 64, 128, 256):
+        _refuse("the head dimension must be 32, 64, 128 or 256")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        _refuse("heads must be a multiple of kv_heads")
+    seqs, qs_ptr, ks_ptr, kl_ptr, lse_ptr = 1, None, None, None, None
     if q_start is not None:
-        seqs = q_start.size(0) - 1
-        _check(seqs >= 1, "q_start must hold at least two entries")
-        _check_index(q_start, "q_start", torch.int32, seqs + 1, device)
-    _check((k_start is None) == (k_len is None), "k_start and k_len go together")
+        seqs = q_start.numel() - 1 if isinstance(q_start, torch.Tensor) else 0
+        if seqs < 1:
+            _refuse("q_start must hold at least two entries")
+        qs_ptr = _vector_ok(q_start, "q_start", torch.int32, seqs + 1, device)
+    if (k_start is None) != (k_len is None):
+        _refuse("k_start and k_len go together")
     if k_start is not None:
-        _check_index(k_start, "k_start", torch.int32, seqs, device)
-        _check_index(k_len, "k_len", torch.int32, seqs, device)
-    else:
-        _check(q_start is None or tk == tq, "without k_start the keys lie as the queries do: k.size(0) == q.size(0)")
+        ks_ptr = _vector_ok(k_start, "k_start", torch.int32, seqs, device)
+        kl_ptr = _vector_ok(k_len, "k_len", torch.int32, seqs, device)
+    elif q_start is not None and tk != tq:
+        _refuse("without k_start the keys lie as the queries do: k.size(0) == q.size(0)")
     if lse is not None:
         _check_input(lse, "lse")
-        _check(lse.dtype == torch.float32 and lse.shape == (tq, heads), "lse must be float32 [Tq, heads]")
-        _check(lse.device == device, "all tensors must be on the same device")
+        if lse.dtype != torch.float32 or lse.shape != (tq, heads):
+            _refuse("lse must be float32 [Tq, heads]")
+        if lse.device != device:
+            _refuse("all tensors must be on the same device")
+        lse_ptr = lse.data_ptr()
     if tq == 0:
         return 0.0
-    st = PromptStrides(*_strides(q), *_strides(k), *_strides(v), *_strides(out))
-    sizes = (seqs, tq, tk, tk if max_k is None else int(max_k), heads, kv_heads, hd)
     lib = library()
-    ms = ctypes.c_float(0.0)
-    with torch.cuda.device(device):
-        need = lib.rptc_attn_prompt_workspace_bytes(*sizes)
-        if need < 0:
-            _status(int(need))
-        # from torch's allocator, so it is this call's own on the current stream and in a graph being captured
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        rc = lib.rptc_attn_prompt(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-                                  None if q_start is None else q_start.data_ptr(), None if k_start is None else k_start.data_ptr(),
-                                  None if k_len is None else k_len.data_ptr(), *sizes, ctypes.byref(st),
-                                  hd ** -0.5 if scale is None else float(scale), 1 if causal else 0, _DTYPES[q.dtype],
-                                  None if ws is None else ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream,
-                                  ctypes.byref(ms) if (_timing if timed is None else timed) else None)
-    _status(rc)
-    return float(ms.value)
+    sizes = (seqs, tq, tk, tk if max_k is None else int(max_k), heads, kv_heads, hd)
+    ws, need = _workspace(device, lib.rptc_attn_prompt_workspace_bytes, *sizes)
+    return _run_on(device, timed, lib.rptc_attn_prompt, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse_ptr, qs_ptr, ks_ptr,
+                   kl_ptr, *sizes, ctypes.byref(st), hd ** -0.5 if scale is None else float(scale), 1 if causal else 0, _DTYPES[dtype],
+                   None if ws is None else ws.data_ptr(), need)
 
 
 def kv4_row_bytes(hd):
     """Bytes of a row (one position of one head) of the 4-bit cache: hd / 2 of codes and a scale and a minimum for every 32 values."""
-    _check(hd in (32, 64, 128, 256), "the head dimension must be 32, 64, 128 or 256")
+    if hd not in (32, 64, 128, 256):
+        _refuse("the head dimension must be 32, 64, 128 or 256")
     return hd // 2 + hd // 8
 
 
@@ -914,20 +961,32 @@ def kv4_cache(seqs, kv_heads, max_len, hd, device="cuda"):
     return torch.zeros(shape, dtype=torch.uint8, device=device), torch.zeros(shape, dtype=torch.uint8, device=device)
 
 
-def _check_kv4(k_cache, v_cache, hd, kv_heads=None):
+def _kv4_ok(k_cache, v_cache, hd):
+    """(sequences, key heads, positions) of a pair of 4-bit caches."""
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         _check_input(t, name)
-        _check(t.dtype == torch.uint8 and t.dim() == 4, f"{name} must be uint8 [seqs, kv_heads, positions, row bytes]")
-    _check(k_cache.shape == v_cache.shape and k_cache.device == v_cache.device, "k_cache and v_cache must be alike")
-    _check(k_cache.size(3) == kv4_row_bytes(hd), "the cache's rows must have kv4_row_bytes(head dimension) bytes")
-    _check(kv_heads is None or k_cache.size(1) == kv_heads, "the cache must have as many heads as k and v")
+        if t.dtype != torch.uint8 or t.dim() != 4:
+            _refuse(f"{name} must be uint8 [seqs, kv_heads, positions, row bytes]")
+    if k_cache.shape != v_cache.shape or k_cache.device != v_cache.device:
+        _refuse("k_cache and v_cache must be alike")
+    seqs, kv_heads, max_len, row = k_cache.shape
+    if row != kv4_row_bytes(hd):
+        _refuse("the cache's rows must have kv4_row_bytes(head dimension) bytes")
+    return seqs, kv_heads, max_len
 
 
-def _kv4_rows(k, v, device):
-    for t, name in ((k, "k"), (v, "v")):
-        _check_rows(t, name, torch.float16)
-        _check(t.device == device, "all tensors must be on the same device")
-    _check(k.shape == v.shape, "v.shape == k.shape")
+def _kv4_rows(k, v, k_cache, v_cache):
+    if not isinstance(k, torch.Tensor) or k.dim() != 3:
+        _refuse("k must be [tokens, kv_heads, head_dim]")
+    total, heads, hd = k.shape
+    seqs, kv_heads, max_len = _kv4_ok(k_cache, v_cache, hd)
+    device = k_cache.device
+    strides = *_rows_ok(k, "k", torch.float16, device), *_rows_ok(v, "v", torch.float16, device)
+    if v.shape != k.shape:
+        _refuse("v.shape == k.shape")
+    if heads != kv_heads:
+        _refuse("the cache must have as many heads as k and v")
+    return device, (seqs, total, kv_heads, hd, max_len), strides
 
 
 def kv4_append(k, v, k_cache, v_cache, pos, q_start=None, timed=None):
@@ -935,75 +994,61 @@ def kv4_append(k, v, k_cache, v_cache, pos, q_start=None, timed=None):
     ``kv4_cache``: sequence s's rows q_start[s] .. q_start[s+1] go to positions pos[s], pos[s] + 1, ... of cache s (int32 and
     int64 tensors on the device; without q_start every sequence has tokens / seqs rows).  Rows that do not fit are
     not written.  Returns elapsed ms."""
-    _check(isinstance(k, torch.Tensor) and k.dim() == 3, "k must be [tokens, kv_heads, head_dim]")
-    total, kv_heads, hd = k.shape
-    _check_kv4(k_cache, v_cache, hd, kv_heads)
-    device = k_cache.device
-    _kv4_rows(k, v, device)
-    seqs, max_len = k_cache.size(0), k_cache.size(2)
-    _check_index(pos, "pos", torch.int64, seqs, device)
+    device, sizes, strides = _kv4_rows(k, v, k_cache, v_cache)
+    seqs, total, _, _, max_len = sizes
+    pos_ptr = _vector_ok(pos, "pos", torch.int64, seqs, device)
+    qs_ptr = None
     if q_start is not None:
-        _check_index(q_start, "q_start", torch.int32, seqs + 1, device)
-    else:
-        _check(total % seqs == 0, "without q_start the rows must divide evenly: k.size(0) % k_cache.size(0) == 0")
+        qs_ptr = _vector_ok(q_start, "q_start", torch.int32, seqs + 1, device)
+    elif seqs < 1 or total % seqs:
+        _refuse("without q_start the rows must divide evenly: k.size(0) % k_cache.size(0) == 0")
     if total == 0 or max_len == 0:
         return 0.0
-    ms = ctypes.c_float(0.0)
-    with torch.cuda.device(device):
-        rc = library().rptc_kv4_append(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pos.data_ptr(),
-                                       None if q_start is None else q_start.data_ptr(), seqs, total, kv_heads, hd, max_len,
-                                       *_strides(k), *_strides(v), torch.cuda.current_stream().cuda_stream,
-                                       ctypes.byref(ms) if (_timing if timed is None else timed) else None)
-    _status(rc)
-    return float(ms.value)
+    return _run_on(device, timed, library().rptc_kv4_append, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pos_ptr,
+                   qs_ptr, *sizes, *strides)
 
 
 def kv4_read(k_cache, v_cache, k, v, timed=None):
     """The first positions of every sequence of the 4-bit caches as fp16: k, v [seqs * rows, kv_heads, hd] (strides as in
     ``attn_prompt``) receive positions 0 .. rows-1, sequence after sequence.  Returns elapsed ms."""
-    _check(isinstance(k, torch.Tensor) and k.dim() == 3, "k must be [tokens, kv_heads, head_dim]")
-    total, kv_heads, hd = k.shape
-    _check_kv4(k_cache, v_cache, hd, kv_heads)
-    device = k_cache.device
-    _kv4_rows(k, v, device)
-    seqs, max_len = k_cache.size(0), k_cache.size(2)
-    _check(seqs >= 1 and total % seqs == 0 and total // seqs <= max_len, "k must hold the same number of rows for every sequence, at most the cache's positions")
+    device, (seqs, total, kv_heads, hd, max_len), strides = _kv4_rows(k, v, k_cache, v_cache)
+    if seqs < 1 or total % seqs or total // seqs > max_len:
+        _refuse("k must hold the same number of rows for every sequence, at most the cache's positions")
     if total == 0:
         return 0.0
-    for t, name in ((k, "k"), (v, "v")):
-        _check(all(s != 0 or n == 1 for s, n in zip(t.stride(), t.shape)), f"{name} must not repeat elements")
-    ms = ctypes.c_float(0.0)
-    with torch.cuda.device(device):
-        rc = library().rptc_kv4_read(k_cache.data_ptr(), v_cache.data_ptr(), k.data_ptr(), v.data_ptr(), seqs, total // seqs, kv_heads,
-                                     hd, max_len, *_strides(k), *_strides(v), torch.cuda.current_stream().cuda_stream,
-                                     ctypes.byref(ms) if (_timing if timed is None else timed) else None)
-    _status(rc)
-    return float(ms.value)
+    if 0 in strides:
+        _refuse("k and v must not repeat elements")
+    return _run_on(device, timed, library().rptc_kv4_read, k_cache.data_ptr(), v_cache.data_ptr(), k.data_ptr(), v.data_ptr(), seqs,
+                   total // seqs, kv_heads, hd, max_len, *strides)
 
 
-def kv4_rope_append(qkv, cos, sin, pos, q_out, k_cache, v_cache):
+def kv4_rope_append(qkv, cos, sin, pos, q_out, k_cache, v_cache, timed=None):
     """One token of every sequence on its way into the 4-bit cache: rotate the (2i, 2i+1) pairs of q and k of qkv (fp16
     [seqs, (heads + 2 kv_heads) * hd]) by cos/sin (fp16 [positions, hd/2]) at pos (int64 [seqs]), write q to q_out (fp16
-    [seqs, heads, hd]) and append k and v at pos.  A sequence whose position lies outside the cache is skipped.  Asynchronous."""
+    [seqs, heads, hd]) and append k and v at pos.  A sequence whose position lies outside the cache is skipped.  Returns
+    elapsed ms."""
     for t, name in ((qkv, "qkv"), (cos, "cos"), (sin, "sin"), (q_out, "q_out")):
         _check_input(t, name)
-        _check(t.dtype == torch.float16, f"{name} must be fp16")
-    _check(q_out.dim() == 3 and qkv.dim() == 2, "q_out must be [seqs, heads, head_dim], qkv [seqs, (heads + 2 kv_heads) * head_dim]")
+        if t.dtype != torch.float16:
+            _refuse(f"{name} must be fp16")
+    if q_out.dim() != 3 or qkv.dim() != 2:
+        _refuse("q_out must be [seqs, heads, head_dim], qkv [seqs, (heads + 2 kv_heads) * head_dim]")
     seqs, heads, hd = q_out.shape
-    _check_kv4(k_cache, v_cache, hd)
-    kv_heads, max_len, device = k_cache.size(1), k_cache.size(2), k_cache.device
-    _check(k_cache.size(0) == seqs and qkv.shape == (seqs, (heads + 2 * kv_heads) * hd), "qkv must be [seqs, (heads + 2 kv_heads) * head_dim]")
-    _check(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "heads must be a multiple of kv_heads")
-    _check(cos.shape == sin.shape and cos.dim() == 2 and cos.size(0) >= max_len and cos.size(1) == hd // 2, "cos and sin must be [positions >= the cache's, head_dim / 2]")
-    _check_index(pos, "pos", torch.int64, seqs, device)
-    _check(all(t.device == device for t in (qkv, cos, sin, q_out)), "all tensors must be on the same device")
+    n, kv_heads, max_len = _kv4_ok(k_cache, v_cache, hd)
+    device = k_cache.device
+    if n != seqs or qkv.shape != (seqs, (heads + 2 * kv_heads) * hd):
+        _refuse("qkv must be [seqs, (heads + 2 kv_heads) * head_dim], the caches hold as many sequences")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        _refuse("heads must be a multiple of kv_heads")
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.size(0) < max_len or cos.size(1) != hd // 2:
+        _refuse("cos and sin must be [positions, head_dim / 2] with as many positions as the cache")
+    pos_ptr = _vector_ok(pos, "pos", torch.int64, seqs, device)
+    if not (qkv.device == cos.device == sin.device == q_out.device == device):
+        _refuse("all tensors must be on the same device")
     if seqs == 0 or max_len == 0:
-        return
-    with torch.cuda.device(device):
-        rc = library().rptc_kv4_rope_append(qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos.data_ptr(), q_out.data_ptr(),
-                                            k_cache.data_ptr(), v_cache.data_ptr(), seqs, heads, kv_heads, hd, max_len,
-                                            torch.cuda.current_stream().cuda_stream)
-    _status(rc)
+        return 0.0
+    return _run_on(device, timed, library().rptc_kv4_rope_append, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos_ptr, q_out.data_ptr(),
+                   k_cache.data_ptr(), v_cache.data_ptr(), seqs, heads, kv_heads, hd, max_len)
 
 
 def kv4_attn_decode(q, k_cache, v_cache, pos, out, scale=None, timed=None):
@@ -1011,34 +1056,29 @@ def kv4_attn_decode(q, k_cache, v_cache, pos, out, scale=None, timed=None):
     0 .. pos[s] of cache s.  q, out fp16 [seqs, heads, hd] (q's sequences may be any multiple of 8 elements apart), head h
     reading key head h // (heads // kv_heads); pos int64 [seqs] on the device.  A sequence whose pos lies outside the cache
     (a padded batch: -1) keeps what ``out`` holds.  ``scale`` defaults to hd ** -0.5.  Returns elapsed ms."""
-    _check(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [seqs, heads, head_dim]")
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        _refuse("q must be [seqs, heads, head_dim]")
     seqs, heads, hd = q.shape
-    _check_kv4(k_cache, v_cache, hd)
+    n, kv_heads, max_len = _kv4_ok(k_cache, v_cache, hd)
     device = k_cache.device
-    _check(q.is_cuda, "q must be a CUDA tensor")
-    _check(q.dtype == torch.float16 and q.stride(2) == 1 and (heads == 1 or q.stride(1) == hd), "q must be fp16 with contiguous heads")
+    token, head = _rows_ok(q, "q", torch.float16, device)
+    if heads > 1 and head != hd:
+        _refuse("q must have contiguous heads")
     _check_input(out, "out")
-    _check(out.dtype == torch.float16 and out.shape == q.shape, "out must be fp16 and have the shape of q")
-    _check(q.device == device and out.device == device, "all tensors must be on the same device")
-    kv_heads, max_len = k_cache.size(1), k_cache.size(2)
-    _check(k_cache.size(0) == seqs, "k_cache.size(0) == q.size(0)")
-    _check(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "heads must be a multiple of kv_heads")
-    _check_index(pos, "pos", torch.int64, seqs, device)
+    if out.dtype != torch.float16 or out.shape != q.shape or out.device != device:
+        _refuse("out must be fp16, of the shape of q and on its device")
+    if n != seqs:
+        _refuse("k_cache.size(0) == q.size(0)")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        _refuse("heads must be a multiple of kv_heads")
+    pos_ptr = _vector_ok(pos, "pos", torch.int64, seqs, device)
     if seqs == 0 or max_len == 0:
         return 0.0
     lib = library()
-    ms = ctypes.c_float(0.0)
-    with torch.cuda.device(device):
-        need = lib.rptc_kv4_attn_decode_workspace_bytes(seqs, heads, kv_heads, hd, max_len)
-        if need < 0:
-            _status(int(need))
-        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        rc = lib.rptc_kv4_attn_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pos.data_ptr(), out.data_ptr(), seqs, heads,
-                                      kv_heads, hd, max_len, q.stride(0) if seqs > 1 else heads * hd,
-                                      hd ** -0.5 if scale is None else float(scale), None if ws is None else ws.data_ptr(), need,
-                                      torch.cuda.current_stream().cuda_stream, ctypes.byref(ms) if (_timing if timed is None else timed) else None)
-    _status(rc)
-    return float(ms.value)
+    ws, need = _workspace(device, lib.rptc_kv4_attn_decode_workspace_bytes, seqs, heads, kv_heads, hd, max_len)
+    return _run_on(device, timed, lib.rptc_kv4_attn_decode, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pos_ptr, out.data_ptr(),
+                   seqs, heads, kv_heads, hd, max_len, token, hd ** -0.5 if scale is None else float(scale),
+                   None if ws is None else ws.data_ptr(), need)
 
 
 def token_logprobs(logits, tokens=None, logprob=None, entropy=None, top_ids=None, top_logprobs=None, timed=None):
@@ -1048,39 +1088,41 @@ def token_logprobs(logits, tokens=None, logprob=None, entropy=None, top_ids=None
     entropy (float32 [rows]): of every row, in nats; top_ids (int64 [rows, k]) and top_logprobs (float32 [rows, k]): the k largest
     logits in falling order, equal ones by the lowest id, k at most 64.  Each output is optional.  A row that holds +inf or a
     not-a-number, or nothing but -inf, gives not-a-number.  Returns elapsed ms."""
-    _check(isinstance(logits, torch.Tensor), "logits must be a torch.Tensor")
-    _check(logits.is_cuda, "logits must be a CUDA tensor")
-    _check(logits.dim() == 2 and logits.dtype in _DTYPES, "logits must be fp16, bf16 or float32 [rows, vocab]")
+    if not isinstance(logits, torch.Tensor):
+        _refuse("logits must be a torch.Tensor")
+    if not logits.is_cuda:
+        _refuse("logits must be a CUDA tensor")
+    if logits.dim() != 2 or logits.dtype not in _DTYPES:
+        _refuse("logits must be fp16, bf16 or float32 [rows, vocab]")
     rows, vocab = logits.shape
-    _check(vocab >= 1, "the vocabulary must not be empty")
-    _check(vocab == 1 or logits.stride(1) == 1, "logits must be contiguous along the vocabulary")
-    _check(not (logprob is None and entropy is None and top_ids is None and top_logprobs is None), "at least one output is needed")
+    row_stride, step = logits.stride()
+    if vocab < 1:
+        _refuse("the vocabulary must not be empty")
+    if vocab > 1 and step != 1:
+        _refuse("logits must be contiguous along the vocabulary")
+    if logprob is None and entropy is None and top_ids is None and top_logprobs is None:
+        _refuse("at least one output is needed")
+    if logprob is not None and tokens is None:
+        _refuse("logprob needs tokens")
     device = logits.device
-    if logprob is not None:
-        _check(tokens is not None, "logprob needs tokens")
-    if tokens is not None:
-        _check_index(tokens, "tokens", torch.int64, rows, device)
-    for t, name in ((logprob, "logprob"), (entropy, "entropy")):
-        if t is not None:
-            _check_index(t, name, torch.float32, rows, device)
+    tok_ptr = None if tokens is None else _vector_ok(tokens, "tokens", torch.int64, rows, device)
+    lp_ptr = None if logprob is None else _vector_ok(logprob, "logprob", torch.float32, rows, device)
+    ent_ptr = None if entropy is None else _vector_ok(entropy, "entropy", torch.float32, rows, device)
     top = 0
     for t, name, dtype in ((top_ids, "top_ids", torch.int64), (top_logprobs, "top_logprobs", torch.float32)):
         if t is not None:
             _check_input(t, name)
-            _check(t.dtype == dtype and t.dim() == 2 and t.size(0) == rows, f"{name} must be {str(dtype)[6:]} [rows, k]")
-            _check(t.device == device, "all tensors must be on the same device")
-            _check(top in (0, t.size(1)), "top_ids and top_logprobs must have the same shape")
+            if t.dtype != dtype or t.dim() != 2 or t.size(0) != rows:
+                _refuse(f"{name} must be {str(dtype)[6:]} [rows, k]")
+            if t.device != device:
+                _refuse("all tensors must be on the same device")
+            if top not in (0, t.size(1)):
+                _refuse("top_ids and top_logprobs must have the same shape")
             top = t.size(1)
-            _check(1 <= top <= min(64, vocab), "1 <= k <= 64, k <= vocabulary")
+            if not 1 <= top <= min(64, vocab):
+                _refuse("1 <= k <= 64, k <= vocabulary")
     if rows == 0:
         return 0.0
-    ms = ctypes.c_float(0.0)
-    with torch.cuda.device(device):
-        rc = library().rptc_token_logprobs(logits.data_ptr(), _DTYPES[logits.dtype], None if tokens is None else tokens.data_ptr(),
-                                           None if logprob is None else logprob.data_ptr(), None if entropy is None else entropy.data_ptr(),
-                                           None if top_ids is None else top_ids.data_ptr(),
-                                           None if top_logprobs is None else top_logprobs.data_ptr(), rows, vocab,
-                                           logits.stride(0) if rows > 1 else vocab, top, torch.cuda.current_stream().cuda_stream,
-                                           ctypes.byref(ms) if (_timing if timed is None else timed) else None)
-    _status(rc)
-    return float(ms.value)
+    return _run_on(device, timed, library().rptc_token_logprobs, logits.data_ptr(), _DTYPES[logits.dtype], tok_ptr, lp_ptr, ent_ptr,
+                   None if top_ids is None else top_ids.data_ptr(), None if top_logprobs is None else top_logprobs.data_ptr(), rows, vocab,
+                   row_stride if rows > 1 else vocab, top)
