@@ -411,7 +411,7 @@ int64_t rptc_lite_viterbi_scratch_bytes(int L, int R, int64_t rows, int64_t step
  *   it only decides how far the keys of a call with few rows are split)
  *   workspace  rptc_attn_prompt_workspace_bytes(...) bytes of device memory, 16-byte aligned (0: may be NULL); no
  *              initialisation, calls that may overlap need one each.  At most 2^24 query rows, 1024 heads, 2^20 sequences,
- *              (total_q / 128 + seqs) * heads below 2^23.
+ *              (total_q / 32 + seqs) * heads below 2^23.
  */
 typedef struct rptc_prompt_strides {
     int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;

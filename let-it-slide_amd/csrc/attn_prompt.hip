@@ -71,29 +71,34 @@ struct PromptArgs {
 
 struct PromptTile {
     int seq, q_begin, q_end, row0;     // the sequence's query rows, the tile's first row
+    int k_first, k_len;                // and its keys
 };
 
 // A value every lane of the wave holds, as one the compiler knows to be such (scalar registers, scalar branches).
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// The sequence that holds tile `tile` when every sequence is cut into tiles of kRows query rows: 64 sequences at a time,
-// a lane each.  A sequence's tiles are taken from its end (the longest rows of a causal prompt first).  The starts come
-// from device memory: a sequence that does not lie inside the query rows has no tiles.
+// The sequence that holds tile `tile` when every sequence is cut into tiles of ROWS query rows: 64 sequences at a time, a
+// lane each.  A sequence's tiles are taken from its end (the longest rows of a causal prompt first).  The starts come from
+// device memory: a sequence that does not lie inside the query rows has no tiles; false for a tile past the last, and
+// for one whose keys do not lie inside k and v (its rows are left as they are).
+template <int ROWS>
 __device__ __forceinline__ bool find_tile(const PromptArgs &a, int tile, PromptTile &t)
 {
     const int lane = threadIdx.x & 63;
     t.seq = -1;
-    t.q_begin = t.q_end = t.row0 = 0;
+    t.q_begin = t.q_end = t.row0 = t.k_first = t.k_len = 0;
     int in_front = 0;                      // tiles of the sequences in front (they do not overlap: at most a.tiles)
     for (int s0 = 0; s0 < a.seqs; s0 += 64) {
         const int s = s0 + lane;
-        int begin = 0, end = 0;
+        int begin = 0, end = 0, kf = 0, kl = 0;
         if (s < a.seqs) {
             begin = a.q_start ? a.q_start[s] : 0;
             end = a.q_start ? a.q_start[s + 1] : a.total_q;
+            kf = a.k_start ? a.k_start[s] : a.q_start ? begin : 0;
+            kl = a.k_len ? a.k_len[s] : a.q_start ? end - begin : a.total_k;
         }
         const bool ok = begin >= 0 && end > begin && end <= a.total_q;
-        const int n = ok ? (end - begin + kRows - 1) / kRows : 0;
+        const int n = ok ? (end - begin + ROWS - 1) / ROWS : 0;
         int incl = n;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
@@ -108,7 +113,9 @@ __device__ __forceinline__ bool find_tile(const PromptArgs &a, int tile, PromptT
             t.seq = s0 + f;
             t.q_begin = __builtin_amdgcn_readlane(begin, f);
             t.q_end = __builtin_amdgcn_readlane(end, f);
-            t.row0 = t.q_begin + (nf - 1 - local) * kRows;
+            t.row0 = t.q_begin + (nf - 1 - local) * ROWS;
+            t.k_first = __builtin_amdgcn_readlane(kf, f);
+            t.k_len = __builtin_amdgcn_readlane(kl, f);
             break;
         }
         in_front += __builtin_amdgcn_readlane(incl, 63);
@@ -117,17 +124,28 @@ __device__ __forceinline__ bool find_tile(const PromptArgs &a, int tile, PromptT
     t.q_begin = uniform(t.q_begin);
     t.q_end = uniform(t.q_end);
     t.row0 = uniform(t.row0);
-    return t.seq >= 0;
+    t.k_first = uniform(t.k_first);
+    t.k_len = uniform(t.k_len);
+    return t.seq >= 0 && t.k_first >= 0 && t.k_len >= 0 && (int64_t)t.k_first + t.k_len <= a.total_k;
 }
 
-// The sequence's keys; false when they do not lie inside k and v (its rows are then left as they are).
-__device__ __forceinline__ bool find_keys(const PromptArgs &a, const PromptTile &t, int &first, int &len)
+// keys a row sees: [0, sees)
+__device__ __forceinline__ int prompt_sees(const PromptArgs &a, const PromptTile &t, int row)
 {
-    first = a.k_start ? a.k_start[t.seq] : a.q_start ? t.q_begin : 0;
-    len = a.k_len ? a.k_len[t.seq] : a.q_start ? t.q_end - t.q_begin : a.total_k;
-    first = uniform(first);
-    len = uniform(len);
-    return first >= 0 && len >= 0 && (int64_t)first + len <= a.total_k;
+    return a.causal ? max(0, t.k_len - (t.q_end - t.q_begin) + 1 + (row - t.q_begin)) : t.k_len;
+}
+
+// Workgroup -> (head, tile, split): tiles from the longest walks to the shortest, so that the last workgroups to start are
+// short ones.  Consecutive workgroups go to the eight XCDs in turn, each with an L2 of its own: where the heads divide
+// evenly an XCD gets a run of heads (those of a group read the same K and V) and walks over the tiles of all of them.
+__device__ __forceinline__ void prompt_item(const PromptArgs &a, int &head, int &tile, int &split)
+{
+    const bool runs = a.heads % 8 == 0;
+    const int run = runs ? a.heads >> 3 : a.heads, local = runs ? blockIdx.x >> 3 : blockIdx.x;
+    const int rest = local / run;
+    head = local - rest * run + (runs ? (blockIdx.x & 7) * run : 0);
+    tile = rest / a.splits;
+    split = rest - tile * a.splits;
 }
 
 // 16 bytes a lane from `offset` of the buffer to LDS at `to` + 16 lane (no register receives anything: the request may
@@ -139,6 +157,15 @@ __device__ __forceinline__ void load_to_lds(uint32_t offset, int4_t resource, ui
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(resource), "s"(to) : "memory");
 }
 __device__ __forceinline__ void wait_for_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// all but the N requests made last
+template <int N>
+__device__ __forceinline__ void wait_for_lds_loads_but()
+{
+    static_assert(N < 64, "the counter has six bits");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// what was read from LDS is in registers: its place may be written over
+__device__ __forceinline__ void wait_for_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ uint32_t lds_address(const void *p)
 {
     return (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p);
@@ -170,22 +197,20 @@ __device__ __forceinline__ int swizzle_v(int row)
     return HD >= 128 ? (row & 3) << 2 : HD == 64 ? (row >> 1 & 1) << 2 : 0;
 }
 
-// One wave's rows in plain fp32, one row after the other, keys [k_lo, k_hi) of those a row sees.  Taken when a sum of the
-// matrix path came out infinite or not a number: that is right where the row sees such a value, and wrong where only
-// a masked key or a masked row of V held it (0 * NaN is NaN), so the rows are worked out again without the masked ones.
+// `rows` rows in plain fp32, one after the other, keys [k_lo, k_hi) of those a row sees.  Taken when a sum of the matrix path
+// came out infinite or not a number: that is right where the row sees such a value, and wrong where only a masked key or a
+// masked row of V held it (0 * NaN is NaN), so the rows are worked out again without the masked ones.
 template <int HD, class T>
-__device__ __forceinline__ void prompt_rows_plain(const PromptArgs &a, const PromptTile &t, int row_first, int head, int kvh,
-                                                            int ks, int lk, int k_lo, int k_hi, int split)
+__device__ __forceinline__ void prompt_rows_plain(const PromptArgs &a, const PromptTile &t, int row_first, int rows, int head, int kvh,
+                                                  int k_lo, int k_hi, int split)
 {
     const int lane = threadIdx.x & 63;
-    const int lq = t.q_end - t.q_begin;
     constexpr int kOut = (HD + 63) / 64;
-    for (int row = row_first; row < min(row_first + 32, t.q_end); row++) {
-        const int see = a.causal ? lk - lq + 1 + (row - t.q_begin) : lk;
-        const int end = min(see, k_hi);
+    for (int row = row_first; row < min(row_first + rows, t.q_end); row++) {
+        const int end = min(prompt_sees(a, t, row), k_hi);
         const uint16_t *q = a.q + (int64_t)row * a.st.q_token + (int64_t)head * a.st.q_head;
         auto score = [&](int j) {
-            const uint16_t *k = a.k + (int64_t)(ks + j) * a.st.k_token + (int64_t)kvh * a.st.k_head;
+            const uint16_t *k = a.k + (int64_t)(t.k_first + j) * a.st.k_token + (int64_t)kvh * a.st.k_head;
             float s = 0.f;
             for (int d = 0; d < HD; d++) s = fmaf(T::to_float(q[d]), T::to_float(k[d]), s);
             return s;
@@ -201,7 +226,7 @@ __device__ __forceinline__ void prompt_rows_plain(const PromptArgs &a, const Pro
             l += p;
             for (int i = 0; i < min(64, end - j0); i++) {
                 const float pi = __shfl(p, i, 64);
-                const uint16_t *v = a.v + (int64_t)(ks + j0 + i) * a.st.v_token + (int64_t)kvh * a.st.v_head;
+                const uint16_t *v = a.v + (int64_t)(t.k_first + j0 + i) * a.st.v_token + (int64_t)kvh * a.st.v_head;
                 for (int u = 0; u < kOut; u++)
                     if (lane + 64 * u < HD) acc[u] = fmaf(pi, T::to_float(v[lane + 64 * u]), acc[u]);
             }
@@ -225,41 +250,153 @@ __device__ __forceinline__ void prompt_rows_plain(const PromptArgs &a, const Pro
     }
 }
 
+// What a wave holds of 32 query rows, and the parts of a step over KEYS keys (a multiple of 32).  Lane (col, c): row col; of
+// every eight keys and of every eight dimensions the four from 4c on.
+template <int HD, class T, int KEYS>
+struct PromptWave {
+    static constexpr int kSteps = HD / 16, kDims = HD / 32, kBlocks = KEYS / 32;
+    short8_t qf[kSteps];
+    float16_t acc[kDims];
+    float m, l;                            // running bound of c * score (log2 units), sum of p over the lane's keys
+
+    __device__ __forceinline__ void begin(const PromptArgs &a, const PromptTile &t, int row, int head)
+    {
+        // a lane without a row of its own takes the sequence's last (its results go nowhere)
+        const uint16_t *q = a.q + (int64_t)min(row, t.q_end - 1) * a.st.q_token + (int64_t)head * a.st.q_head + 8 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+        for (int i = 0; i < kSteps; i++) qf[i] = *reinterpret_cast<const short8_t *>(q + 16 * i);
+#pragma unroll
+        for (int d = 0; d < kDims; d++) acc[d] = (float16_t)(0.f);
+        m = -INFINITY;
+        l = 0.f;
+    }
+    // the query is there: a wait inside the loop would wait for the step's K and V as well
+    __device__ __forceinline__ void settle()
+    {
+#pragma unroll
+        for (int i = 0; i < kSteps; i++) asm volatile("" : "+v"(qf[i]));
+    }
+    // S^T of the keys in LDS at kt
+    __device__ __forceinline__ void scores(const uint16_t *kt, float16_t (&s)[kBlocks]) const
+    {
+        const int lane = threadIdx.x & 63, c = lane >> 5, col = lane & 31;
+#pragma unroll
+        for (int h = 0; h < kBlocks; h++) {
+            s[h] = (float16_t)(0.f);
+            const int r = 32 * h + col;
+#pragma unroll
+            for (int i = 0; i < kSteps; i++) {
+                const short8_t kf = *reinterpret_cast<const short8_t *>(kt + r * HD + ((2 * i + c) ^ swizzle_k<HD>(r)) * 8);
+                s[h] = T::mfma(kf, qf[i], s[h]);
+            }
+        }
+    }
+    // keys from `left` on (counted from the step's first) are not the row's
+    static __device__ __forceinline__ void mask(float16_t (&s)[kBlocks], int left)
+    {
+        left -= 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+        for (int h = 0; h < kBlocks; h++)
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (32 * h + 8 * (r / 4) + r % 4 >= left) s[h][r] = -INFINITY;
+    }
+    // raises the bound where a score exceeds it by more than 2^kLazy; returns the bound to take off
+    __device__ __forceinline__ float bound(const float16_t (&s)[kBlocks], float scale)
+    {
+        float mx = s[0][0];
+#pragma unroll
+        for (int h = 0; h < kBlocks; h++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[h][r]);
+        mx = halves_max(mx) * scale;
+        if (__ballot(mx > m + kLazy)) {
+            const float up = fmaxf(m, mx);
+            const float f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - up);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < kDims; d++) acc[d] *= f;
+            m = up;
+        }
+        return m == -INFINITY ? 0.f : m;
+    }
+    // p = exp2(c s - bound), packed in pairs of keys
+    __device__ __forceinline__ void weights(const float16_t (&s)[kBlocks], float scale, float off, uint32_t (&p)[kBlocks][8])
+    {
+#pragma unroll
+        for (int h = 0; h < kBlocks; h++)
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[h][r], scale, -off)), p1 = __builtin_amdgcn_exp2f(fmaf(s[h][r + 1], scale, -off));
+                l += p0;
+                l += p1;
+                p[h][r / 2] = T::pack(p0, p1);
+            }
+    }
+    // acc += V^T P^T, V in LDS at vt: the lane's dimension of a tile of 32, keys in the order the scores' registers have them
+    __device__ __forceinline__ void product(const uint16_t *vt, const uint32_t (&p)[kBlocks][8])
+    {
+        typedef __attribute__((address_space(3))) short4_t lds_short4;
+        const int lane = threadIdx.x & 63, c = lane >> 5, g16 = lane >> 4, rr = (lane & 15) >> 2, piece = lane & 3;
+#pragma unroll
+        for (int h = 0; h < kBlocks; h++)
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const uint4 pv = make_uint4(p[h][4 * g], p[h][4 * g + 1], p[h][4 * g + 2], p[h][4 * g + 3]);
+                const int key = 32 * h + 16 * g + 4 * c + rr;
+#pragma unroll
+                for (int d = 0; d < kDims; d++) {
+                    const int ch = (4 * d + 2 * (g16 & 1) + piece / 2) ^ swizzle_v<HD>(key);   // key and key + 8: the same swizzle
+                    const uint16_t *va = vt + key * HD + ch * 8 + (piece & 1) * 4;
+                    const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)va);
+                    const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(va + 8 * HD));
+                    acc[d] = T::mfma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), __builtin_bit_cast(short8_t, pv), acc[d]);
+                }
+            }
+    }
+    // whether a sum of the wave is infinite or not a number
+    __device__ __forceinline__ bool odd() const
+    {
+        float bad = 0.f;
+#pragma unroll
+        for (int d = 0; d < kDims; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) bad = fmaf(acc[d][r], 0.f, bad);
+        return __ballot(bad != 0.f) != 0;      // (not-a-number compares unequal)
+    }
+};
+
+// the buffer descriptor of `rows` rows, in scalar registers; what lies at or past its end reads as zero
+template <int HD>
+__device__ __forceinline__ int4_t prompt_resource(const uint16_t *base, int64_t token, int rows)
+{
+    const uint64_t p = reinterpret_cast<uint64_t>(base);
+    const int4_t r = {uniform((int)p), uniform((int)(p >> 32) & 0xFFFF), uniform(((rows - 1) * (int)token + HD) * 2), 0x00027000};
+    return r;
+}
+
+// Many rows: 128 query rows of a head a workgroup, 32 a wave; all waves walk over the same keys, which are brought to LDS
+// once for the four of them, a step ahead.
 template <int HD, class T>
 __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_kernel(const PromptArgs a)
 {
-    extern __shared__ __align__(16) uint16_t lds[];       // [2][K, V][kKeys][HD]
+    extern __shared__ __align__(16) uint16_t lds[];       // two buffers of K, two of V, [kKeys][HD] each
     constexpr int kTile = kKeys * HD;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int c = lane >> 5, col = lane & 31;
-
-    // Workgroup -> (head, tile, split).  Consecutive workgroups go to the eight XCDs in turn, each with an L2 of its own:
-    // the items are renumbered so that an XCD gets a run of them, heads of one group of queries (the same K and V) together.
-    const int items = a.heads * a.tiles * a.splits, per_xcd = gridDim.x >> 3;
-    const int item = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if (item >= items) return;
-    const int head = item / (a.tiles * a.splits), rest = item - head * a.tiles * a.splits;
-    const int tile = rest / a.splits, split = rest - tile * a.splits;
+    int head, tile, split;
+    prompt_item(a, head, tile, split);
     PromptTile t;
-    if (!find_tile(a, tile, t)) return;
-    int ks, lk;
-    if (!find_keys(a, t, ks, lk)) return;
+    if (!find_tile<kRows>(a, tile, t)) return;
     const int kvh = head / (a.heads / a.kv_heads);
-    const int lq = t.q_end - t.q_begin;
 
-    // keys a row sees: [0, see); of the tile's last row the most
-    const int last = min(t.row0 + kRows, t.q_end) - 1;
-    auto sees = [&](int row) { return a.causal ? max(0, lk - lq + 1 + (row - t.q_begin)) : lk; };
-    const int k_most = uniform(sees(last));
-    const int per_split = ((k_most + a.splits - 1) / a.splits + kKeys - 1) / kKeys * kKeys;
-    const int k_lo = uniform((int)min((int64_t)k_most, (int64_t)split * per_split));
-    const int k_hi = uniform((int)min((int64_t)k_most, (int64_t)k_lo + per_split));
+    const int k_hi = uniform(prompt_sees(a, t, min(t.row0 + kRows, t.q_end) - 1));      // of the tile's last row: the most
     const int row_first = t.row0 + 32 * wave, row = row_first + col;
     const bool wave_live = row_first < t.q_end;
-    const int see = row < t.q_end ? sees(row) : 0;
+    const int see = row < t.q_end ? prompt_sees(a, t, row) : 0;
     // what all rows of the wave see, and what one of them sees
-    const int see_least = uniform(wave_live ? min(sees(row_first), k_hi) : 0);
-    const int see_most = uniform(wave_live ? min(sees(min(row_first + 31, t.q_end - 1)), k_hi) : 0);
+    const int see_least = uniform(wave_live ? prompt_sees(a, t, row_first) : 0);
+    const int see_most = uniform(wave_live ? prompt_sees(a, t, min(row_first + 31, t.q_end - 1)) : 0);
 
     // K and V, 16 bytes a lane and request: a request covers 1024 bytes of LDS, the lane's source is chosen so that the
     // chunks land swizzled.  Past the sequence's last key the buffer's bounds check gives zeros.
@@ -272,154 +409,215 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
         k_off[u] = (uint32_t)(r * a.st.k_token + (ch ^ swizzle_k<HD>(r)) * 8) * 2u;
         v_off[u] = (uint32_t)(r * a.st.v_token + (ch ^ swizzle_v<HD>(r)) * 8) * 2u;
     }
-    const uint16_t *k_base = a.k + (int64_t)ks * a.st.k_token + (int64_t)kvh * a.st.k_head;
-    const uint16_t *v_base = a.v + (int64_t)ks * a.st.v_token + (int64_t)kvh * a.st.v_head;
-    // the descriptor of `rows` rows, in scalar registers; offsets at or past its end read as zero
-    auto resource = [&](const uint16_t *base, int64_t token, int rows) {
-        const uint64_t p = reinterpret_cast<uint64_t>(base);
-        const int4_t r = {uniform((int)p), uniform((int)(p >> 32) & 0xFFFF), uniform(((rows - 1) * (int)token + HD) * 2), 0x00027000};
-        return r;
-    };
+    const uint16_t *k_base = a.k + (int64_t)t.k_first * a.st.k_token + (int64_t)kvh * a.st.k_head;
+    const uint16_t *v_base = a.v + (int64_t)t.k_first * a.st.v_token + (int64_t)kvh * a.st.v_head;
     const uint32_t lds_base = lds_address(lds) + (uint32_t)wave * 1024u;
-    auto request = [&](int k0, int buf) {
-        const int rows = min(lk - k0, kKeys);
-        const int4_t kr = resource(k_base + (int64_t)k0 * a.st.k_token, a.st.k_token, rows);
-        const int4_t vr = resource(v_base + (int64_t)k0 * a.st.v_token, a.st.v_token, rows);
-        const uint32_t to = lds_base + (uint32_t)buf * (4u * kTile);
+    auto request_k = [&](int k0, int buf) {
+        const int4_t r = prompt_resource<HD>(k_base + (int64_t)k0 * a.st.k_token, a.st.k_token, min(t.k_len - k0, kKeys));
 #pragma unroll
-        for (int u = 0; u < kRequests; u++) load_to_lds(k_off[u], kr, to + u * 4096u);
+        for (int u = 0; u < kRequests; u++) load_to_lds(k_off[u], r, lds_base + (uint32_t)buf * (2u * kTile) + u * 4096u);
+    };
+    auto request_v = [&](int k0, int buf) {
+        const int4_t r = prompt_resource<HD>(v_base + (int64_t)k0 * a.st.v_token, a.st.v_token, min(t.k_len - k0, kKeys));
 #pragma unroll
-        for (int u = 0; u < kRequests; u++) load_to_lds(v_off[u], vr, to + 2u * kTile + u * 4096u);
+        for (int u = 0; u < kRequests; u++) load_to_lds(v_off[u], r, lds_base + (uint32_t)(2 + buf) * (2u * kTile) + u * 4096u);
     };
 
-    constexpr int kSteps = HD / 16, kDims = HD / 32;
-    short8_t qf[kSteps];
-    {
-        // a lane without a row of its own takes the sequence's last (its results go nowhere)
-        const uint16_t *q = a.q + (int64_t)min(row, t.q_end - 1) * a.st.q_token + (int64_t)head * a.st.q_head + 8 * c;
-#pragma unroll
-        for (int i = 0; i < kSteps; i++) qf[i] = *reinterpret_cast<const short8_t *>(q + 16 * i);
-        // waited for here: a wait inside the loop would wait for the step's K and V as well
-#pragma unroll
-        for (int i = 0; i < kSteps; i++) asm volatile("" : "+v"(qf[i]));
+    if (k_hi > 0) {
+        request_k(0, 0);
+        request_v(0, 0);
+        if (kKeys < k_hi) request_k(kKeys, 1);
     }
-    float16_t acc[kDims];
-#pragma unroll
-    for (int d = 0; d < kDims; d++) acc[d] = (float16_t)(0.f);
-    float m = -INFINITY, l = 0.f;           // running bound in units of c * score (log2), sum of p over the lane's keys
-
-    if (k_lo < k_hi) request(k_lo, 0);
-    int buf = 0;
-    for (int k0 = k_lo; k0 < k_hi; k0 += kKeys, buf ^= 1) {
-        wait_for_lds_loads();                              // this wave's part of the step is in LDS
-        __syncthreads();                                   // everyone's is, and nobody reads the other buffer any more
-        if (k0 + kKeys < k_hi) request(k0 + kKeys, buf ^ 1);
-        if (k0 >= see_most) continue;
-        const uint16_t *kt = lds + buf * 2 * kTile, *vt = kt + kTile;
-
-        float16_t s[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            s[h] = (float16_t)(0.f);
-            const int r = 32 * h + col;
-#pragma unroll
-            for (int i = 0; i < kSteps; i++) {
-                const short8_t kf = *reinterpret_cast<const short8_t *>(kt + r * HD + ((2 * i + c) ^ swizzle_k<HD>(r)) * 8);
-                s[h] = T::mfma(kf, qf[i], s[h]);
-            }
-        }
-        if (k0 + kKeys > see_least) {                      // some row of the wave does not see all of the step's keys
-            const int left = min(see, k_hi) - k0 - 4 * c;
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if (32 * h + 8 * (r / 4) + r % 4 >= left) s[h][r] = -INFINITY;
-        }
-        float mx = s[0][0];
-#pragma unroll
-        for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[0][r]);
-#pragma unroll
-        for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[1][r]);
-        mx = halves_max(mx) * a.c;
-        if (__ballot(mx > m + kLazy)) {
-            const float up = fmaxf(m, mx);
-            const float f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - up);
-            l *= f;
-#pragma unroll
-            for (int d = 0; d < kDims; d++) acc[d] *= f;
-            m = up;
-        }
-        const float mc = m == -INFINITY ? 0.f : m;
+    PromptWave<HD, T, kKeys> w;
+    w.begin(a, t, row, head);
+    w.settle();
+    // One step: the softmax of the scores s of the keys from k0 on and their product with V, while the matrix unit forms the
+    // next step's scores (behind the last step these are of whatever the buffer holds, and nobody looks at them).
+    auto step = [&](int k0, int buf, float16_t (&s)[2], float16_t (&next)[2]) {
+        wait_for_lds_loads();                              // this wave's part of the next K and of this V is in LDS
+        __syncthreads();                                   // everyone's is, and nobody reads what is requested over now
+        if (k0 + 2 * kKeys < k_hi) request_k(k0 + 2 * kKeys, buf);
+        if (k0 + kKeys < k_hi) request_v(k0 + kKeys, buf ^ 1);
+        if (k0 >= see_most) return;
+        if (k0 + kKeys > see_least) w.mask(s, see - k0);   // some row of the wave does not see all of the step's keys
+        const float off = w.bound(s, a.c);
+        w.scores(lds + (buf ^ 1) * kTile, next);
         uint32_t p[2][8];
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[h][r], a.c, -mc)), p1 = __builtin_amdgcn_exp2f(fmaf(s[h][r + 1], a.c, -mc));
-                l += p0;
-                l += p1;
-                p[h][r / 2] = T::pack(p0, p1);
-            }
-        // V^T: lane's dimension col of a tile of 32, keys in the order the scores' registers have them
-        const int g16 = lane >> 4, rr = (lane & 15) >> 2, piece = lane & 3;
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int g = 0; g < 2; g++) {
-                const uint4 pv = make_uint4(p[h][4 * g], p[h][4 * g + 1], p[h][4 * g + 2], p[h][4 * g + 3]);
-                const int key = 32 * h + 16 * g + 4 * c + rr;
-#pragma unroll
-                for (int d = 0; d < kDims; d++) {
-                    typedef __attribute__((address_space(3))) short4_t lds_short4;
-                    const int ch = (4 * d + 2 * (g16 & 1) + piece / 2) ^ swizzle_v<HD>(key);   // key and key + 8: the same swizzle
-                    const uint16_t *va = vt + key * HD + ch * 8 + (piece & 1) * 4;
-                    const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)va);
-                    const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(va + 8 * HD));
-                    acc[d] = T::mfma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), __builtin_bit_cast(short8_t, pv), acc[d]);
-                }
-            }
+        w.weights(s, a.c, off, p);
+        w.product(lds + (2 + buf) * kTile, p);
+    };
+    if (k_hi > 0) {
+        float16_t sa[2], sb[2];
+        wait_for_lds_loads();
+        __syncthreads();
+        w.scores(lds, sa);
+        for (int k0 = 0; k0 < k_hi; k0 += 2 * kKeys) {
+            step(k0, 0, sa, sb);
+            if (k0 + kKeys >= k_hi) break;
+            step(k0 + kKeys, 1, sb, sa);
+        }
     }
     if (!wave_live) return;
-    l = halves_sum(l);
-
-    float bad = 0.f;
-#pragma unroll
-    for (int d = 0; d < kDims; d++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) bad = fmaf(acc[d][r], 0.f, bad);
-    if (__ballot(bad != 0.f)) {                            // (not-a-number compares unequal)
-        prompt_rows_plain<HD, T>(a, t, row_first, head, kvh, ks, lk, k_lo, k_hi, split);
+    if (w.odd()) {
+        prompt_rows_plain<HD, T>(a, t, row_first, 32, head, kvh, 0, k_hi, 0);
         return;
     }
-    const int64_t at = (int64_t)row * a.heads + head;
-    if (a.splits > 1) {
-        if (row >= t.q_end) return;
-        const int64_t pa = at * a.splits + split;
-        float *o = a.part_acc + pa * HD + 4 * c;
-#pragma unroll
-        for (int d = 0; d < kDims; d++)
-#pragma unroll
-            for (int b = 0; b < 4; b++)
-                *reinterpret_cast<float4 *>(o + 32 * d + 8 * b) = make_float4(acc[d][4 * b], acc[d][4 * b + 1], acc[d][4 * b + 2], acc[d][4 * b + 3]);
-        if (c == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * pa) = make_float2(l == 0.f ? -INFINITY : m, l);
-        return;
-    }
+    const float l = halves_sum(w.l);
     const float inv = l == 0.f ? 0.f : 1.f / l;            // a row that sees nothing: zeros
     uint16_t *o = a.out + (int64_t)min(row, t.q_end - 1) * a.st.out_token + (int64_t)head * a.st.out_head + 8 * c;
 #pragma unroll
-    for (int d = 0; d < kDims; d++)
+    for (int d = 0; d < HD / 32; d++)
 #pragma unroll
         for (int b = 0; b < 4; b += 2) {
             // the lane's four dimensions of blocks b and b + 1 (8 dimensions each, the halves of the wave four): a swap of
             // the halves leaves eight consecutive ones of block b + c in each lane
-            uint32_t x0 = T::pack(acc[d][4 * b] * inv, acc[d][4 * b + 1] * inv), x1 = T::pack(acc[d][4 * b + 2] * inv, acc[d][4 * b + 3] * inv);
-            uint32_t y0 = T::pack(acc[d][4 * b + 4] * inv, acc[d][4 * b + 5] * inv), y1 = T::pack(acc[d][4 * b + 6] * inv, acc[d][4 * b + 7] * inv);
+            const float16_t &x = w.acc[d];
+            uint32_t x0 = T::pack(x[4 * b] * inv, x[4 * b + 1] * inv), x1 = T::pack(x[4 * b + 2] * inv, x[4 * b + 3] * inv);
+            uint32_t y0 = T::pack(x[4 * b + 4] * inv, x[4 * b + 5] * inv), y1 = T::pack(x[4 * b + 6] * inv, x[4 * b + 7] * inv);
             const auto w0 = __builtin_amdgcn_permlane32_swap(x0, y0, false, false), w1 = __builtin_amdgcn_permlane32_swap(x1, y1, false, false);
             if (row < t.q_end)
                 *reinterpret_cast<uint4 *>(o + 32 * d + 8 * b) = make_uint4((uint32_t)w0[0], (uint32_t)w1[0], (uint32_t)w0[1], (uint32_t)w1[1]);
         }
-    if (a.lse && c == 0 && row < t.q_end) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
+    if (a.lse && c == 0 && row < t.q_end) a.lse[(int64_t)row * a.heads + head] = l == 0.f ? -INFINITY : (w.m + log2f(l)) * 0.693147180559945f;
+}
+
+// Few rows: 32 query rows of a head a workgroup; the four waves hold the same rows and take the steps over the keys (of this
+// workgroup's piece of them) in turn, each with K and V of its own in LDS and no barrier until they join at the end: K of
+// a wave's next step is on its way while it works on V, and the other way round.
+constexpr int kNarrowRows = 32;
+template <int HD>
+constexpr int kNarrowKeys = HD > 128 ? 32 : 64;
+
+template <int HD, class T>
+__global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_narrow_kernel(const PromptArgs a)
+{
+    constexpr int kStep = kNarrowKeys<HD>, kTile = kStep * HD, kJoinRow = HD > 128 ? HD : HD + 4;
+    static_assert(kNarrowRows * kJoinRow * 4 <= 2 * kTile * 2, "a wave's sums fit where its K and V were");
+    extern __shared__ __align__(16) uint16_t lds[];       // [wave][K, V][kStep][HD]
+    __shared__ float s_ml[4][kNarrowRows][2];
+    __shared__ int s_odd;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int c = lane >> 5, col = lane & 31;
+    int head, tile, split;
+    prompt_item(a, head, tile, split);
+    PromptTile t;
+    if (!find_tile<kNarrowRows>(a, tile, t)) return;
+    if (tid == 0) s_odd = 0;
+    const int kvh = head / (a.heads / a.kv_heads);
+    const int k_most = uniform(prompt_sees(a, t, min(t.row0 + kNarrowRows, t.q_end) - 1));
+    const int per_split = ((k_most + a.splits - 1) / a.splits + kStep - 1) / kStep * kStep;
+    const int k_lo = uniform((int)min((int64_t)k_most, (int64_t)split * per_split));
+    const int k_hi = uniform((int)min((int64_t)k_most, (int64_t)k_lo + per_split));
+    const int row = t.row0 + col;
+    const int see = min(row < t.q_end ? prompt_sees(a, t, row) : 0, k_hi);
+    const int see_least = uniform(min(prompt_sees(a, t, t.row0), k_hi));
+
+    // a request is 1024 bytes: 512 / HD rows; the swizzles repeat every 16 rows (K) and every 4 (V)
+    constexpr int kChunks = HD / 8, kRequests = kTile * 2 / 1024, kReqRows = 512 / HD;
+    constexpr int kKOff = 16 / kReqRows < 1 ? 1 : 16 / kReqRows, kVOff = 4 / kReqRows < 1 ? 1 : 4 / kReqRows;
+    uint32_t k_off[kKOff], v_off[kVOff];
+#pragma unroll
+    for (int u = 0; u < kKOff; u++) {
+        const int r = u * kReqRows + lane / kChunks, ch = lane % kChunks;
+        k_off[u] = (uint32_t)(r * a.st.k_token + (ch ^ swizzle_k<HD>(r)) * 8) * 2u;
+        if (u < kVOff) v_off[u] = (uint32_t)(r * a.st.v_token + (ch ^ swizzle_v<HD>(r)) * 8) * 2u;
+    }
+    const uint16_t *k_base = a.k + (int64_t)t.k_first * a.st.k_token + (int64_t)kvh * a.st.k_head;
+    const uint16_t *v_base = a.v + (int64_t)t.k_first * a.st.v_token + (int64_t)kvh * a.st.v_head;
+    uint16_t *kt = lds + wave * 2 * kTile, *vt = kt + kTile;
+    const uint32_t k_to = lds_address(kt), v_to = lds_address(vt);
+    auto request_k = [&](int k0) {
+        const int4_t r = prompt_resource<HD>(k_base + (int64_t)k0 * a.st.k_token, a.st.k_token, min(t.k_len - k0, kStep));
+#pragma unroll
+        for (int u = 0; u < kRequests; u++)
+            load_to_lds(k_off[u % kKOff] + (uint32_t)(u / kKOff * kKOff * kReqRows * (int)a.st.k_token * 2), r, k_to + u * 1024u);
+    };
+    auto request_v = [&](int k0) {
+        const int4_t r = prompt_resource<HD>(v_base + (int64_t)k0 * a.st.v_token, a.st.v_token, min(t.k_len - k0, kStep));
+#pragma unroll
+        for (int u = 0; u < kRequests; u++)
+            load_to_lds(v_off[u % kVOff] + (uint32_t)(u / kVOff * kVOff * kReqRows * (int)a.st.v_token * 2), r, v_to + u * 1024u);
+    };
+
+    constexpr int kStride = 4 * kStep;
+    int k0 = k_lo + wave * kStep;
+    if (k0 < k_hi) {
+        request_k(k0);
+        request_v(k0);
+    }
+    PromptWave<HD, T, kStep> w;
+    w.begin(a, t, row, head);
+    w.settle();
+    for (; k0 < k_hi; k0 += kStride) {
+        const bool more = k0 + kStride < k_hi;
+        wait_for_lds_loads_but<kRequests>();               // K is there (V was asked for behind it)
+        float16_t s[kStep / 32];
+        w.scores(kt, s);
+        wait_for_lds_reads();
+        if (more) request_k(k0 + kStride);
+        if (k0 + kStep > see_least) w.mask(s, see - k0);
+        const float off = w.bound(s, a.c);
+        uint32_t p[kStep / 32][8];
+        w.weights(s, a.c, off, p);
+        if (more) wait_for_lds_loads_but<kRequests>();     // V is there (the next K was asked for behind it)
+        else wait_for_lds_loads();
+        w.product(vt, p);
+        wait_for_lds_reads();
+        if (more) request_v(k0 + kStride);
+    }
+
+    // the waves join: sums to where K and V were, row by row (four floats of padding where there is room: rows on different banks)
+    float *mine = reinterpret_cast<float *>(kt);
+    const bool odd = w.odd();
+    const float l = halves_sum(w.l);
+    __syncthreads();                                       // s_odd is cleared
+    if (odd && lane == 0) s_odd = 1;
+#pragma unroll
+    for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+            *reinterpret_cast<float4 *>(mine + col * kJoinRow + 32 * d + 8 * b + 4 * c) =
+                make_float4(w.acc[d][4 * b], w.acc[d][4 * b + 1], w.acc[d][4 * b + 2], w.acc[d][4 * b + 3]);
+    if (c == 0) {
+        s_ml[wave][col][0] = l == 0.f ? -INFINITY : w.m;
+        s_ml[wave][col][1] = l;
+    }
+    __syncthreads();
+    if (s_odd) {
+        prompt_rows_plain<HD, T>(a, t, t.row0 + 8 * wave, 8, head, kvh, k_lo, k_hi, split);
+        return;
+    }
+    constexpr int kRowChunks = HD / 8;
+    for (int i = tid; i < kNarrowRows * kRowChunks; i += kPromptThreads) {
+        const int r = i / kRowChunks, d = i % kRowChunks * 8;
+        if (t.row0 + r >= t.q_end) break;
+        const float M = fmaxf(fmaxf(s_ml[0][r][0], s_ml[1][r][0]), fmaxf(s_ml[2][r][0], s_ml[3][r][0]));
+        float den = 0.f, num[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) num[u] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float mj = s_ml[j][r][0];
+            const float f = mj == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mj - M);
+            den = fmaf(s_ml[j][r][1], f, den);
+            const float *src = reinterpret_cast<const float *>(lds + j * 2 * kTile) + r * kJoinRow + d;
+#pragma unroll
+            for (int u = 0; u < 8; u++) num[u] = fmaf(src[u], f, num[u]);
+        }
+        const int64_t at = (int64_t)(t.row0 + r) * a.heads + head;
+        if (a.splits > 1) {
+            const int64_t pa = at * a.splits + split;
+            float4 *o = reinterpret_cast<float4 *>(a.part_acc + pa * HD + d);
+            o[0] = make_float4(num[0], num[1], num[2], num[3]);
+            o[1] = make_float4(num[4], num[5], num[6], num[7]);
+            if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * pa) = make_float2(M, den);
+            continue;
+        }
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        *reinterpret_cast<uint4 *>(a.out + (int64_t)(t.row0 + r) * a.st.out_token + (int64_t)head * a.st.out_head + d) =
+            make_uint4(T::pack(num[0] * inv, num[1] * inv), T::pack(num[2] * inv, num[3] * inv), T::pack(num[4] * inv, num[5] * inv), T::pack(num[6] * inv, num[7] * inv));
+        if (a.lse && d == 0) a.lse[at] = den == 0.f ? -INFINITY : (M + log2f(den)) * 0.693147180559945f;
+    }
 }
 
 // Joins the pieces of a row, a workgroup per (row, head).  The rows are found as the kernel above found them: rows of no
@@ -429,10 +627,8 @@ __global__ __launch_bounds__(kJoinThreads) void attn_prompt_merge_kernel(const P
 {
     const int head = blockIdx.y;
     PromptTile t;
-    if (!find_tile(a, blockIdx.x / kRows, t)) return;
-    int ks, lk;
-    if (!find_keys(a, t, ks, lk)) return;
-    const int row = t.row0 + blockIdx.x % kRows;
+    if (!find_tile<kNarrowRows>(a, blockIdx.x / kNarrowRows, t)) return;
+    const int row = t.row0 + blockIdx.x % kNarrowRows;
     if (row >= t.q_end) return;
     const int64_t at = (int64_t)row * a.heads + head;
     float M, l;
@@ -444,26 +640,44 @@ __global__ __launch_bounds__(kJoinThreads) void attn_prompt_merge_kernel(const P
 
 template <int HD>
 static constexpr size_t prompt_lds() { return (size_t)2 * 2 * kKeys * HD * 2; }
+template <int HD>
+static constexpr size_t narrow_lds() { return (size_t)4 * 2 * kNarrowKeys<HD> * HD * 2; }
+
+template <int HD, class T>
+static int prepare_prompt()
+{
+    const int rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<HD, T>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<HD>());
+    if (rc) return rc;
+    return (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_narrow_kernel<HD, T>), hipFuncAttributeMaxDynamicSharedMemorySize, narrow_lds<HD>());
+}
 
 int prepare_attn_prompt()
 {
     int rc;
-    if ((rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<128, TypeF16>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<128>()))) return rc;
-    if ((rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<128, TypeBf16>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<128>()))) return rc;
-    if ((rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<256, TypeF16>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<256>()))) return rc;
-    return (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<256, TypeBf16>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<256>());
+    if ((rc = prepare_prompt<64, TypeF16>())) return rc;
+    if ((rc = prepare_prompt<64, TypeBf16>())) return rc;
+    if ((rc = prepare_prompt<128, TypeF16>())) return rc;
+    if ((rc = prepare_prompt<128, TypeBf16>())) return rc;
+    if ((rc = prepare_prompt<256, TypeF16>())) return rc;
+    return prepare_prompt<256, TypeBf16>();
 }
 
-// Pieces a row's keys are cut into.  A call with fewer workgroups (128 rows of a head each) than compute units leaves
-// most of the chip idle and its workgroups with long walks: the keys are then split so that about two workgroups a
-// unit run, none with fewer than 256 keys of the longest sequence, and a second launch joins the pieces.
-static int prompt_splits(int64_t tiles, int64_t heads, int64_t max_k, int cus)
+struct PromptPlan {
+    bool narrow;
+    int tiles, splits;
+};
+
+static PromptPlan prompt_plan(int64_t seqs, int64_t total_q, int64_t heads, int64_t max_k, int cus)
 {
-    const int64_t groups = tiles * heads;
-    if (groups >= cus) return 1;
-    int64_t n = (2 * (int64_t)cus + groups - 1) / groups;
-    if (n > max_k / 256) n = max_k / 256;
-    return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+    PromptPlan p = {false, (int)(total_q / kRows + seqs), 1};
+    if (p.tiles * heads >= 2 * cus) return p;
+    p.narrow = true;
+    p.tiles = (int)(total_q / kNarrowRows + seqs);
+    const int64_t groups = p.tiles * heads;
+    int64_t n = (cus + groups - 1) / groups;
+    if (n > max_k / 512) n = max_k / 512;
+    p.splits = n < 1 ? 1 : n > 64 ? 64 : (int)n;
+    return p;
 }
 
 static int prompt_sizes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads, int64_t hd)
@@ -471,17 +685,21 @@ static int prompt_sizes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t 
     if (seqs < 1 || total_q < 1 || total_k < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0) return RPTC_ESHAPE;
     if (hd != 32 && hd != 64 && hd != 128 && hd != 256) return RPTC_ESHAPE;
     if (heads > 1024 || seqs > (1 << 20) || total_q > (1 << 24) || total_k >= ((int64_t)1 << 31) - 64) return RPTC_ELIMIT;
-    if ((total_q / kRows + seqs) * heads >= (int64_t)1 << 23) return RPTC_ELIMIT;      // workgroups of one launch
+    if ((total_q / kNarrowRows + seqs) * heads >= (int64_t)1 << 23) return RPTC_ELIMIT;      // workgroups of one launch
     return 0;
 }
 
 template <int HD, class T>
-static void launch_prompt(const PromptArgs &a, hipStream_t s)
+static void launch_prompt(const PromptArgs &a, bool narrow, hipStream_t s)
 {
-    const int items = a.heads * a.tiles * a.splits;
-    hipLaunchKernelGGL((attn_prompt_kernel<HD, T>), dim3((unsigned)((items + 7) / 8 * 8)), dim3(kPromptThreads), prompt_lds<HD>(), s, a);
+    const dim3 grid((unsigned)(a.heads * a.tiles * a.splits));
+    if (!narrow) {
+        hipLaunchKernelGGL((attn_prompt_kernel<HD, T>), grid, dim3(kPromptThreads), prompt_lds<HD>(), s, a);
+        return;
+    }
+    hipLaunchKernelGGL((attn_prompt_narrow_kernel<HD, T>), grid, dim3(kPromptThreads), narrow_lds<HD>(), s, a);
     if (a.splits > 1)
-        hipLaunchKernelGGL((attn_prompt_merge_kernel<HD, T>), dim3((unsigned)a.tiles * kRows, (unsigned)a.heads), dim3(kJoinThreads), 0, s, a);
+        hipLaunchKernelGGL((attn_prompt_merge_kernel<HD, T>), dim3((unsigned)a.tiles * kNarrowRows, (unsigned)a.heads), dim3(kJoinThreads), 0, s, a);
 }
 
 }  // namespace rptc
@@ -495,7 +713,7 @@ extern "C" int64_t rptc_attn_prompt_workspace_bytes(int64_t seqs, int64_t total_
     if (rc) return rc;
     DeviceInfo *dev;
     if ((rc = device_info(&dev))) return rc < 0 ? rc : RPTC_EDEVICE;
-    const int splits = prompt_splits(total_q / kRows + seqs, heads, max_k < total_k ? max_k : total_k, dev->cus);
+    const int splits = prompt_plan(seqs, total_q, heads, max_k < total_k ? max_k : total_k, dev->cus).splits;
     return splits > 1 ? (int64_t)splits * total_q * heads * (hd + 2) * 4 : 0;
 }
 
@@ -538,8 +756,9 @@ extern "C" int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint
     a.total_k = (int)total_k;
     a.heads = (int)heads;
     a.kv_heads = (int)kv_heads;
-    a.tiles = (int)(total_q / kRows + seqs);
-    a.splits = prompt_splits(a.tiles, heads, max_k < total_k ? max_k : total_k, dev->cus);
+    const PromptPlan plan = prompt_plan(seqs, total_q, heads, max_k < total_k ? max_k : total_k, dev->cus);
+    a.tiles = plan.tiles;
+    a.splits = plan.splits;
     a.causal = causal ? 1 : 0;
     a.c = scale * 1.44269504088896f;
     a.part_acc = a.part_ml = nullptr;
@@ -556,10 +775,10 @@ extern "C" int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint
     if ((rc = timer.begin(dev, s, ms))) return rc;
     const bool f16 = dtype == RPTC_F16;
     switch (hd) {
-    case 32: f16 ? launch_prompt<32, TypeF16>(a, s) : launch_prompt<32, TypeBf16>(a, s); break;
-    case 64: f16 ? launch_prompt<64, TypeF16>(a, s) : launch_prompt<64, TypeBf16>(a, s); break;
-    case 128: f16 ? launch_prompt<128, TypeF16>(a, s) : launch_prompt<128, TypeBf16>(a, s); break;
-    default: f16 ? launch_prompt<256, TypeF16>(a, s) : launch_prompt<256, TypeBf16>(a, s); break;
+    case 32: f16 ? launch_prompt<32, TypeF16>(a, plan.narrow, s) : launch_prompt<32, TypeBf16>(a, plan.narrow, s); break;
+    case 64: f16 ? launch_prompt<64, TypeF16>(a, plan.narrow, s) : launch_prompt<64, TypeBf16>(a, plan.narrow, s); break;
+    case 128: f16 ? launch_prompt<128, TypeF16>(a, plan.narrow, s) : launch_prompt<128, TypeBf16>(a, plan.narrow, s); break;
+    default: f16 ? launch_prompt<256, TypeF16>(a, plan.narrow, s) : launch_prompt<256, TypeBf16>(a, plan.narrow, s); break;
     }
     return timer.end();
 }
