@@ -212,7 +212,11 @@ __device__ __forceinline__ void prompt_rows_plain(const PromptArgs &a, const Pro
         auto score = [&](int j) {
             const uint16_t *k = a.k + (int64_t)(t.k_first + j) * a.st.k_token + (int64_t)kvh * a.st.k_head;
             float s = 0.f;
-            for (int d = 0; d < HD; d++) s = fmaf(T::to_float(q[d]), T::to_float(k[d]), s);
+            for (int d = 0; d < HD; d += 8) {
+                const short8_t qv = *reinterpret_cast<const short8_t *>(q + d), kv = *reinterpret_cast<const short8_t *>(k + d);
+#pragma unroll
+                for (int u = 0; u < 8; u++) s = fmaf(T::to_float((uint16_t)qv[u]), T::to_float((uint16_t)kv[u]), s);
+            }
             return s;
         };
         float m = -INFINITY;
@@ -252,7 +256,9 @@ __device__ __forceinline__ void prompt_rows_plain(const PromptArgs &a, const Pro
 
 // What a wave holds of 32 query rows, and the parts of a step over KEYS keys (a multiple of 32).  Lane (col, c): row col; of
 // every eight keys and of every eight dimensions the four from 4c on.
-template <int HD, class T, int KEYS>
+// TERMS = 2: p enters the product as the sum of two numbers of the type (its rounding and what that left), so that
+// the output's own rounding is what is left: for the calls that leave the matrix unit idle.
+template <int HD, class T, int KEYS, int TERMS>
 struct PromptWave {
     static constexpr int kSteps = HD / 16, kDims = HD / 32, kBlocks = KEYS / 32;
     short8_t qf[kSteps];
@@ -321,7 +327,7 @@ struct PromptWave {
         return m == -INFINITY ? 0.f : m;
     }
     // p = exp2(c s - bound), packed in pairs of keys
-    __device__ __forceinline__ void weights(const float16_t (&s)[kBlocks], float scale, float off, uint32_t (&p)[kBlocks][8])
+    __device__ __forceinline__ void weights(const float16_t (&s)[kBlocks], float scale, float off, uint32_t (&p)[TERMS][kBlocks][8])
     {
 #pragma unroll
         for (int h = 0; h < kBlocks; h++)
@@ -330,11 +336,15 @@ struct PromptWave {
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(s[h][r], scale, -off)), p1 = __builtin_amdgcn_exp2f(fmaf(s[h][r + 1], scale, -off));
                 l += p0;
                 l += p1;
-                p[h][r / 2] = T::pack(p0, p1);
+                p[0][h][r / 2] = T::pack(p0, p1);
+                if (TERMS > 1) {
+                    const uint32_t w = p[0][h][r / 2];
+                    p[TERMS - 1][h][r / 2] = T::pack(p0 - T::to_float((uint16_t)w), p1 - T::to_float((uint16_t)(w >> 16)));
+                }
             }
     }
     // acc += V^T P^T, V in LDS at vt: the lane's dimension of a tile of 32, keys in the order the scores' registers have them
-    __device__ __forceinline__ void product(const uint16_t *vt, const uint32_t (&p)[kBlocks][8])
+    __device__ __forceinline__ void product(const uint16_t *vt, const uint32_t (&p)[TERMS][kBlocks][8])
     {
         typedef __attribute__((address_space(3))) short4_t lds_short4;
         const int lane = threadIdx.x & 63, c = lane >> 5, g16 = lane >> 4, rr = (lane & 15) >> 2, piece = lane & 3;
@@ -342,7 +352,9 @@ struct PromptWave {
         for (int h = 0; h < kBlocks; h++)
 #pragma unroll
             for (int g = 0; g < 2; g++) {
-                const uint4 pv = make_uint4(p[h][4 * g], p[h][4 * g + 1], p[h][4 * g + 2], p[h][4 * g + 3]);
+                uint4 pv[TERMS];
+#pragma unroll
+                for (int u = 0; u < TERMS; u++) pv[u] = make_uint4(p[u][h][4 * g], p[u][h][4 * g + 1], p[u][h][4 * g + 2], p[u][h][4 * g + 3]);
                 const int key = 32 * h + 16 * g + 4 * c + rr;
 #pragma unroll
                 for (int d = 0; d < kDims; d++) {
@@ -350,7 +362,9 @@ struct PromptWave {
                     const uint16_t *va = vt + key * HD + ch * 8 + (piece & 1) * 4;
                     const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)va);
                     const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4 *)(va + 8 * HD));
-                    acc[d] = T::mfma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), __builtin_bit_cast(short8_t, pv), acc[d]);
+#pragma unroll
+                    for (int u = 0; u < TERMS; u++)
+                        acc[d] = T::mfma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), __builtin_bit_cast(short8_t, pv[u]), acc[d]);
                 }
             }
     }
@@ -428,7 +442,7 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
         request_v(0, 0);
         if (kKeys < k_hi) request_k(kKeys, 1);
     }
-    PromptWave<HD, T, kKeys> w;
+    PromptWave<HD, T, kKeys, 1> w;
     w.begin(a, t, row, head);
     w.settle();
     // One step: the softmax of the scores s of the keys from k0 on and their product with V, while the matrix unit forms the
@@ -442,7 +456,7 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
         if (k0 + kKeys > see_least) w.mask(s, see - k0);   // some row of the wave does not see all of the step's keys
         const float off = w.bound(s, a.c);
         w.scores(lds + (buf ^ 1) * kTile, next);
-        uint32_t p[2][8];
+        uint32_t p[1][2][8];
         w.weights(s, a.c, off, p);
         w.product(lds + (2 + buf) * kTile, p);
     };
@@ -545,7 +559,7 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
         request_k(k0);
         request_v(k0);
     }
-    PromptWave<HD, T, kStep> w;
+    PromptWave<HD, T, kStep, 2> w;
     w.begin(a, t, row, head);
     w.settle();
     for (; k0 < k_hi; k0 += kStride) {
@@ -557,7 +571,7 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
         if (more) request_k(k0 + kStride);
         if (k0 + kStep > see_least) w.mask(s, see - k0);
         const float off = w.bound(s, a.c);
-        uint32_t p[kStep / 32][8];
+        uint32_t p[2][kStep / 32][8];
         w.weights(s, a.c, off, p);
         if (more) wait_for_lds_loads_but<kRequests>();     // V is there (the next K was asked for behind it)
         else wait_for_lds_loads();
@@ -667,14 +681,27 @@ struct PromptPlan {
     int tiles, splits;
 };
 
-static PromptPlan prompt_plan(int64_t seqs, int64_t total_q, int64_t heads, int64_t max_k, int cus)
+// sequences cut into tiles: at most so many (whatever the sequences' lengths are)
+static int64_t prompt_tiles(int64_t seqs, int64_t total_q, int64_t rows) { return (total_q + seqs * (rows - 1)) / rows; }
+
+// Which of the two kernels, by the estimates that the measurements below fit (us; steps: 64 keys of the longest walk):
+// a workgroup of 128 rows takes 6 + 1 a step whether its compute unit has one or two of them, one of 32 rows 8 + 0.4 a step
+// (its four waves share the walk, but also fetch four times the K and V a row: later rounds of them, half as long on
+// average where they are causal, cost more than their share).  Measured (128 rows / 32 rows): 512 rows of 32 heads x 128
+// 15.4 / 18.7, 1024 rows 25.7 / 41, 2300 rows of 8 heads 43.7 / 37.5, of 2 heads 42.4 / 26.8, 1000 rows of 16 heads x 64 17.5 / 10.5,
+// 37 rows of 32 heads 6.7 / 8.4, 32 rows behind 8000 124 / 30 (split).  The keys of a call that leaves compute units without a
+// workgroup are split, not below 512 a piece, and a second launch joins the pieces.
+static PromptPlan prompt_plan(int64_t seqs, int64_t total_q, int64_t heads, int64_t hd, int64_t max_k, int cus)
 {
-    PromptPlan p = {false, (int)(total_q / kRows + seqs), 1};
-    if (p.tiles * heads >= 2 * cus) return p;
+    PromptPlan p = {false, (int)prompt_tiles(seqs, total_q, kRows), 1};
+    const double steps = (double)(max_k + 63) / 64;
+    const double wide = (double)p.tiles * heads / (2.0 * cus);
+    const int64_t tiles = prompt_tiles(seqs, total_q, kNarrowRows), slots = (int64_t)cus * (hd > 64 ? 1 : 2);
+    const double rounds = (double)tiles * heads / (double)slots < 1 ? 1 : (double)tiles * heads / (double)slots;
+    if (6 + steps * (wide < 1 ? 1 : wide) <= 8 * rounds + 0.2 * steps * (1 + rounds)) return p;
     p.narrow = true;
-    p.tiles = (int)(total_q / kNarrowRows + seqs);
-    const int64_t groups = p.tiles * heads;
-    int64_t n = (cus + groups - 1) / groups;
+    p.tiles = (int)tiles;
+    int64_t n = slots / (tiles * heads);
     if (n > max_k / 512) n = max_k / 512;
     p.splits = n < 1 ? 1 : n > 64 ? 64 : (int)n;
     return p;
@@ -685,7 +712,7 @@ static int prompt_sizes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t 
     if (seqs < 1 || total_q < 1 || total_k < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0) return RPTC_ESHAPE;
     if (hd != 32 && hd != 64 && hd != 128 && hd != 256) return RPTC_ESHAPE;
     if (heads > 1024 || seqs > (1 << 20) || total_q > (1 << 24) || total_k >= ((int64_t)1 << 31) - 64) return RPTC_ELIMIT;
-    if ((total_q / kNarrowRows + seqs) * heads >= (int64_t)1 << 23) return RPTC_ELIMIT;      // workgroups of one launch
+    if (prompt_tiles(seqs, total_q, kNarrowRows) * heads >= (int64_t)1 << 23) return RPTC_ELIMIT;      // workgroups of one launch
     return 0;
 }
 
@@ -713,7 +740,7 @@ extern "C" int64_t rptc_attn_prompt_workspace_bytes(int64_t seqs, int64_t total_
     if (rc) return rc;
     DeviceInfo *dev;
     if ((rc = device_info(&dev))) return rc < 0 ? rc : RPTC_EDEVICE;
-    const int splits = prompt_plan(seqs, total_q, heads, max_k < total_k ? max_k : total_k, dev->cus).splits;
+    const int splits = prompt_plan(seqs, total_q, heads, hd, max_k < total_k ? max_k : total_k, dev->cus).splits;
     return splits > 1 ? (int64_t)splits * total_q * heads * (hd + 2) * 4 : 0;
 }
 
@@ -756,7 +783,7 @@ extern "C" int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint
     a.total_k = (int)total_k;
     a.heads = (int)heads;
     a.kv_heads = (int)kv_heads;
-    const PromptPlan plan = prompt_plan(seqs, total_q, heads, max_k < total_k ? max_k : total_k, dev->cus);
+    const PromptPlan plan = prompt_plan(seqs, total_q, heads, hd, max_k < total_k ? max_k : total_k, dev->cus);
     a.tiles = plan.tiles;
     a.splits = plan.splits;
     a.causal = causal ? 1 : 0;
