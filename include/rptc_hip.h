@@ -444,7 +444,7 @@ int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint16_t *v, ui
  *                         contiguous.  A sequence whose position lies outside [0, max_len) (a padded batch) is left unwritten.
  *                         workspace: rptc_kv4_attn_decode_workspace_bytes(...) bytes, 16-byte aligned (0: may be NULL),
  *                         no initialisation; calls that may overlap need one each.
- * At most 65535 sequences, 1024 heads, 2^26 positions; q_out, out and the caches must not overlap the inputs.
+ * At most 65535 sequences, 1024 heads (2^22 key heads of all sequences together), 2^26 positions; q_out, out and the caches must not overlap the inputs.
  */
 int64_t rptc_kv4_row_bytes(int64_t hd);
 int rptc_kv4_append(const uint16_t *k, const uint16_t *v, uint8_t *k_cache, uint8_t *v_cache, const int64_t *pos,

@@ -15,6 +15,7 @@
 // factor of a row is a factor of a lane.  K and V come from memory straight into LDS (two buffers, 16 bytes a lane);
 // V^T is read with the transposing LDS read.
 #include "join.hpp"
+#include "lds_load.hpp"
 
 namespace rptc {
 
@@ -24,7 +25,6 @@ constexpr int kKeys = 64;              // keys of a step
 constexpr float kLazy = 8.f;           // exponents of 2 a score may exceed the running bound by
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
-typedef int int4_t __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef short short8_t __attribute__((ext_vector_type(8)));
 typedef float float2_t __attribute__((ext_vector_type(2)));
@@ -73,9 +73,6 @@ struct PromptTile {
     int seq, q_begin, q_end, row0;     // the sequence's query rows, the tile's first row
     int k_first, k_len;                // and its keys
 };
-
-// A value every lane of the wave holds, as one the compiler knows to be such (scalar registers, scalar branches).
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // The sequence that holds tile `tile` when every sequence is cut into tiles of ROWS query rows: 64 sequences at a time, a
 // lane each.  A sequence's tiles are taken from its end (the longest rows of a causal prompt first).  The starts come from
@@ -146,29 +143,6 @@ __device__ __forceinline__ void prompt_item(const PromptArgs &a, int &head, int 
     head = local - rest * run + (runs ? (blockIdx.x & 7) * run : 0);
     tile = rest / a.splits;
     split = rest - tile * a.splits;
-}
-
-// 16 bytes a lane from `offset` of the buffer to LDS at `to` + 16 lane (no register receives anything: the request may
-// stay in flight behind the statement).  As assembly because the compiler, which cannot tell the two buffers in LDS
-// apart, waits for such a request in front of the next transposing LDS read, which reads the other buffer.  (m0 is
-// reserved for such single uses: the compiler sets it in front of each of its own.)
-__device__ __forceinline__ void load_to_lds(uint32_t offset, int4_t resource, uint32_t to)
-{
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(offset), "s"(resource), "s"(to) : "memory");
-}
-__device__ __forceinline__ void wait_for_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-// all but the N requests made last
-template <int N>
-__device__ __forceinline__ void wait_for_lds_loads_but()
-{
-    static_assert(N < 64, "the counter has six bits");
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-// what was read from LDS is in registers: its place may be written over
-__device__ __forceinline__ void wait_for_lds_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ uint32_t lds_address(const void *p)
-{
-    return (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p);
 }
 
 // x of the lane 32 away, in both halves of the wave: returns op(own, other)
@@ -380,15 +354,6 @@ struct PromptWave {
     }
 };
 
-// the buffer descriptor of `rows` rows, in scalar registers; what lies at or past its end reads as zero
-template <int HD>
-__device__ __forceinline__ int4_t prompt_resource(const uint16_t *base, int64_t token, int rows)
-{
-    const uint64_t p = reinterpret_cast<uint64_t>(base);
-    const int4_t r = {uniform((int)p), uniform((int)(p >> 32) & 0xFFFF), uniform(((rows - 1) * (int)token + HD) * 2), 0x00027000};
-    return r;
-}
-
 // Many rows: 128 query rows of a head a workgroup, 32 a wave; all waves walk over the same keys, which are brought to LDS
 // once for the four of them, a step ahead.
 template <int HD, class T>
@@ -427,12 +392,12 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
     const uint16_t *v_base = a.v + (int64_t)t.k_first * a.st.v_token + (int64_t)kvh * a.st.v_head;
     const uint32_t lds_base = lds_address(lds) + (uint32_t)wave * 1024u;
     auto request_k = [&](int k0, int buf) {
-        const int4_t r = prompt_resource<HD>(k_base + (int64_t)k0 * a.st.k_token, a.st.k_token, min(t.k_len - k0, kKeys));
+        const int4_t r = buffer_resource(k_base + (int64_t)k0 * a.st.k_token, ((min(t.k_len - k0, kKeys) - 1) * (int)a.st.k_token + HD) * 2);
 #pragma unroll
         for (int u = 0; u < kRequests; u++) load_to_lds(k_off[u], r, lds_base + (uint32_t)buf * (2u * kTile) + u * 4096u);
     };
     auto request_v = [&](int k0, int buf) {
-        const int4_t r = prompt_resource<HD>(v_base + (int64_t)k0 * a.st.v_token, a.st.v_token, min(t.k_len - k0, kKeys));
+        const int4_t r = buffer_resource(v_base + (int64_t)k0 * a.st.v_token, ((min(t.k_len - k0, kKeys) - 1) * (int)a.st.v_token + HD) * 2);
 #pragma unroll
         for (int u = 0; u < kRequests; u++) load_to_lds(v_off[u], r, lds_base + (uint32_t)(2 + buf) * (2u * kTile) + u * 4096u);
     };
@@ -541,13 +506,13 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
     uint16_t *kt = lds + wave * 2 * kTile, *vt = kt + kTile;
     const uint32_t k_to = lds_address(kt), v_to = lds_address(vt);
     auto request_k = [&](int k0) {
-        const int4_t r = prompt_resource<HD>(k_base + (int64_t)k0 * a.st.k_token, a.st.k_token, min(t.k_len - k0, kStep));
+        const int4_t r = buffer_resource(k_base + (int64_t)k0 * a.st.k_token, ((min(t.k_len - k0, kStep) - 1) * (int)a.st.k_token + HD) * 2);
 #pragma unroll
         for (int u = 0; u < kRequests; u++)
             load_to_lds(k_off[u % kKOff] + (uint32_t)(u / kKOff * kKOff * kReqRows * (int)a.st.k_token * 2), r, k_to + u * 1024u);
     };
     auto request_v = [&](int k0) {
-        const int4_t r = prompt_resource<HD>(v_base + (int64_t)k0 * a.st.v_token, a.st.v_token, min(t.k_len - k0, kStep));
+        const int4_t r = buffer_resource(v_base + (int64_t)k0 * a.st.v_token, ((min(t.k_len - k0, kStep) - 1) * (int)a.st.v_token + HD) * 2);
 #pragma unroll
         for (int u = 0; u < kRequests; u++)
             load_to_lds(v_off[u % kVOff] + (uint32_t)(u / kVOff * kVOff * kReqRows * (int)a.st.v_token * 2), r, v_to + u * 1024u);

@@ -10,19 +10,27 @@ constexpr int kJoinThreads = 256, kJoinMost = 128;
 #ifdef __HIPCC__
 // One workgroup, one row: acc [pieces][hd] and ml [pieces][2] (bound in log2 units and sum; sum 0 = the piece holds no key).
 // Returns the numerator of dimension threadIdx.x (threads below hd); M and the denominator in every thread.  Every
-// thread of the workgroup calls it.  The factors come first, one piece a thread; then 256 / hd groups of threads take
-// every so-manieth piece, eight requests in flight, and are added up in a fixed order.
+// thread of the workgroup calls it.  256 / hd groups of threads take every so-manieth piece and are added up in a fixed
+// order; the first 16 of a thread are asked for before the factors are worked out, one piece a thread, so that a row of
+// up to 32 pieces at hd 128 costs one trip to memory.
 __device__ __forceinline__ float join_pieces(const float *__restrict__ acc, const float *__restrict__ ml, int pieces, int hd,
                                              float &M, float &den)
 {
+    constexpr int kAhead = 16;
     __shared__ float s_f[kJoinMost], s_red[2 * kJoinThreads / 64], s_part[kJoinThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    float m = -INFINITY, l = 0.f;
+    const int groups = kJoinThreads / hd, g = tid / hd, dim = tid - g * hd;
+    float m = -INFINITY, l = 0.f, v[kAhead];
     if (tid < pieces) {
-        const float2 v = reinterpret_cast<const float2 *>(ml)[tid];
-        m = v.x;
-        l = v.y;
+        const float2 w = reinterpret_cast<const float2 *>(ml)[tid];
+        m = w.x;
+        l = w.y;
     }
+    auto ask = [&](int i0) {                   // (a piece past the last: the last once more, with factor 0)
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) v[u] = acc[min(i0 + u * groups, pieces - 1) * hd + dim];
+    };
+    ask(g);
     float mx = m;
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
@@ -38,14 +46,11 @@ __device__ __forceinline__ float join_pieces(const float *__restrict__ acc, cons
     if (lane == 0) s_red[kJoinThreads / 64 + wave] = d;
     __syncthreads();
     den = s_red[kJoinThreads / 64] + s_red[kJoinThreads / 64 + 1];
-    const int groups = kJoinThreads / hd, g = tid / hd, dim = tid - g * hd;
     float num = 0.f;
-    for (int i0 = g; i0 < pieces; i0 += 8 * groups) {
-        float v[8];
+    for (int i0 = g; i0 < pieces; i0 += kAhead * groups) {
+        if (i0 != g) ask(i0);
 #pragma unroll
-        for (int u = 0; u < 8; u++) v[u] = i0 + u * groups < pieces ? acc[(int64_t)(i0 + u * groups) * hd + dim] : 0.f;
-#pragma unroll
-        for (int u = 0; u < 8; u++)
+        for (int u = 0; u < kAhead; u++)
             if (i0 + u * groups < pieces) num = fmaf(v[u], s_f[i0 + u * groups], num);
     }
     s_part[tid] = num;

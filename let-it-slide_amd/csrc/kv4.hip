@@ -9,10 +9,13 @@
 // holds the values 8w .. 8w+7, nibble t the value 8w + 2t and nibble t + 4 the value 8w + 2t + 1: one mask of a word gives a
 // pair of neighbours in the two halves of a register.
 #include "join.hpp"
+#include "lds_load.hpp"
 
 namespace rptc {
 
 constexpr int kKv4Group = 32;
+constexpr int kKv4Tile = 32;                // positions a wave takes at a time
+typedef float float2v_t __attribute__((ext_vector_type(2)));
 typedef float float4v_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half8v_t __attribute__((ext_vector_type(8)));
 
@@ -22,36 +25,29 @@ __device__ __forceinline__ half2_t as_half2(uint32_t w) { return __builtin_bit_c
 __device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-// Nibbles 0, 1, 2, 3 of both halves of w as pairs of fp16 numbers: the bits of a code are put into the mantissa of 1024 (at
-// its lowest bits) or of 64 (four bits up, so without a shift), and the power taken off again, exactly.
-template <int N>
-__device__ __forceinline__ void nibble_pairs(uint32_t w, half2_t *c)
+// A byte 0000cccc read as an fp8 number (e4m3) is c / 512, denormal or not, so the conversion of two fp8 numbers with the scale
+// 512 gives two codes as fp16, exactly, in one instruction (against three: into a power's mantissa by mask and or, the
+// power taken off).
+template <bool HIGH>
+__device__ __forceinline__ half2_t byte_codes(uint32_t w)
 {
-    const half2_t k1024 = {(_Float16)1024.f, (_Float16)1024.f}, k64 = {(_Float16)64.f, (_Float16)64.f};
-    c[0] = as_half2((w & 0x000F000Fu) | 0x64006400u) - k1024;
-    if (N > 1) c[1] = as_half2((w & 0x00F000F0u) | 0x54005400u) - k64;
-    if (N > 2) {
-        const uint32_t v = w >> 8;
-        c[2] = as_half2((v & 0x000F000Fu) | 0x64006400u) - k1024;
-        c[3] = as_half2((v & 0x00F000F0u) | 0x54005400u) - k64;
-    }
+    return __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 512.f, HIGH));
 }
 
-// the eight values of a word, in order
-__device__ __forceinline__ half8v_t word_values(uint32_t w, uint32_t par)
+// The eight values of a word, in the order of its bytes' nibbles: 0, 4, 1, 5, 2, 6, 3, 7 (kWordOrder).
+__device__ __forceinline__ void word_values(uint32_t w, uint32_t par, half2_t (&r)[4])
 {
     const half2_t s = as_half2(low_halves(par, par)), m = as_half2(high_halves(par, par));
-    half2_t c[4];
-    nibble_pairs<4>(w, c);
-#pragma unroll
-    for (int t = 0; t < 4; t++) c[t] = __builtin_elementwise_fma(c[t], s, m);
-    half8v_t r;
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-        r[2 * t] = c[t].x;
-        r[2 * t + 1] = c[t].y;
-    }
-    return r;
+    const uint32_t even = w & 0x0F0F0F0Fu, odd = (w >> 4) & 0x0F0F0F0Fu;
+    r[0] = __builtin_elementwise_fma(byte_codes<false>(even), s, m);
+    r[1] = __builtin_elementwise_fma(byte_codes<true>(even), s, m);
+    r[2] = __builtin_elementwise_fma(byte_codes<false>(odd), s, m);
+    r[3] = __builtin_elementwise_fma(byte_codes<true>(odd), s, m);
+}
+__device__ __forceinline__ half8v_t as_half8(const half2_t (&r)[4])
+{
+    const half8v_t v = {r[0].x, r[0].y, r[1].x, r[1].y, r[2].x, r[2].y, r[3].x, r[3].y};
+    return v;
 }
 
 // The codes of a lane's eight values and its group's parameters (four consecutive lanes hold a group).
@@ -167,7 +163,11 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4ReadArgs a)
     const uint32_t par = *reinterpret_cast<const uint32_t *>(row + HD / 2 + word / 4 * 4);
     const int64_t token = (int64_t)seq * a.rows + p;
     uint16_t *out = is_v ? a.v + token * a.v_token + (int64_t)head * a.v_head : a.k + token * a.k_token + (int64_t)head * a.k_head;
-    *reinterpret_cast<half8v_t *>(out + 8 * word) = word_values(code, par);
+    half2_t r[4];
+    word_values(code, par, r);
+    // from the order 0, 4, 1, 5, 2, 6, 3, 7 to the natural one
+    const half2_t v[4] = {{r[0].x, r[1].x}, {r[2].x, r[3].x}, {r[0].y, r[1].y}, {r[2].y, r[3].y}};
+    *reinterpret_cast<half8v_t *>(out + 8 * word) = as_half8(v);
 }
 
 // One token of a decode step: rotates the (2i, 2i+1) pairs of q and k by the angle of the token's position (the fp16
@@ -225,22 +225,98 @@ __global__ __launch_bounds__(256) void kv4_rope_append_kernel(const uint16_t *__
 //   that is raised only where a score exceeds it by more than 2^8).
 // A wave takes 32 positions of one key head at a time, for up to 16 query heads of its group, and needs nothing from
 // another lane but the maxima: S^T = K q^T with 16x16x32 matrix instructions, the lane holding one quarter of a row's
-// words as the row operand (16 bytes of 16 consecutive rows: a run of memory); its result has, in a lane, scores of one head
-// for four positions of each of two tiles, which is, with the positions renumbered accordingly, the operand P of
-// O^T = V^T P^T; V^T's operand wants eight positions of one dimension in a lane, so the lane reads one word (eight
-// dimensions) of its eight rows and pairs the positions up with byte permutes.  Values are formed in fp16, as stored.
+// words as the row operand; its result has, in a lane, scores of one head for four positions of each of two tiles, which is,
+// with the positions renumbered accordingly, the operand P of O^T = V^T P^T; V^T's operand wants eight positions of one
+// dimension in a lane, so the lane reads one word (eight dimensions) of its eight rows and pairs the positions up with byte
+// permutes.  Values are formed in fp16, as stored; p enters the product rounded to fp16, and, where half of the
+// columns are free, what that left enters through them.
+// The 32 rows are a run of memory, and come straight into LDS, two stages a wave in flight (10 KB of them at hd 128, up to
+// 160 KB a compute unit); the row length in words (20 at hd 128) puts the lanes of every LDS read on different banks.
 // The matrix unit is mostly idle (15 of 16 columns with one query head a key head); what counts is the vector unit's work of
-// unpacking, 4 instructions a pair of values, which stays under the time of the bytes.
+// unpacking, about three instructions a pair of values.
 struct Kv4AttnArgs {
     const uint16_t *q;
     const uint8_t *k_cache, *v_cache;
     const int64_t *pos;
     uint16_t *out;
-    float *part;                            // splits > 1: [seq][head][split][hd] sums, then [seq][head][split][2] bound and sum of p
+    float *part;                            // pieces: [head][slot][hd] sums, then [head][slot][2] bound and sum of p
     int64_t q_token, max_len, part_ml;      // part_ml: where the second part begins
-    int heads, kv_heads, group, head_blocks, splits;
+    int seqs, heads, kv_heads, group, head_blocks;
+    int slots;                              // workgroups a key head (block): every sequence takes one a piece
+    int want, least;                        // the pieces of all sequences together that fill the chip; tiles of the shortest
     float c;                                // scale * log2(e)
 };
+
+// How the sequences' positions are cut into pieces, a workgroup each (and key head): pieces of one length, whatever the
+// sequences' own, so that the workgroups of a batch of unequal sequences end together and few are without a piece (one
+// of those holds its place for about 2 us).  The positions come from device memory: every wave works the cut out for
+// itself, a lane a sequence, 64 at a time.  Lengths in tiles of 32 positions (at most 1024 sequences of 2^21).
+struct Kv4Piece {
+    int seq, len, pieces, piece, slot0;     // the sequence, its positions and pieces, which of them, the slot of its first
+};
+__device__ __forceinline__ int kv4_length(const Kv4AttnArgs &a, int s)
+{
+    const int64_t p = s < a.seqs ? a.pos[s] : -1;
+    return p >= 0 && p < a.max_len ? (int)p + 1 : 0;       // a position outside the cache: no piece, nothing is read or written
+}
+// sums over lanes 0 .. own, by DPP (see wave_sum)
+__device__ __forceinline__ uint32_t scan64(uint32_t v)
+{
+#define RPTC_DPP_ADD(ctrl, row_mask) v += __builtin_amdgcn_update_dpp(0u, v, ctrl, row_mask, 0xF, false)
+    RPTC_DPP_ADD(0x111, 0xF);
+    RPTC_DPP_ADD(0x112, 0xF);
+    RPTC_DPP_ADD(0x114, 0xF);
+    RPTC_DPP_ADD(0x118, 0xF);
+    RPTC_DPP_ADD(0x142, 0xA);
+    RPTC_DPP_ADD(0x143, 0xC);
+#undef RPTC_DPP_ADD
+    return v;
+}
+
+// The piece of slot `slot`, or (by_seq) the first piece of sequence `slot`.  False: there is none.
+__device__ __forceinline__ bool kv4_find(const Kv4AttnArgs &a, int slot, bool by_seq, Kv4Piece &r)
+{
+    r.piece = 0;
+    if (a.want == 1) {                                     // nothing is cut
+        r.seq = r.slot0 = slot;
+        r.len = uniform(kv4_length(a, slot));
+        r.pieces = 1;
+        return r.len > 0;
+    }
+    const int lane = threadIdx.x & 63;
+    uint32_t total = 0;
+    int len = 0;
+    for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+        len = kv4_length(a, s0 + lane);
+        total += (uint32_t)(len + kKv4Tile - 1) / kKv4Tile;
+    }
+    total = (uint32_t)__builtin_amdgcn_readlane((int)scan64(total), 63);
+    const uint32_t size = max((uint32_t)a.least, (total + (uint32_t)a.want - 1) / (uint32_t)a.want);      // so at most seqs + want - 1 pieces
+    uint32_t in_front = 0;
+    r.seq = -1;
+    r.len = r.pieces = r.slot0 = 0;
+    for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+        if (a.seqs > 64) len = kv4_length(a, s0 + lane);
+        const uint32_t n = min(((uint32_t)(len + kKv4Tile - 1) / kKv4Tile + size - 1) / size, (uint32_t)kJoinMost);
+        const uint32_t incl = scan64(n);
+        const uint64_t hit = __ballot(by_seq ? s0 + lane == slot : in_front + incl > (uint32_t)slot);
+        if (hit) {
+            const int f = __builtin_ctzll(hit);
+            r.seq = s0 + f;
+            r.len = __builtin_amdgcn_readlane(len, f);
+            r.pieces = __builtin_amdgcn_readlane((int)n, f);
+            r.slot0 = (int)in_front + __builtin_amdgcn_readlane((int)incl, f) - r.pieces;
+            break;
+        }
+        in_front += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+    }
+    r.seq = uniform(r.seq);
+    r.len = uniform(r.len);
+    r.pieces = uniform(r.pieces);
+    r.slot0 = uniform(r.slot0);
+    r.piece = by_seq ? 0 : slot - r.slot0;
+    return r.seq >= 0 && r.pieces > 0;
+}
 
 __device__ __forceinline__ float rows_max(float x)
 {
@@ -261,76 +337,131 @@ __device__ __forceinline__ float rows_sum(float x)
     return __builtin_bit_cast(float, (uint32_t)s[0]) + __builtin_bit_cast(float, (uint32_t)s[1]);
 }
 
-constexpr int kKv4Waves = 8;
-constexpr int kKv4Tile = 32;                // positions a wave takes at a time
+constexpr int kKv4Stages = 2;               // of them on their way or in LDS
 constexpr float kKv4Lazy = 8.f;
+template <int HD>
+constexpr int kKv4Waves = HD > 128 ? 4 : 8;
+template <int HD>
+constexpr int kKv4Stage = kKv4Tile * kv4_row_bytes(HD);     // bytes of K, and of V, of a stage: 640, 1280, 2560, 5120
+template <int HD>
+constexpr int kv4_lds(int live)
+{
+    // the stages, later the waves' sums [wave][column][HD + 4] and [wave][16][2]
+    const int columns = live <= 8 ? 2 * live : live;
+    const int ring = kKv4Waves<HD> * kKv4Stages * 2 * kKv4Stage<HD>, sums = (kKv4Waves<HD> * columns * (HD + 4) + kKv4Waves<HD> * 32) * 4;
+    return ring > sums ? ring : sums;
+}
 
 template <int HD>
-__global__ __launch_bounds__(64 * kKv4Waves) void kv4_attn_kernel(const Kv4AttnArgs a)
+__global__ __launch_bounds__(64 * kKv4Waves<HD>, HD > 128 ? 2 : 4) void kv4_attn_kernel(const Kv4AttnArgs a)
 {
-    extern __shared__ __align__(16) float lds4[];          // [wave][head][HD], then [wave][16][2]
-    constexpr int kRow = kv4_row_bytes(HD);
+    extern __shared__ __align__(16) uint8_t lds4[];
+    constexpr int kRow = kv4_row_bytes(HD), kStage = kKv4Stage<HD>, kWaves = kKv4Waves<HD>;
+    constexpr int kRequests = (kStage + 1023) / 1024, kLastLanes = (kStage % 1024) / 16;      // of a wave's 1024 bytes; lanes of a part of one
     constexpr int kW = HD / 32;                            // words of a row a lane holds of K
     constexpr int kE = HD / 16;                            // dimensions of a row a lane holds of V
     constexpr int kVW = HD >= 128 ? HD / 128 : 1;          // words of that
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int n = lane & 15, c = lane >> 4;
-    const int split = blockIdx.x, kvh = blockIdx.y / a.head_blocks, hb = blockIdx.y % a.head_blocks, seq = blockIdx.z;
-    const int64_t pos = a.pos[seq];
-    // a position outside the cache: nothing is read or written
-    if (pos < 0 || pos >= a.max_len) return;
-    const int64_t len = pos + 1;
-    const int64_t per = ((len + a.splits - 1) / a.splits + kKv4Tile - 1) / kKv4Tile * kKv4Tile;
-    const int64_t lo = split * per, hi = min(len, lo + per);
+    // the heads of a piece together, the slots without a piece at the end: workgroups with one fall on different compute units
+    const int groups = a.kv_heads * a.head_blocks, slot = blockIdx.x / groups, group = blockIdx.x - slot * groups;
+    const int kvh = group / a.head_blocks, hb = group - kvh * a.head_blocks;
     const int live = min(16, a.group - 16 * hb);           // query heads of this workgroup
     const int head0 = kvh * a.group + 16 * hb;
-    const int64_t head_base = ((int64_t)seq * a.kv_heads + kvh) * a.max_len;
+    Kv4Piece r;
+    if (!kv4_find(a, slot, false, r)) return;
+    const int per = ((r.len + r.pieces - 1) / r.pieces + kKv4Tile - 1) / kKv4Tile * kKv4Tile;
+    const int lo = (int)min((int64_t)r.len, (int64_t)r.piece * per), hi = min(r.len, lo + per);
+    const int64_t head_base = ((int64_t)r.seq * a.kv_heads + kvh) * a.max_len;
+    const uint8_t *k_base = a.k_cache + head_base * kRow, *v_base = a.v_cache + head_base * kRow;
 
+    // this wave's tiles: from lo + 32 wave on, every kWaves-th; rows past the piece's end come as zeros
+    const int first = lo + wave * kKv4Tile, tiles = uniform(first < hi ? (hi - first + kWaves * kKv4Tile - 1) / (kWaves * kKv4Tile) : 0);
+    uint8_t *ring = lds4 + wave * (kKv4Stages * 2 * kStage);
+    const uint32_t ring_to = lds_address(ring);
+    auto request = [&](int i) {
+        const int j0 = first + i * kWaves * kKv4Tile, bytes = min(kStage, (hi - j0) * kRow);
+        const int4_t kr = buffer_resource(k_base + (int64_t)j0 * kRow, bytes), vr = buffer_resource(v_base + (int64_t)j0 * kRow, bytes);
+        const uint32_t to = ring_to + (uint32_t)(i % kKv4Stages) * (2u * kStage);
+#pragma unroll
+        for (int u = 0; u < kStage / 1024; u++) load_to_lds(lane * 16u + u * 1024u, kr, to + u * 1024u);
+#pragma unroll
+        for (int u = 0; u < kStage / 1024; u++) load_to_lds(lane * 16u + u * 1024u, vr, to + kStage + u * 1024u);
+        if (lane < kLastLanes) {
+            load_to_lds(lane * 16u + kStage / 1024 * 1024u, kr, to + kStage / 1024 * 1024u);
+            load_to_lds(lane * 16u + kStage / 1024 * 1024u, vr, to + kStage + kStage / 1024 * 1024u);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kKv4Stages; i++)
+        if (i < tiles) request(i);
+    // Column n of the products is head n; with at most eight heads the columns from 8 on hold them once more, and take
+    // what the rounding of p to fp16 leaves.
+    const bool twice = live <= 8, second = twice && n >= 8;
+    const int column = second ? n - 8 : n;
     half8v_t qf[kW];
 #pragma unroll
     for (int w = 0; w < kW; w++) {
-        qf[w] = (half8v_t)((_Float16)0.f);
-        if (n < live)
-            qf[w] = *reinterpret_cast<const half8v_t *>(a.q + seq * a.q_token + (int64_t)(head0 + n) * HD + 8 * (c * kW + w));
+        half8v_t q = (half8v_t)((_Float16)0.f);
+        if (column < live)
+            q = *reinterpret_cast<const half8v_t *>(a.q + r.seq * a.q_token + (int64_t)(head0 + column) * HD + 8 * (c * kW + w));
+        qf[w] = __builtin_shufflevector(q, q, 0, 4, 1, 5, 2, 6, 3, 7);     // as word_values orders a word
     }
+    // the queries are there: a wait inside the loop would wait for rows on their way as well
+#pragma unroll
+    for (int w = 0; w < kW; w++) asm volatile("" : "+v"(qf[w]));
+
+    // hd 64, 32: the lane's four or two dimensions are nibbles of two bytes of the word (hd 32: of one parity)
+    const uint32_t v_bytes = 0x06020400u + 0x01010101u * (uint32_t)(HD == 64 ? n & 1 : n >> 1 & 1);
+    const int v_shift = HD == 32 ? 4 * (n & 1) : 0;
     float4v_t acc[kE];
 #pragma unroll
     for (int e = 0; e < kE; e++) acc[e] = (float4v_t)(0.f);
     float m = -INFINITY, l = 0.f;
-
-    for (int64_t j0 = lo + wave * kKv4Tile; j0 < hi; j0 += kKv4Waves * kKv4Tile) {
-        // rows past the piece: its last row, masked below (its values count with p = 0)
-        const uint8_t *kb = a.k_cache + (head_base + j0) * kRow, *vb = a.v_cache + (head_base + j0) * kRow;
-        const int left = (int)min((int64_t)kKv4Tile, hi - j0);
+    for (int i = 0; i < tiles; i++) {
+        if (i + 1 < tiles) wait_for_lds_loads_but<(kKv4Stages - 1) * 2 * kRequests>();
+        else wait_for_lds_loads();
+        static_assert(kKv4Stages == 2, "the wait above");
+        const uint8_t *ks = ring + (i % kKv4Stages) * 2 * kStage, *vs = ks + kStage;
         uint32_t kw[2][kW], kp[2][(kW + 3) / 4], vw[8][kVW], vp[8];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const uint8_t *r = kb + min(16 * t + n, left - 1) * kRow;
+            const uint8_t *r = ks + (16 * t + n) * kRow;
 #pragma unroll
             for (int w = 0; w < kW; w++) kw[t][w] = *reinterpret_cast<const uint32_t *>(r + 4 * (c * kW + w));
 #pragma unroll
             for (int g = 0; g < (kW + 3) / 4; g++) kp[t][g] = *reinterpret_cast<const uint32_t *>(r + HD / 2 + 4 * (c * kW / 4 + g));
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint8_t *r = vb + min(16 * (i / 4) + 4 * c + i % 4, left - 1) * kRow;
+        for (int j = 0; j < 8; j++) {
+            const uint8_t *r = vs + (16 * (j / 4) + 4 * c + j % 4) * kRow;
 #pragma unroll
-            for (int w = 0; w < kVW; w++) vw[i][w] = *reinterpret_cast<const uint32_t *>(r + 4 * (HD >= 128 ? n * kVW + w : n * kE / 8));
-            vp[i] = *reinterpret_cast<const uint32_t *>(r + HD / 2 + 4 * (n * kE / 32));
+            for (int w = 0; w < kVW; w++) vw[j][w] = *reinterpret_cast<const uint32_t *>(r + 4 * (HD >= 128 ? n * kVW + w : n * kE / 8));
+            vp[j] = *reinterpret_cast<const uint32_t *>(r + HD / 2 + 4 * (n * kE / 32));
         }
+        wait_for_lds_reads();
+        if (i + kKv4Stages < tiles) request(i + kKv4Stages);
+
         float4v_t s[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             s[t] = (float4v_t)(0.f);
 #pragma unroll
-            for (int w = 0; w < kW; w++) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(word_values(kw[t][w], kp[t][w / 4]), qf[w], s[t], 0, 0, 0);
+            for (int w = 0; w < kW; w++) {
+                half2_t v[4];
+                word_values(kw[t][w], kp[t][w / 4], v);
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(v), qf[w], s[t], 0, 0, 0);
+            }
         }
+        const int left = hi - (first + i * kWaves * kKv4Tile);
+        if (left < kKv4Tile) {
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (16 * (i / 4) + 4 * c + i % 4 >= left) s[i / 4][i % 4] = -INFINITY;
+            for (int j = 0; j < 8; j++)
+                if (16 * (j / 4) + 4 * c + j % 4 >= left) s[j / 4][j % 4] = -INFINITY;
+        }
         float mx = s[0][0];
 #pragma unroll
-        for (int i = 1; i < 8; i++) mx = fmaxf(mx, s[i / 4][i % 4]);
+        for (int j = 1; j < 8; j++) mx = fmaxf(mx, s[j / 4][j % 4]);
         mx = rows_max(mx) * a.c;
         if (__ballot(mx > m + kKv4Lazy)) {
             const float up = fmaxf(m, mx);
@@ -341,99 +472,129 @@ __global__ __launch_bounds__(64 * kKv4Waves) void kv4_attn_kernel(const Kv4AttnA
             m = up;
         }
         const float mc = m == -INFINITY ? 0.f : m;
-        half8v_t p;
+        half2_t p2[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], a.c, -mc));
+        for (int j = 0; j < 4; j++) {
+            const int r = 2 * j;
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[r / 4][r % 4], a.c, -mc)), y = __builtin_amdgcn_exp2f(fmaf(s[r / 4][r % 4 + 1], a.c, -mc));
             l += x;
-            p[i] = (_Float16)x;
+            l += y;
+            const float2v_t xy = {x, y};
+            p2[j] = __builtin_convertvector(xy, half2_t);
+            const float2v_t left_over = {x - (float)p2[j].x, y - (float)p2[j].y};
+            p2[j] = second ? __builtin_convertvector(left_over, half2_t) : p2[j];
         }
-        // V: the positions in pairs, the nibbles of a dimension of both in one register
+        const half8v_t p = as_half8(p2);
+        // V: the same byte of two positions' words side by side, then the nibbles of a dimension of both in one register
         half2_t val[kE][4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const half2_t sc = as_half2(low_halves(vp[2 * i], vp[2 * i + 1])), mn = as_half2(high_halves(vp[2 * i], vp[2 * i + 1]));
+        for (int j = 0; j < 4; j++) {
+            const half2_t sc = as_half2(low_halves(vp[2 * j], vp[2 * j + 1])), mn = as_half2(high_halves(vp[2 * j], vp[2 * j + 1]));
 #pragma unroll
             for (int w = 0; w < kVW; w++) {
-                uint32_t x = vw[2 * i][w], y = vw[2 * i + 1][w];
-                constexpr int kN = kE >= 8 ? 4 : kE / 2;   // pairs of dimensions of the word that are the lane's
-                if (kE < 8) {
-                    x >>= 2 * kE * (n % (8 / kE));
-                    y >>= 2 * kE * (n % (8 / kE));
-                }
-                half2_t even[4], oddv[4];
-                nibble_pairs<kN>(low_halves(x, y), even);
-                nibble_pairs<kN>(high_halves(x, y), oddv);
+                const uint32_t x = vw[2 * j][w], y = vw[2 * j + 1][w];
+                if (kE >= 8) {
 #pragma unroll
-                for (int t = 0; t < kN; t++) {
-                    val[8 * w + 2 * t][i] = __builtin_elementwise_fma(even[t], sc, mn);
-                    val[8 * w + 2 * t + 1][i] = __builtin_elementwise_fma(oddv[t], sc, mn);
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t xy = __builtin_amdgcn_perm(y, x, h ? 0x07030602u : 0x05010400u);
+                        const uint32_t even = xy & 0x0F0F0F0Fu, odd = (xy >> 4) & 0x0F0F0F0Fu;
+                        val[8 * w + h][j] = __builtin_elementwise_fma(byte_codes<false>(even), sc, mn);
+                        val[8 * w + 4 + h][j] = __builtin_elementwise_fma(byte_codes<true>(even), sc, mn);
+                        val[8 * w + 2 + h][j] = __builtin_elementwise_fma(byte_codes<false>(odd), sc, mn);
+                        val[8 * w + 6 + h][j] = __builtin_elementwise_fma(byte_codes<true>(odd), sc, mn);
+                    }
+                } else {
+                    const uint32_t xy = __builtin_amdgcn_perm(y, x, v_bytes) >> v_shift;
+                    const uint32_t even = xy & 0x0F0F0F0Fu;
+                    val[0][j] = __builtin_elementwise_fma(byte_codes<false>(even), sc, mn);
+                    val[1][j] = __builtin_elementwise_fma(byte_codes<true>(even), sc, mn);
+                    if (kE > 2) {
+                        const uint32_t odd = (xy >> 4) & 0x0F0F0F0Fu;
+                        val[2 % kE][j] = __builtin_elementwise_fma(byte_codes<false>(odd), sc, mn);
+                        val[3 % kE][j] = __builtin_elementwise_fma(byte_codes<true>(odd), sc, mn);
+                    }
                 }
             }
         }
 #pragma unroll
-        for (int e = 0; e < kE; e++) {
-            const half8v_t v8 = {val[e][0].x, val[e][0].y, val[e][1].x, val[e][1].y, val[e][2].x, val[e][2].y, val[e][3].x, val[e][3].y};
-            acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, p, acc[e], 0, 0, 0);
-        }
+        for (int e = 0; e < kE; e++) acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(val[e]), p, acc[e], 0, 0, 0);
     }
 
-    // the waves join through LDS: lane (head n, quarter c) holds the dimensions 4 kE c .. 4 kE (c + 1)
-    float *w_acc = lds4 + (size_t)wave * live * HD, *w_ml = lds4 + (size_t)kKv4Waves * live * HD;
+    // The waves join through LDS: lane (column n, quarter c) holds the dimensions 4 kE c .. 4 kE (c + 1) of its column, a run of
+    // floats; a column has four floats of padding, so that the columns' runs begin on different banks.
+    __syncthreads();                                       // nobody reads a stage any more
+    constexpr int kColumn = HD + 4;
+    float *sums = reinterpret_cast<float *>(lds4);
+    const int columns = twice ? 2 * live : live, wave_sums = columns * kColumn;
+    float *w_ml = sums + (size_t)kWaves * wave_sums;       // [wave][16][2]: bound and sum, later the wave's factor and the sum by it
     l = rows_sum(l);
-    if (n < live) {
+    if (column < live) {
+        float4 *to = reinterpret_cast<float4 *>(sums + (size_t)wave * wave_sums + (second ? live + column : n) * kColumn + 4 * kE * c);
 #pragma unroll
-        for (int r = 0; r < 4; r++)
-#pragma unroll
-            for (int e = 0; e < kE; e++) w_acc[n * HD + kE * (4 * c + r) + e] = acc[e][r];
-        if (c == 0) {
+        for (int i = 0; i < kE; i++)                       // float i * 4 + k of the run: dimension e = (4 i + k) % kE of row r = (4 i + k) / kE
+            to[i] = make_float4(acc[(4 * i) % kE][(4 * i) / kE], acc[(4 * i + 1) % kE][(4 * i + 1) / kE], acc[(4 * i + 2) % kE][(4 * i + 2) / kE],
+                                acc[(4 * i + 3) % kE][(4 * i + 3) / kE]);
+        if (c == 0 && !second) {
             w_ml[2 * (wave * 16 + n)] = m;
             w_ml[2 * (wave * 16 + n) + 1] = l;
         }
     }
     __syncthreads();
-    for (int i = tid; i < live * HD; i += 64 * kKv4Waves) {
-        const int h = i / HD, d = i % HD;
-        float M = -INFINITY;
+    float M = -INFINITY, f = 0.f, lw = 0.f;                // thread (head, wave) of the first 16 kWaves
+    if (tid < 16 * kWaves && tid / kWaves < live) {
+        const int h = tid / kWaves, w = tid % kWaves;
+        const float mw = w_ml[2 * (w * 16 + h)];
+        lw = w_ml[2 * (w * 16 + h) + 1];
 #pragma unroll
-        for (int w = 0; w < kKv4Waves; w++) M = fmaxf(M, w_ml[2 * (w * 16 + h)]);
+        for (int i = 0; i < kWaves; i++) M = fmaxf(M, w_ml[2 * (i * 16 + h)]);
+        // a wave without a position has sum 0 (and accumulators 0); a bound of -inf with a sum is not-a-numbers
+        f = lw == 0.f ? 0.f : mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - M);
+    }
+    __syncthreads();
+    if (tid < 16 * kWaves && tid / kWaves < live) {
+        const int h = tid / kWaves, w = tid % kWaves;
+        w_ml[2 * (w * 16 + h)] = f;
+        w_ml[2 * (w * 16 + h) + 1] = lw * f;
+        if (r.pieces > 1 && w == 0) a.part[a.part_ml + 2 * ((int64_t)(head0 + h) * a.slots + slot)] = M;
+    }
+    __syncthreads();
+    for (int i = tid; i < live * HD; i += 64 * kWaves) {
+        const int h = i / HD, d = i % HD;
         float num = 0.f, den = 0.f;
 #pragma unroll
-        for (int w = 0; w < kKv4Waves; w++) {
-            const float mw = w_ml[2 * (w * 16 + h)], lw = w_ml[2 * (w * 16 + h) + 1];
-            if (lw == 0.f) continue;                       // the wave had no position
-            const float f = mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - M);
-            num = fmaf(lds4[(size_t)w * live * HD + i], f, num);
-            den = fmaf(lw, f, den);
+        for (int w = 0; w < kWaves; w++) {
+            float part = sums[(size_t)w * wave_sums + h * kColumn + d];
+            if (twice) part += sums[(size_t)w * wave_sums + (live + h) * kColumn + d];
+            num = fmaf(part, w_ml[2 * (w * 16 + h)], num);
+            den += w_ml[2 * (w * 16 + h) + 1];
         }
-        const int64_t at = (int64_t)seq * a.heads + head0 + h;
-        if (a.splits == 1) {
-            a.out[at * HD + d] = float_to_half_bits(num / den);
+        if (r.pieces == 1) {
+            a.out[((int64_t)r.seq * a.heads + head0 + h) * HD + d] = float_to_half_bits(num / den);
         } else {
-            a.part[(at * a.splits + split) * HD + d] = num;
-            if (d == 0) *reinterpret_cast<float2 *>(a.part + a.part_ml + 2 * (at * a.splits + split)) = make_float2(M, den);
+            const int64_t at = (int64_t)(head0 + h) * a.slots + slot;
+            a.part[at * HD + d] = num;
+            if (d == 0) a.part[a.part_ml + 2 * at + 1] = den;
         }
     }
 }
 
-// Joins the pieces of a head, a workgroup per (sequence, head).
-__global__ __launch_bounds__(kJoinThreads) void kv4_merge_kernel(const float *__restrict__ part, int64_t part_ml, const int64_t *__restrict__ pos,
-                                                                 uint16_t *__restrict__ out, int heads, int hd, int splits, int64_t max_len)
+// Joins the pieces of a head, a workgroup per (head, sequence).
+template <int HD>
+__global__ __launch_bounds__(kJoinThreads) void kv4_merge_kernel(const Kv4AttnArgs a)
 {
     const int head = blockIdx.x, seq = blockIdx.y;
-    if (pos[seq] < 0 || pos[seq] >= max_len) return;
-    const int64_t at = (int64_t)seq * heads + head;
+    Kv4Piece r;
+    if (!kv4_find(a, seq, true, r) || r.pieces == 1) return;
+    const int64_t at = (int64_t)head * a.slots + r.slot0;
     float M, den;
-    const float num = join_pieces(part + at * splits * hd, part + part_ml + 2 * at * splits, splits, hd, M, den);
-    if (threadIdx.x < hd) out[at * hd + threadIdx.x] = float_to_half_bits(num / den);
+    const float num = join_pieces(a.part + at * HD, a.part + a.part_ml + 2 * at, r.pieces, HD, M, den);
+    if (threadIdx.x < HD) a.out[((int64_t)seq * a.heads + head) * HD + threadIdx.x] = float_to_half_bits(num / den);
 }
-
-template <int HD>
-static size_t kv4_lds(int live) { return ((size_t)kKv4Waves * live * HD + kKv4Waves * 32) * 4; }
 
 int prepare_kv4()
 {
     int rc;
+    if ((rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&kv4_attn_kernel<64>), hipFuncAttributeMaxDynamicSharedMemorySize, kv4_lds<64>(16)))) return rc;
     if ((rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&kv4_attn_kernel<128>), hipFuncAttributeMaxDynamicSharedMemorySize, kv4_lds<128>(16)))) return rc;
     return (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&kv4_attn_kernel<256>), hipFuncAttributeMaxDynamicSharedMemorySize, kv4_lds<256>(16));
 }
@@ -446,11 +607,23 @@ static int kv4_sizes(int64_t seqs, int64_t kv_heads, int64_t hd, int64_t max_len
     return 0;
 }
 
-static int64_t kv4_splits(int64_t groups, int64_t max_len, int cus)
+struct Kv4Plan {
+    int slots, want, least;
+};
+
+// groups: workgroups a piece has (key heads, times blocks of 16 query heads).  Cut into pieces, so that about one workgroup
+// a compute unit runs, and joined by a second launch (4 us): caches of 2048 positions and more (a workgroup walks 1024 in
+// 4 steps of its waves, 2 us) with fewer sequences and heads than compute units, and of 8192 and more up to four times as
+// many, for what one long sequence among short ones would cost.  Pieces are no shorter than 512 positions.  Measured, uncut /
+// cut, heads x 128: one sequence of 1024, 32 heads: 10.4 / 11.3 us; of 8192, 32 heads: 34 / 18; 32 of 2000, 8 heads x 64: 14.4 / 17.3.
+static Kv4Plan kv4_plan(int64_t seqs, int64_t groups, int64_t max_len, int cus)
 {
-    int64_t n = (2 * (int64_t)cus + groups - 1) / groups;
-    if (n > max_len / (2 * kKv4Waves * kKv4Tile)) n = max_len / (2 * kKv4Waves * kKv4Tile);
-    return n < 1 ? 1 : n > 128 ? 128 : n;
+    Kv4Plan p = {(int)seqs, 1, 512 / kKv4Tile};
+    if (max_len < 2048 || seqs > 1024 || seqs * groups >= (max_len >= 8192 ? 4 : 1) * (int64_t)cus) return p;
+    p.want = (int)((cus + groups - 1) / groups);
+    if (p.want < 2) p.want = 2;
+    p.slots = (int)seqs + p.want - 1;          // pieces of one length: fewer than want whole ones and one more a sequence
+    return p;
 }
 
 }  // namespace rptc
@@ -568,19 +741,21 @@ extern "C" int64_t rptc_kv4_attn_decode_workspace_bytes(int64_t seqs, int64_t he
     int rc = kv4_sizes(seqs, kv_heads, hd, max_len);
     if (rc) return rc;
     if (heads < 1 || heads % kv_heads != 0) return RPTC_ESHAPE;
-    if (heads > 1024) return RPTC_ELIMIT;
+    if (heads > 1024 || seqs * kv_heads * ((heads / kv_heads + 15) / 16) >= (int64_t)1 << 22) return RPTC_ELIMIT;
     DeviceInfo *dev;
     if ((rc = device_info(&dev))) return rc < 0 ? rc : RPTC_EDEVICE;
-    const int64_t splits = kv4_splits(seqs * kv_heads * ((heads / kv_heads + 15) / 16), max_len, dev->cus);
-    return splits > 1 ? seqs * heads * splits * (hd + 2) * 4 : 0;
+    const Kv4Plan plan = kv4_plan(seqs, kv_heads * ((heads / kv_heads + 15) / 16), max_len, dev->cus);
+    return plan.want > 1 ? heads * plan.slots * (hd + 2) * 4 : 0;
 }
 
 template <int HD>
-static void launch_kv4_attn(const Kv4AttnArgs &a, int seqs, hipStream_t s)
+static void launch_kv4_attn(const Kv4AttnArgs &a, hipStream_t s)
 {
     const int live = a.group < 16 ? a.group : 16;
-    hipLaunchKernelGGL(kv4_attn_kernel<HD>, dim3((unsigned)a.splits, (unsigned)(a.kv_heads * a.head_blocks), (unsigned)seqs),
-                       dim3(64 * kKv4Waves), kv4_lds<HD>(live), s, a);
+    hipLaunchKernelGGL(kv4_attn_kernel<HD>, dim3((unsigned)(a.slots * a.kv_heads * a.head_blocks)), dim3(64 * kKv4Waves<HD>),
+                       kv4_lds<HD>(live), s, a);
+    if (a.want > 1)
+        hipLaunchKernelGGL(kv4_merge_kernel<HD>, dim3((unsigned)a.heads, (unsigned)a.seqs), dim3(kJoinThreads), 0, s, a);
 }
 
 extern "C" int rptc_kv4_attn_decode(const uint16_t *q, const uint8_t *k_cache, const uint8_t *v_cache, const int64_t *pos, uint16_t *out,
@@ -591,7 +766,7 @@ extern "C" int rptc_kv4_attn_decode(const uint16_t *q, const uint8_t *k_cache, c
     int rc = kv4_sizes(seqs, kv_heads, hd, max_len);
     if (rc) return rc;
     if (heads < 1 || heads % kv_heads != 0 || q_token < 0 || !(scale > 0.f) || !(scale < 1e30f)) return RPTC_ESHAPE;
-    if (heads > 1024) return RPTC_ELIMIT;
+    if (heads > 1024 || seqs * kv_heads * ((heads / kv_heads + 15) / 16) >= (int64_t)1 << 22) return RPTC_ELIMIT;
     if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || q_token % 8) return RPTC_EALIGN;
     if (out == q) return RPTC_EALIAS;
     DeviceInfo *dev;
@@ -608,27 +783,28 @@ extern "C" int rptc_kv4_attn_decode(const uint16_t *q, const uint8_t *k_cache, c
     a.kv_heads = (int)kv_heads;
     a.group = (int)(heads / kv_heads);
     a.head_blocks = (a.group + 15) / 16;
-    a.splits = (int)kv4_splits(seqs * kv_heads * a.head_blocks, max_len, dev->cus);
+    const Kv4Plan plan = kv4_plan(seqs, kv_heads * a.head_blocks, max_len, dev->cus);
+    a.seqs = (int)seqs;
+    a.slots = plan.slots;
+    a.want = plan.want;
+    a.least = plan.least;
     a.c = scale * 1.44269504088896f;
     a.part = nullptr;
-    a.part_ml = seqs * heads * a.splits * hd;
-    if (a.splits > 1) {
+    a.part_ml = heads * a.slots * hd;
+    if (a.want > 1) {
         if (!workspace) return RPTC_ENULL;
         if (!aligned16(workspace)) return RPTC_EALIGN;
-        if (workspace_bytes < seqs * heads * a.splits * (hd + 2) * 4) return RPTC_ESHAPE;
+        if (workspace_bytes < heads * a.slots * (hd + 2) * 4) return RPTC_ESHAPE;
         a.part = static_cast<float *>(workspace);
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
     Timer timer;
     if ((rc = timer.begin(dev, s, ms))) return rc;
     switch (hd) {
-    case 32: launch_kv4_attn<32>(a, (int)seqs, s); break;
-    case 64: launch_kv4_attn<64>(a, (int)seqs, s); break;
-    case 128: launch_kv4_attn<128>(a, (int)seqs, s); break;
-    default: launch_kv4_attn<256>(a, (int)seqs, s); break;
+    case 32: launch_kv4_attn<32>(a, s); break;
+    case 64: launch_kv4_attn<64>(a, s); break;
+    case 128: launch_kv4_attn<128>(a, s); break;
+    default: launch_kv4_attn<256>(a, s); break;
     }
-    if (a.splits > 1)
-        hipLaunchKernelGGL(kv4_merge_kernel, dim3((unsigned)heads, (unsigned)seqs), dim3(kJoinThreads), 0, s, a.part, a.part_ml, pos, out, (int)heads,
-                           (int)hd, a.splits, max_len);
     return timer.end();
 }
