@@ -409,8 +409,8 @@ int64_t rptc_lite_viterbi_scratch_bytes(int L, int R, int64_t rows, int64_t step
  *   k_start and k_len NULL (both or neither): the keys lie as the queries do (total_k == total_q), or, without q_start, are
  *   all key rows.  max_k an upper bound of k_len (total_k will do:
  *   it only decides how far the keys of a call with few rows are split)
- *   workspace  rptc_attn_prompt_workspace_bytes(...) bytes of device memory, 16-byte aligned (0: may be NULL); no
- *              initialisation, calls that may overlap need one each.  At most 2^24 query rows, 1024 heads, 2^20 sequences,
+ *   workspace  rptc_attn_prompt_workspace_bytes(...) bytes (a negative status for sizes the call does not take) of device
+ *              memory, 16-byte aligned (0: may be NULL); no initialisation, calls that may overlap need one each.  At most 2^24 query rows, 1024 heads, 2^20 sequences,
  *              (total_q / 32 + seqs) * heads below 2^23.
  */
 typedef struct rptc_prompt_strides {
@@ -426,7 +426,7 @@ int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint16_t *v, ui
 
 /*
  * A key/value cache held in 4 bits.  No counterpart in the reference (it generates with transformers, quantize_hf.py:229-236).
- * k_cache, v_cache: uint8 [seqs][kv_heads][max_len][rptc_kv4_row_bytes(hd)], hd in {32, 64, 128, 256}.  A row holds hd fp16
+ * k_cache, v_cache: uint8 [seqs][kv_heads][max_len][rptc_kv4_row_bytes(hd)], hd in {32, 64, 128, 256} (a negative status for others).  A row holds hd fp16
  * values in groups of 32: m = min x, s = fp16((max x - min x) / 15), code = clamp(rint((x - m) / s), 0, 15) (0 where s = 0; the
  * quotients in fp32), and stands for fp16(code * s + m).  A group with a value that is no finite number reads as
  * not-a-number.  hd / 2 bytes of codes (word w: values 8w .. 8w+7, nibble t the value 8w + 2t, nibble t + 4 the value
@@ -470,7 +470,7 @@ int rptc_kv4_attn_decode(const uint16_t *q, const uint8_t *k_cache, const uint8_
  *   entropy       float [rows], nats
  *   top_ids       int64 [rows][top], top_logprobs float [rows][top]: the `top` largest logits of a row in falling order, equal
  *                 ones by the lowest id (a not-a-number counts as -inf); top <= 64 and <= vocab
- * Each output may be NULL (top == 0 without the last two).  fp32 inside.  A row that holds +inf or a not-a-number, or nothing
+ * Each output may be NULL (top == 0 without the last two), none may overlap the logits.  fp32 inside.  A row that holds +inf or a not-a-number, or nothing
  * but -inf, has not-a-number for probabilities and entropy.
  */
 int rptc_token_logprobs(const void *logits, int dtype, const int64_t *tokens, float *logprob, float *entropy, int64_t *top_ids,

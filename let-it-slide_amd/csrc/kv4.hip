@@ -643,7 +643,8 @@ extern "C" int rptc_kv4_append(const uint16_t *k, const uint16_t *v, uint8_t *k_
     if (total > (1 << 24)) return RPTC_ELIMIT;
     if (!aligned16(k) || !aligned16(v) || !aligned16(k_cache) || !aligned16(v_cache)) return RPTC_EALIGN;
     if (k_token % 8 || k_head % 8 || v_token % 8 || v_head % 8) return RPTC_EALIGN;
-    if (k_cache == v_cache) return RPTC_EALIAS;
+    auto rows = [&](const void *c) { return c == k || c == v; };
+    if (k_cache == v_cache || rows(k_cache) || rows(v_cache)) return RPTC_EALIAS;
     DeviceInfo *dev;
     if ((rc = device_info(&dev))) return rc;
     Kv4AppendArgs a;
@@ -686,6 +687,8 @@ extern "C" int rptc_kv4_read(const uint8_t *k_cache, const uint8_t *v_cache, uin
     if (rows < 1 || rows > max_len || k_token < 0 || k_head < 0 || v_token < 0 || v_head < 0) return RPTC_ESHAPE;
     if (!aligned16(k) || !aligned16(v) || !aligned16(k_cache) || !aligned16(v_cache)) return RPTC_EALIGN;
     if (k_token % 8 || k_head % 8 || v_token % 8 || v_head % 8) return RPTC_EALIGN;
+    auto cache = [&](const void *o) { return o == k_cache || o == v_cache; };
+    if (k == v || cache(k) || cache(v)) return RPTC_EALIAS;
     DeviceInfo *dev;
     if ((rc = device_info(&dev))) return rc;
     Kv4ReadArgs a;
@@ -724,7 +727,8 @@ extern "C" int rptc_kv4_rope_append(const uint16_t *qkv, const uint16_t *cos_t, 
     if (heads < 1 || heads % kv_heads != 0) return RPTC_ESHAPE;
     if (heads > 1024) return RPTC_ELIMIT;
     if (!aligned16(qkv) || !aligned16(cos_t) || !aligned16(sin_t) || !aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache)) return RPTC_EALIGN;
-    if (q_out == qkv || k_cache == v_cache) return RPTC_EALIAS;
+    auto cache = [&](const void *p) { return p == k_cache || p == v_cache; };
+    if (q_out == qkv || k_cache == v_cache || cache(q_out) || cache(qkv)) return RPTC_EALIAS;
     DeviceInfo *dev;
     if ((rc = device_info(&dev))) return rc;
     const int items = (int)((heads + 2 * kv_heads) * (hd / 8));
@@ -768,7 +772,8 @@ extern "C" int rptc_kv4_attn_decode(const uint16_t *q, const uint8_t *k_cache, c
     if (heads < 1 || heads % kv_heads != 0 || q_token < 0 || !(scale > 0.f) || !(scale < 1e30f)) return RPTC_ESHAPE;
     if (heads > 1024 || seqs * kv_heads * ((heads / kv_heads + 15) / 16) >= (int64_t)1 << 22) return RPTC_ELIMIT;
     if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || q_token % 8) return RPTC_EALIGN;
-    if (out == q) return RPTC_EALIAS;
+    auto read = [&](const void *o) { return o == q || o == k_cache || o == v_cache; };
+    if (read(out)) return RPTC_EALIAS;
     DeviceInfo *dev;
     if ((rc = device_info(&dev))) return rc;
     Kv4AttnArgs a;

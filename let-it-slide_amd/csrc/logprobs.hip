@@ -337,8 +337,15 @@ extern "C" int rptc_token_logprobs(const void *logits, int dtype, const int64_t 
     if (dtype != RPTC_F16 && dtype != RPTC_BF16 && dtype != RPTC_F32) return RPTC_EMODE;
     if (rows < 1 || vocab < 1 || row_stride < 0 || top < 0 || top > vocab) return RPTC_ESHAPE;
     if ((top > 0) != (top_ids || top_logprobs)) return RPTC_ESHAPE;
-    if (rows >= (int64_t)1 << 22 || vocab >= (int64_t)1 << 30 || top > kScoreGroups) return RPTC_ELIMIT;
-    if (reinterpret_cast<uintptr_t>(logits) % (dtype == RPTC_F32 ? 4 : 2) != 0) return RPTC_EALIGN;
+    if (rows >= (int64_t)1 << 22 || vocab >= (int64_t)1 << 30 || row_stride >= (int64_t)1 << 34 || top > kScoreGroups) return RPTC_ELIMIT;
+    const int64_t width = dtype == RPTC_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(logits) % width != 0) return RPTC_EALIGN;
+    const int64_t bytes = ((rows - 1) * row_stride + vocab) * width;
+    auto inside = [&](const void *out, int64_t out_bytes) {
+        const char *lo = static_cast<const char *>(logits), *o = static_cast<const char *>(out);
+        return out && o < lo + bytes && lo < o + out_bytes;
+    };
+    if (inside(logprob, rows * 4) || inside(entropy, rows * 4) || inside(top_ids, rows * top * 8) || inside(top_logprobs, rows * top * 4)) return RPTC_EALIAS;
     DeviceInfo *dev;
     int rc = device_info(&dev);
     if (rc) return rc;

@@ -84,6 +84,49 @@ def llama_logits_fn(model, chunk=32):
     return fn
 
 
+def score_tokens(model, tokens, lens=None, top=0):
+    """Log probabilities of given texts under a ``llama_decode.QuantizedLlama``, in one packed pass: tokens [T] (sequences of
+    ``lens`` tokens one behind the other, None: one).  Returns a dict of tensors over the T tokens: ``logprob`` of the token
+    behind it (not-a-number for a sequence's last token, which has none), ``entropy`` of that prediction in nats and, with
+    ``top``, ``top_ids`` and ``top_logprobs`` [T, top] of its most likely tokens."""
+    import rptc_kernels as rk
+    dev = model.embed.device
+    tokens = torch.as_tensor(tokens, dtype=torch.int64).reshape(-1).to(dev)
+    lens = [tokens.numel()] if lens is None else [int(n) for n in lens]
+    with torch.no_grad():
+        logits = model.forward_prompt(tokens, lens, all_logits=True, half_logits=True)
+    T = tokens.numel()
+    following = torch.cat([tokens[1:], tokens.new_full((1,), -1)])
+    following[(torch.tensor(lens).cumsum(0) - 1).to(dev)] = -1
+    out = {"logprob": torch.empty(T, dtype=torch.float32, device=dev), "entropy": torch.empty(T, dtype=torch.float32, device=dev)}
+    if top:
+        out["top_ids"] = torch.empty((T, top), dtype=torch.int64, device=dev)
+        out["top_logprobs"] = torch.empty((T, top), dtype=torch.float32, device=dev)
+    rk.token_logprobs(logits, following, timed=False, **out)
+    return out
+
+
+def packed_perplexity(model, tokens, seqlen, windows_per_pass=4, progress=None):
+    """``perplexity`` of a ``llama_decode.QuantizedLlama`` with several windows in one pass through ``forward_prompt``; the
+    same windows, the same measure, the same three results."""
+    tokens = torch.as_tensor(tokens, dtype=torch.int64).reshape(-1)
+    nsamples = tokens.numel() // seqlen
+    if nsamples < 1:
+        raise ValueError(f"{tokens.numel()} tokens do not fill one window of {seqlen}")
+    if seqlen < 2 or windows_per_pass < 1:
+        raise ValueError("a window needs two tokens, a pass one window")
+    acc = 0.0
+    for w0 in range(0, nsamples, windows_per_pass):
+        n = min(windows_per_pass, nsamples - w0)
+        scored = score_tokens(model, tokens[w0 * seqlen:(w0 + n) * seqlen], [seqlen] * n)
+        losses = -scored["logprob"].view(n, seqlen)[:, :-1].double().mean(dim=1)
+        acc += float(losses.sum())
+        if progress is not None:
+            progress(w0 + n, nsamples, acc / (w0 + n))
+    avg = acc / nsamples
+    return math.exp(avg), avg, nsamples
+
+
 def main(argv=None):
     from .llama_decode import LlamaShape, QuantizedLlama
     ap = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
@@ -96,13 +139,18 @@ def main(argv=None):
     ap.add_argument("--d-ff", type=int, default=11008)
     ap.add_argument("--vocab", type=int, default=32000)
     ap.add_argument("--seed", type=int, default=42)
+    ap.add_argument("--packed", type=int, default=0, metavar="N",
+                    help="N windows a pass, through the prompt attention and the token log probabilities (0: chunks of 32 tokens)")
     a = ap.parse_args(argv)
     shape = LlamaShape(layers=a.layers, d_model=a.d_model, heads=a.heads, d_ff=a.d_ff, vocab=a.vocab, max_len=a.seqlen)
     model = QuantizedLlama(shape, seed=a.seed)
     tokens = load_tokens(a.tokens) if a.tokens else synthetic_tokens(a.windows * a.seqlen, a.vocab, a.seed)
     if int(tokens.max()) >= a.vocab or int(tokens.min()) < 0:
         raise ValueError("token ids outside the model's vocabulary")
-    ppl, loss, n = perplexity(llama_logits_fn(model), tokens, a.seqlen)
+    if a.packed:
+        ppl, loss, n = packed_perplexity(model, tokens, a.seqlen, a.packed)
+    else:
+        ppl, loss, n = perplexity(llama_logits_fn(model), tokens, a.seqlen)
     print(json.dumps({"perplexity": ppl, "avg_loss": loss, "windows": n, "seqlen": a.seqlen,
                       "tokens": a.tokens or "synthetic", "model": "random-init Llama shape on 2-bit streams"}))
 

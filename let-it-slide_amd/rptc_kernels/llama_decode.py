@@ -8,9 +8,12 @@ grouped the way the reference groups them for its Hessians (quantize_hf.py:14-22
 built from its shape only (random-init norms, embeddings and lm_head; for the projections seeded random
 streams, or random-init dense weights quantized with the reference's procedure): nothing is downloaded.
 
-Two ways through a token: ``forward_tokens`` (torch ops between the projections; used for the
-prompt, any number of tokens) and ``decode_step`` (this library's fused glue kernels, one token).
-Greedy decoding captures one ``decode_step`` in a HIP graph and replays it per token.
+Three ways through tokens: ``forward_tokens`` (torch ops between the projections; used for the
+prompt, any number of tokens), ``forward_prompt`` (whole prompts, several of them packed into one pass, through this
+library's prompt attention) and ``decode_step`` (this library's fused glue kernels, one token).
+Greedy decoding captures one ``decode_step`` in a HIP graph and replays it per token.  The key/value cache holds fp16
+values or, with ``cache_bits=4``, the rows of ``kv4_cache`` (5 bits a value with their scales: 160 bytes a position, head and
+layer at head dimension 128 instead of 512).
 """
 import ctypes
 import time
@@ -31,13 +34,17 @@ class LlamaShape:
 class QuantizedLlama(torch.nn.Module):
     EPS = 1e-5
 
-    def __init__(self, shape, S=8, seed=42, device="cuda", quantize_init=False, init_std=0.02):
+    def __init__(self, shape, S=8, seed=42, device="cuda", quantize_init=False, init_std=0.02, cache_bits=16):
         """quantize_init=False: seeded random streams (decode cost does not depend on the data).
         quantize_init=True: every projection is a random-init dense weight (normal, ``init_std``: the
         initialisation of the reference's model class) put through the reference's procedure - row/column
         factorisation (quantize_hf.py:77-117), then the trellis search on the normalised matrix - and run
-        with its four vectors applied inside the mat-vec kernels."""
+        with its four vectors applied inside the mat-vec kernels.
+        cache_bits=4: the cache in 4 bits (a head dimension of 32, 64, 128 or 256)."""
         super().__init__()
+        if cache_bits not in (4, 16):
+            raise ValueError("cache_bits must be 4 or 16")
+        self.cache_bits = cache_bits
         self.shape = shape
         g = torch.Generator(device=device)
         g.manual_seed(seed)
@@ -68,8 +75,13 @@ class QuantizedLlama(torch.nn.Module):
         inv = 1.0 / (shape.rope_theta ** (torch.arange(0, hd, 2, device=device).float() / hd))
         ang = torch.arange(shape.max_len, device=device).float()[:, None] * inv[None, :]
         self.cos, self.sin = ang.cos().half().contiguous(), ang.sin().half().contiguous()    # [max_len, hd/2]
-        self.k_cache = torch.zeros((shape.layers, shape.heads, shape.max_len, hd), dtype=torch.float16, device=device)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        if cache_bits == 4:
+            # a layer: uint8 [1 sequence][heads][max_len][row bytes]
+            caches = [rk.kv4_cache(1, shape.heads, shape.max_len, hd, device=device) for _ in range(shape.layers)]
+            self.k_cache, self.v_cache = ([c[j] for c in caches] for j in range(2))
+        else:
+            self.k_cache = torch.zeros((shape.layers, shape.heads, shape.max_len, hd), dtype=torch.float16, device=device)
+            self.v_cache = torch.zeros_like(self.k_cache)
         # work buffers of the one-token path
         z = lambda k: torch.zeros(k, dtype=torch.float16, device=device)
         self._x, self._x2, self._h, self._qkv, self._q, self._att = z(d), z(d), z(d), z(3 * d), z(d), z(d)
@@ -93,26 +105,93 @@ class QuantizedLlama(torch.nn.Module):
         returns the logits of the last token ([1, vocab]), or of every token ([T, vocab]) with
         ``all_logits``.  Attention looks at cache positions <= the token's own."""
         sh = self.shape
-        T, d, f = tokens.numel(), sh.d_model, sh.d_ff
+        T, d = tokens.numel(), sh.d_model
         x = self.embed[tokens]                                                     # [T, d]
-        key_pos = torch.arange(sh.max_len, device=x.device)
-        mask = key_pos[None, :] <= pos[:, None]                                    # [T, max_len]
+        if self.cache_bits == 4:
+            # the rows a chunk reads back (one token: none, the attention reads the cache itself)
+            rows = 1 if T == 1 else int(pos[-1]) + 1
+            attend = lambda i, q, k, v: self._attend_kv4(i, q, k, v, pos, rows)
+        else:
+            key_pos = torch.arange(sh.max_len, device=x.device)
+            mask = key_pos[None, :] <= pos[:, None]                                # [T, max_len]
+
+            def attend(i, q, k, v):
+                self.k_cache[i].index_copy_(1, pos, k.transpose(0, 1))
+                self.v_cache[i].index_copy_(1, pos, v.transpose(0, 1))
+                o = torch.nn.functional.scaled_dot_product_attention(q.transpose(0, 1), self.k_cache[i], self.v_cache[i],
+                                                                     attn_mask=mask[None])  # [heads, T, hd]
+                return o.transpose(0, 1).reshape(T, d)
+        x = self._layers(x, pos, attend)
+        h = self._rms(x if all_logits else x[-1:], self.final_norm)
+        return (h @ self.lm_head.t()).float()                                      # [T or 1, vocab]
+
+    def _layers(self, x, pos, attend):
+        """The decoder layers over the residual stream x [T, d] of tokens at positions pos; ``attend(i, q, k, v)`` is layer i's
+        attention on rotated q, k and v [T, heads, head_dim] -> [T, d]."""
+        sh = self.shape
+        T, d, f = x.size(0), sh.d_model, sh.d_ff
         for i, blk in enumerate(self.blocks):
             h = self._rms(x, blk.norm1)
             q, k, v = blk.qkv_proj(h).split(d, dim=-1)
             q = self._rope(q.reshape(T, sh.heads, sh.head_dim), pos)
             k = self._rope(k.reshape(T, sh.heads, sh.head_dim), pos)
             v = v.reshape(T, sh.heads, sh.head_dim)
-            self.k_cache[i].index_copy_(1, pos, k.transpose(0, 1))
-            self.v_cache[i].index_copy_(1, pos, v.transpose(0, 1))
-            o = torch.nn.functional.scaled_dot_product_attention(q.transpose(0, 1), self.k_cache[i], self.v_cache[i],
-                                                                 attn_mask=mask[None])      # [heads, T, hd]
-            x = x + blk.o_proj(o.transpose(0, 1).reshape(T, d))
+            x = x + blk.o_proj(attend(i, q, k, v))
             h = self._rms(x, blk.norm2)
             g, u = blk.gate_up_proj(h).split(f, dim=-1)
             x = x + blk.down_proj(torch.nn.functional.silu(g) * u)
-        h = self._rms(x if all_logits else x[-1:], self.final_norm)
-        return (h @ self.lm_head.t()).float()                                      # [T or 1, vocab]
+        return x
+
+    def _attend_kv4(self, i, q, k, v, pos, rows):
+        """Layer i's attention through the 4-bit cache: append k and v at pos, attend to what the cache then stands for."""
+        T, d = q.size(0), self.shape.d_model
+        rk.kv4_append(k, v, self.k_cache[i], self.v_cache[i], pos[:1], timed=False)
+        out = torch.empty_like(q)
+        if T == 1:
+            rk.kv4_attn_decode(q, self.k_cache[i], self.v_cache[i], pos, out, timed=False)
+            return out.reshape(T, d)
+        ks, vs = (torch.empty((rows, self.shape.heads, self.shape.head_dim), dtype=torch.float16, device=q.device) for _ in range(2))
+        rk.kv4_read(self.k_cache[i], self.v_cache[i], ks, vs, timed=False)
+        rk.attn_prompt(q, ks, vs, out, timed=False)
+        return out.reshape(T, d)
+
+    # ---------------------------------------------------------------- whole prompts
+
+    def forward_prompt(self, tokens, lens=None, all_logits=False, half_logits=False, store=False):
+        """Whole prompts in one pass: tokens [T] long holds sequences of ``lens`` tokens one behind the other (None: one
+        sequence), each from position 0 and seeing only itself.  Returns the logits of every sequence's last token
+        ([sequences, vocab]; of every token, [T, vocab], with ``all_logits``; fp16 as the lm_head product leaves them with
+        ``half_logits``).  ``store`` (one sequence): its keys and values go into the cache, positions 0 .. T-1, for
+        ``decode_step`` to go on from; the prompt itself attends to them as they are before a 4-bit cache rounds them."""
+        sh = self.shape
+        T = tokens.numel()
+        lens = [T] if lens is None else [int(n) for n in lens]
+        if sum(lens) != T or not lens or min(lens) < 1:
+            raise ValueError("lens must be positive and add up to the number of tokens")
+        if max(lens) > sh.max_len:
+            raise ValueError(f"a prompt of {max(lens)} tokens exceeds the model's max_len {sh.max_len}")
+        if store and len(lens) != 1:
+            raise ValueError("store takes one sequence: the cache holds one")
+        dev = self.embed.device
+        pos = torch.cat([torch.arange(n) for n in lens]).to(dev)
+        ends = torch.tensor(lens).cumsum(0)
+        q_start = torch.cat([torch.zeros(1, dtype=torch.long), ends]).to(torch.int32).to(dev)
+        zero = torch.zeros(1, dtype=torch.long, device=dev)
+
+        def attend(i, q, k, v):
+            if store and self.cache_bits == 4:
+                rk.kv4_append(k, v, self.k_cache[i], self.v_cache[i], zero, timed=False)
+            elif store:
+                self.k_cache[i, :, :T] = k.transpose(0, 1)
+                self.v_cache[i, :, :T] = v.transpose(0, 1)
+            out = torch.empty_like(q)
+            rk.attn_prompt(q, k, v, out, q_start=q_start, max_k=max(lens), timed=False)
+            return out.reshape(T, sh.d_model)
+
+        x = self._layers(self.embed[tokens.to(dev)], pos, attend)
+        h = self._rms(x if all_logits else x[(ends - 1).to(dev)], self.final_norm)
+        logits = h @ self.lm_head.t()
+        return logits if half_logits else logits.float()
 
     # ---------------------------------------------------------------- fused one-token path
 
@@ -132,7 +211,8 @@ class QuantizedLlama(torch.nn.Module):
 
         ``fuse`` (default): five launches per layer - the qkv and gate/up projections do the residual add and
         RMS norm in their prologue, the down projection the SiLU gate, and one kernel rotates q and k, appends
-        to the cache and attends.  ``fuse=False``: the same arithmetic as nine launches per layer."""
+        to the cache and attends (with a 4-bit cache one that rotates and appends, and the attention).  ``fuse=False``: the
+        same arithmetic as nine launches per layer."""
         sh = self.shape
         lib = rk.library()
         stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
@@ -191,6 +271,23 @@ class QuantizedLlama(torch.nn.Module):
                                                out.data_ptr(), layer.out_features, layer.in_features, layer.S,
                                                layer.carry_mode, stream, None))
 
+        def attend(i):
+            # rotation, append and attention of layer i from self._qkv to self._att
+            if self.cache_bits == 4:
+                q = self._q.view(1, sh.heads, sh.head_dim)
+                rk.kv4_rope_append(self._qkv.view(1, -1), self.cos, self.sin, pos, q, self.k_cache[i], self.v_cache[i], timed=False)
+                rk.kv4_attn_decode(q, self.k_cache[i], self.v_cache[i], pos, self._att.view(1, sh.heads, sh.head_dim), timed=False)
+            elif fuse:
+                ok(lib.rptc_rope_attn_decode(self._qkv.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(), pos.data_ptr(),
+                                             self.k_cache[i].data_ptr(), self.v_cache[i].data_ptr(), self._att.data_ptr(),
+                                             sh.heads, sh.head_dim, sh.max_len, stream))
+            else:
+                ok(lib.rptc_rope_cache(self._qkv.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(), pos.data_ptr(),
+                                       self._q.data_ptr(), self.k_cache[i].data_ptr(), self.v_cache[i].data_ptr(),
+                                       sh.heads, sh.head_dim, sh.max_len, stream))
+                ok(lib.rptc_attn_decode(self._q.data_ptr(), self.k_cache[i].data_ptr(), self.v_cache[i].data_ptr(),
+                                        pos.data_ptr(), self._att.data_ptr(), sh.heads, sh.head_dim, sh.max_len, stream))
+
         if not input_ready:
             self._x.copy_(self.embed[token].reshape(-1))
         delta = None
@@ -198,9 +295,7 @@ class QuantizedLlama(torch.nn.Module):
             xa, xb = self._x, self._x2          # the residual stream alternates between two buffers
             for i, blk in enumerate(self.blocks):
                 gemv_norm(blk.qkv_proj, xa, delta, blk.norm1, xb, self._qkv)
-                ok(lib.rptc_rope_attn_decode(self._qkv.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(), pos.data_ptr(),
-                                             self.k_cache[i].data_ptr(), self.v_cache[i].data_ptr(), self._att.data_ptr(),
-                                             sh.heads, sh.head_dim, sh.max_len, stream))
+                attend(i)
                 gemv(blk.o_proj, self._att, self._o)
                 gemv_norm(blk.gate_up_proj, xb, self._o.data_ptr(), blk.norm2, xa, self._gu)
                 gemv_silu(blk.down_proj, self._gu, self._down)
@@ -215,11 +310,7 @@ class QuantizedLlama(torch.nn.Module):
             ok(lib.rptc_add_rmsnorm(self._x.data_ptr(), delta, blk.norm1.data_ptr(), self._x.data_ptr(),
                                     self._h.data_ptr(), d, self.EPS, stream))
             gemv(blk.qkv_proj, self._h, self._qkv)
-            ok(lib.rptc_rope_cache(self._qkv.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(), pos.data_ptr(),
-                                   self._q.data_ptr(), self.k_cache[i].data_ptr(), self.v_cache[i].data_ptr(),
-                                   sh.heads, sh.head_dim, sh.max_len, stream))
-            ok(lib.rptc_attn_decode(self._q.data_ptr(), self.k_cache[i].data_ptr(), self.v_cache[i].data_ptr(),
-                                    pos.data_ptr(), self._att.data_ptr(), sh.heads, sh.head_dim, sh.max_len, stream))
+            attend(i)
             gemv(blk.o_proj, self._att, self._o)
             ok(lib.rptc_add_rmsnorm(self._x.data_ptr(), self._o.data_ptr(), blk.norm2.data_ptr(), self._x.data_ptr(),
                                     self._h.data_ptr(), d, self.EPS, stream))
@@ -244,9 +335,9 @@ def check_context(shape, prompt_len, new_tokens):
                          f"cache positions, the model was built with max_len = {shape.max_len}")
 
 
-def greedy_decode(model, prompt, new_tokens, mode="fused_graph"):
-    """Prefill the prompt (in chunks of 32 tokens: the batch the fused mat-mat kernel takes), then decode
-    ``new_tokens`` greedily one at a time.  mode: "fused_graph" (five launches per layer, one HIP graph per
+def greedy_decode(model, prompt, new_tokens, mode="fused_graph", whole_prompt=False):
+    """Prefill the prompt (in chunks of 32 tokens: the batch the fused mat-mat kernel takes; with ``whole_prompt`` in one
+    pass through ``forward_prompt``), then decode ``new_tokens`` greedily one at a time.  mode: "fused_graph" (five launches per layer, one HIP graph per
     token), "fused" (the same, direct launches), "glue_graph" / "glue" (nine launches per layer: the
     element-wise steps as kernels of their own), "torch_graph" / "torch" (framework ops between the projections).
     Returns (token list, seconds spent in the decode loop)."""
@@ -262,7 +353,9 @@ def greedy_decode(model, prompt, new_tokens, mode="fused_graph"):
         step = model.forward_tokens
     with torch.no_grad():
         logits = None
-        for p0 in range(0, P, 32):
+        if whole_prompt:
+            logits = model.forward_prompt(prompt, store=True)
+        for p0 in range(0, 0 if whole_prompt else P, 32):
             chunk = prompt[p0:p0 + 32]
             logits = model.forward_tokens(chunk, torch.arange(p0, p0 + chunk.numel(), device=dev))
         tok = logits.argmax(-1)                                                    # [1]
