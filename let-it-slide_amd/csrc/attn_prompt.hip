@@ -8,7 +8,8 @@
 // Scores, m, l and the output sums are fp32; p is rounded to the inputs' type for the matrix unit (relative 2^-12 or
 // 2^-9, as the products need two operands of one type), l adds the unrounded p.
 //
-// A workgroup of four waves owns kRows = 128 query rows of one head, 32 a wave, and walks over its keys 64 at a time.
+// A workgroup of four waves owns 128 query rows of one head (64 or 32 in the forms for fewer rows), 32 a wave, and walks over its
+// keys 64 at a time.
 // The products are formed transposed, S^T = K Q^T and O^T = V^T P^T with 32x32x16 matrix instructions: a lane then holds
 // scores of one query only (the row maximum is 31 maxima in the lane and one swap of the wave's halves), the scores'
 // layout is, up to a renumbering of the keys that V follows, the layout the second product wants P in, and every
@@ -20,8 +21,7 @@
 namespace rptc {
 
 constexpr int kPromptThreads = 256;
-constexpr int kRows = 128;             // query rows of a workgroup
-constexpr int kKeys = 64;              // keys of a step
+constexpr int kWideRows = 128;         // query rows of a workgroup of the wide kernel
 constexpr float kLazy = 8.f;           // exponents of 2 a score may exceed the running bound by
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
@@ -354,13 +354,22 @@ struct PromptWave {
     }
 };
 
-// Many rows: 128 query rows of a head a workgroup, 32 a wave; all waves walk over the same keys, which are brought to LDS
-// once for the four of them, a step ahead.
-template <int HD, class T>
+// Many rows: 128 query rows of a head a workgroup, 32 a wave (G = 1); all waves walk over the same keys, which are brought to
+// LDS once for the four of them, a step ahead.  G = 2: 64 query rows, two waves a row, one for the first and one for the second half of
+// a step's 64 keys, joined at the end: twice the workgroups with half the walk, where the longest walk is what the call waits
+// for (64 keys a wave and a step of 128 need twice the LDS: 1024 rows of 32 heads x 128 29.4 us instead of 21.6; G = 1 with
+// 32 keys a step meets twice as often: 8192 rows 567 us instead of 520).
+template <int HD, int G>
+constexpr int kWaveKeys = G == 2 ? 32 : 64;    // keys of a step and wave
+
+template <int HD, class T, int G>
 __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_kernel(const PromptArgs a)
 {
     extern __shared__ __align__(16) uint16_t lds[];       // two buffers of K, two of V, [kKeys][HD] each
-    constexpr int kTile = kKeys * HD;
+    constexpr int kMine = kWaveKeys<HD, G>, kKeys = G * kMine, kTile = kKeys * HD, kRows = kWideRows / G;
+    static_assert(G == 1 || 2 * 32 * HD * 4 <= 4 * kTile * 2, "the sums of two waves fit where K and V were");
+    __shared__ float s_ml[2][32][2];
+    __shared__ int s_odd[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int c = lane >> 5, col = lane & 31;
     int head, tile, split;
@@ -370,7 +379,8 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
     const int kvh = head / (a.heads / a.kv_heads);
 
     const int k_hi = uniform(prompt_sees(a, t, min(t.row0 + kRows, t.q_end) - 1));      // of the tile's last row: the most
-    const int row_first = t.row0 + 32 * wave, row = row_first + col;
+    const int group = G == 2 ? wave >> 1 : 0, koff = group * kMine;
+    const int row_first = t.row0 + 32 * (wave & (4 / G - 1)), row = row_first + col;
     const bool wave_live = row_first < t.q_end;
     const int see = row < t.q_end ? prompt_sees(a, t, row) : 0;
     // what all rows of the wave see, and what one of them sees
@@ -407,41 +417,76 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
         request_v(0, 0);
         if (kKeys < k_hi) request_k(kKeys, 1);
     }
-    PromptWave<HD, T, kKeys, 1> w;
+    PromptWave<HD, T, kMine, 1> w;
     w.begin(a, t, row, head);
     w.settle();
     // One step: the softmax of the scores s of the keys from k0 on and their product with V, while the matrix unit forms the
     // next step's scores (behind the last step these are of whatever the buffer holds, and nobody looks at them).
-    auto step = [&](int k0, int buf, float16_t (&s)[2], float16_t (&next)[2]) {
+    auto step = [&](int k0, int buf, float16_t (&s)[kMine / 32], float16_t (&next)[kMine / 32]) {
         wait_for_lds_loads();                              // this wave's part of the next K and of this V is in LDS
         __syncthreads();                                   // everyone's is, and nobody reads what is requested over now
         if (k0 + 2 * kKeys < k_hi) request_k(k0 + 2 * kKeys, buf);
         if (k0 + kKeys < k_hi) request_v(k0 + kKeys, buf ^ 1);
-        if (k0 >= see_most) return;
-        if (k0 + kKeys > see_least) w.mask(s, see - k0);   // some row of the wave does not see all of the step's keys
+        if (k0 + koff >= see_most) return;
+        if (k0 + koff + kMine > see_least) w.mask(s, see - k0 - koff);   // some row of the wave does not see all of its keys
         const float off = w.bound(s, a.c);
-        w.scores(lds + (buf ^ 1) * kTile, next);
-        uint32_t p[1][2][8];
+        w.scores(lds + (buf ^ 1) * kTile + koff * HD, next);
+        uint32_t p[1][kMine / 32][8];
         w.weights(s, a.c, off, p);
-        w.product(lds + (2 + buf) * kTile, p);
+        w.product(lds + (2 + buf) * kTile + koff * HD, p);
     };
     if (k_hi > 0) {
-        float16_t sa[2], sb[2];
+        float16_t sa[kMine / 32], sb[kMine / 32];
         wait_for_lds_loads();
         __syncthreads();
-        w.scores(lds, sa);
+        w.scores(lds + koff * HD, sa);
         for (int k0 = 0; k0 < k_hi; k0 += 2 * kKeys) {
             step(k0, 0, sa, sb);
             if (k0 + kKeys >= k_hi) break;
             step(k0 + kKeys, 1, sb, sa);
         }
     }
+    bool odd = w.odd();
+    float l = halves_sum(w.l);
+    if (G == 2) {
+        // sums of the second half's waves to the first's, a register of all lanes after the other
+        float4 *sums = reinterpret_cast<float4 *>(lds) + (wave & 1) * (HD * 8) + lane;
+        __syncthreads();                                   // nobody reads K or V now
+        if (group == 1) {
+#pragma unroll
+            for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+                for (int b = 0; b < 4; b++)
+                    sums[64 * (4 * d + b)] = make_float4(w.acc[d][4 * b], w.acc[d][4 * b + 1], w.acc[d][4 * b + 2], w.acc[d][4 * b + 3]);
+            if (c == 0) {
+                s_ml[wave & 1][col][0] = w.m;
+                s_ml[wave & 1][col][1] = l;
+            }
+            if (lane == 0) s_odd[wave & 1] = odd;
+        }
+        __syncthreads();
+        if (group == 1) return;
+        odd = odd || s_odd[wave];
+        const float m1 = s_ml[wave][col][0], M = fmaxf(w.m, m1);
+        const float f0 = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - M), f1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - M);
+        l = l * f0 + s_ml[wave][col][1] * f1;
+        w.m = M;
+#pragma unroll
+        for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                const float4 o = sums[64 * (4 * d + b)];
+                w.acc[d][4 * b] = fmaf(o.x, f1, w.acc[d][4 * b] * f0);
+                w.acc[d][4 * b + 1] = fmaf(o.y, f1, w.acc[d][4 * b + 1] * f0);
+                w.acc[d][4 * b + 2] = fmaf(o.z, f1, w.acc[d][4 * b + 2] * f0);
+                w.acc[d][4 * b + 3] = fmaf(o.w, f1, w.acc[d][4 * b + 3] * f0);
+            }
+    }
     if (!wave_live) return;
-    if (w.odd()) {
+    if (odd) {
         prompt_rows_plain<HD, T>(a, t, row_first, 32, head, kvh, 0, k_hi, 0);
         return;
     }
-    const float l = halves_sum(w.l);
     const float inv = l == 0.f ? 0.f : 1.f / l;            // a row that sees nothing: zeros
     uint16_t *o = a.out + (int64_t)min(row, t.q_end - 1) * a.st.out_token + (int64_t)head * a.st.out_head + 8 * c;
 #pragma unroll
@@ -617,15 +662,17 @@ __global__ __launch_bounds__(kJoinThreads) void attn_prompt_merge_kernel(const P
     if (a.lse && threadIdx.x == 0) a.lse[at] = l == 0.f ? -INFINITY : (M + log2f(l)) * 0.693147180559945f;
 }
 
-template <int HD>
-static constexpr size_t prompt_lds() { return (size_t)2 * 2 * kKeys * HD * 2; }
+template <int HD, int G>
+static constexpr size_t prompt_lds() { return (size_t)2 * 2 * G * kWaveKeys<HD, G> * HD * 2; }
 template <int HD>
 static constexpr size_t narrow_lds() { return (size_t)4 * 2 * kNarrowKeys<HD> * HD * 2; }
 
 template <int HD, class T>
 static int prepare_prompt()
 {
-    const int rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<HD, T>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<HD>());
+    int rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<HD, T, 1>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<HD, 1>());
+    if (rc) return rc;
+    rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<HD, T, 2>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<HD, 2>());
     if (rc) return rc;
     return (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_narrow_kernel<HD, T>), hipFuncAttributeMaxDynamicSharedMemorySize, narrow_lds<HD>());
 }
@@ -642,29 +689,40 @@ int prepare_attn_prompt()
 }
 
 struct PromptPlan {
-    bool narrow;
+    int rows;                              // query rows of a workgroup: 128 or 64 (the wide kernel), 32 (the narrow one)
     int tiles, splits;
 };
 
 // sequences cut into tiles: at most so many (whatever the sequences' lengths are)
 static int64_t prompt_tiles(int64_t seqs, int64_t total_q, int64_t rows) { return (total_q + seqs * (rows - 1)) / rows; }
 
-// Which of the two kernels, by the estimates that the measurements below fit (us; steps: 64 keys of the longest walk):
-// a workgroup of 128 rows takes 6 + 1 a step whether its compute unit has one or two of them, one of 32 rows 8 + 0.4 a step
-// (its four waves share the walk, but also fetch four times the K and V a row: later rounds of them, half as long on
-// average where they are causal, cost more than their share).  Measured (128 rows / 32 rows): 512 rows of 32 heads x 128
-// 15.4 / 18.7, 1024 rows 25.7 / 41, 2300 rows of 8 heads 43.7 / 37.5, of 2 heads 42.4 / 26.8, 1000 rows of 16 heads x 64 17.5 / 10.5,
-// 37 rows of 32 heads 6.7 / 8.4, 32 rows behind 8000 124 / 30 (split).  The keys of a call that leaves compute units without a
-// workgroup are split, not below 512 a piece, and a second launch joins the pieces.
+// Which form, by the workgroups that 128 rows each would make for every compute unit (w) and the steps of 64 keys of the longest walk (s).
+// 128 rows read K and V least often and win where they fill the places of the compute units (3 a unit up to hd 64, 2 at 128, 1 at 256);
+// measured 128 / 64 rows, us: hd 128 w 1.5 37.2 / 36.8, w 2 52.2 / 55.9, w 3 91.8 / 107.7, w 8 520 / 609; hd 64 w 2 60.3 / 51.6, w 3
+// 56.5 / 56.5, w 5 31.6 / 35.2; hd 256 w 1 104.7 / 88.5, w 1.5 143 / 175.  Below that the longest walk decides, and the two other
+// forms by the estimates that fit the measurements: 64 rows take h0 + h1 a step, more where compute units have several; the
+// narrow form, whose four waves share a walk but fetch four times the K and V a row, n0 + 2 n1 a step for its first round of
+// workgroups (r of them, shorter and shorter as the walk of a causal prompt does).  Measured 64 / 32 rows, us: hd 128 300 rows
+// of 8 heads 9.8 / 10.9, 1000 rows of 8 17.9 / 15.9, of 16 18.6 / 24.3, 2300 rows of 2 30.9 / 23.0; hd 64 400 rows of 32
+// 8.6 / 8.8, 1000 rows of 16 13.1 / 12.2, 2400 rows of 4 23.0 / 18.4, 2000 rows of 16 21.6 / 27.7; hd 256 700 rows of 8
+// 30.5 / 22.5, 300 rows of 32 19.1 / 26.8; 32 rows of 32 heads x 128 behind 8000 91 / 30 (keys split).  The keys of a call that
+// leaves compute units without a workgroup are split, not below 512 a piece, and a second launch joins the pieces.
 static PromptPlan prompt_plan(int64_t seqs, int64_t total_q, int64_t heads, int64_t hd, int64_t max_k, int cus)
 {
-    PromptPlan p = {false, (int)prompt_tiles(seqs, total_q, kRows), 1};
-    const double steps = (double)(max_k + 63) / 64;
-    const double wide = (double)p.tiles * heads / (2.0 * cus);
-    const int64_t tiles = prompt_tiles(seqs, total_q, kNarrowRows), slots = (int64_t)cus * (hd > 64 ? 1 : 2);
-    const double rounds = (double)tiles * heads / (double)slots < 1 ? 1 : (double)tiles * heads / (double)slots;
-    if (6 + steps * (wide < 1 ? 1 : wide) <= 8 * rounds + 0.2 * steps * (1 + rounds)) return p;
-    p.narrow = true;
+    struct Form { double full, h0, h1, share0, share1, n0, n1; int places; };
+    static const Form forms[3] = {{3.00, 5.5, 0.47, 0.50, 0.50, 6, 0.17, 2}, {1.75, 6, 0.75, 0.45, 0.90, 8, 0.20, 1}, {1.00, 7, 2.10, 0, 1, 14, 0.35, 1}};
+    const Form &f = forms[hd <= 64 ? 0 : hd == 128 ? 1 : 2];
+    PromptPlan p = {kWideRows, (int)prompt_tiles(seqs, total_q, kWideRows), 1};
+    const double w = (double)p.tiles * heads / cus, s = (double)(max_k + 63) / 64;
+    if (w > f.full) return p;
+    const int64_t tiles = prompt_tiles(seqs, total_q, kNarrowRows), slots = (int64_t)cus * f.places;
+    const double share = f.share0 + f.share1 * w, r = (double)tiles * heads / (double)slots;
+    if (f.h0 + f.h1 * s * (share < 1 ? 1 : share) <= f.n0 * (r < 1 ? 1 : r) + f.n1 * s * (1 + (r < 1 ? 1 : r))) {
+        p.rows = kWideRows / 2;
+        p.tiles = (int)prompt_tiles(seqs, total_q, p.rows);
+        return p;
+    }
+    p.rows = kNarrowRows;
     p.tiles = (int)tiles;
     int64_t n = slots / (tiles * heads);
     if (n > max_k / 512) n = max_k / 512;
@@ -682,11 +740,15 @@ static int prompt_sizes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t 
 }
 
 template <int HD, class T>
-static void launch_prompt(const PromptArgs &a, bool narrow, hipStream_t s)
+static void launch_prompt(const PromptArgs &a, int rows, hipStream_t s)
 {
     const dim3 grid((unsigned)(a.heads * a.tiles * a.splits));
-    if (!narrow) {
-        hipLaunchKernelGGL((attn_prompt_kernel<HD, T>), grid, dim3(kPromptThreads), prompt_lds<HD>(), s, a);
+    if (rows == kWideRows) {
+        hipLaunchKernelGGL((attn_prompt_kernel<HD, T, 1>), grid, dim3(kPromptThreads), (prompt_lds<HD, 1>()), s, a);
+        return;
+    }
+    if (rows == kWideRows / 2) {
+        hipLaunchKernelGGL((attn_prompt_kernel<HD, T, 2>), grid, dim3(kPromptThreads), (prompt_lds<HD, 2>()), s, a);
         return;
     }
     hipLaunchKernelGGL((attn_prompt_narrow_kernel<HD, T>), grid, dim3(kPromptThreads), narrow_lds<HD>(), s, a);
@@ -767,10 +829,10 @@ extern "C" int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint
     if ((rc = timer.begin(dev, s, ms))) return rc;
     const bool f16 = dtype == RPTC_F16;
     switch (hd) {
-    case 32: f16 ? launch_prompt<32, TypeF16>(a, plan.narrow, s) : launch_prompt<32, TypeBf16>(a, plan.narrow, s); break;
-    case 64: f16 ? launch_prompt<64, TypeF16>(a, plan.narrow, s) : launch_prompt<64, TypeBf16>(a, plan.narrow, s); break;
-    case 128: f16 ? launch_prompt<128, TypeF16>(a, plan.narrow, s) : launch_prompt<128, TypeBf16>(a, plan.narrow, s); break;
-    default: f16 ? launch_prompt<256, TypeF16>(a, plan.narrow, s) : launch_prompt<256, TypeBf16>(a, plan.narrow, s); break;
+    case 32: f16 ? launch_prompt<32, TypeF16>(a, plan.rows, s) : launch_prompt<32, TypeBf16>(a, plan.rows, s); break;
+    case 64: f16 ? launch_prompt<64, TypeF16>(a, plan.rows, s) : launch_prompt<64, TypeBf16>(a, plan.rows, s); break;
+    case 128: f16 ? launch_prompt<128, TypeF16>(a, plan.rows, s) : launch_prompt<128, TypeBf16>(a, plan.rows, s); break;
+    default: f16 ? launch_prompt<256, TypeF16>(a, plan.rows, s) : launch_prompt<256, TypeBf16>(a, plan.rows, s); break;
     }
     return timer.end();
 }

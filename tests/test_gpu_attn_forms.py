@@ -1,0 +1,184 @@
+"""rptc_kernels.attn_prompt where it takes its forms for many rows: 128 query rows a workgroup (calls that fill the device) and 64
+(calls whose longest walk over the keys counts), against the formula in 64 bits.  Tolerances as derived in
+test_gpu_attn_prompt.py: one rounding of the output, one of every weight, fp32 scores."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def rk():
+    import rptc_kernels
+    assert torch.cuda.is_available(), "GPU tests need a GPU"
+    assert rptc_kernels.library().rptc_init() == 0
+    return rptc_kernels
+
+
+@pytest.fixture(autouse=True)
+def _announce(request):
+    print(f"\n[case] {request.node.nodeid}", flush=True)
+    yield
+
+
+def randn(seed, *shape, dtype=F16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(shape, generator=g, device="cuda").to(dtype)
+
+
+def ints(xs):
+    return torch.tensor(xs, dtype=torch.int32, device="cuda")
+
+
+def formula(q, k, v, causal):
+    """out, lse [n, heads], tolerances of both for one sequence, in 64 bits."""
+    n, H, hd = q.shape
+    L, g, u = k.size(0), H // k.size(1), torch.finfo(q.dtype).eps / 2
+    qd = q.double().transpose(0, 1)
+    kd = k.double().repeat_interleave(g, 1).permute(1, 2, 0).contiguous()
+    vd = v.double().repeat_interleave(g, 1).transpose(0, 1).contiguous()
+    s = torch.matmul(qd, kd) * hd ** -0.5
+    see = torch.ones(n, L, dtype=torch.bool, device=q.device)
+    if causal:
+        see = torch.arange(L, device=q.device)[None] <= torch.arange(n, device=q.device)[:, None] + L - n
+    s = s.masked_fill(~see, -math.inf)
+    E = hd ** -0.5 * (hd + 4) * 2.0 ** -24 * torch.matmul(qd.abs(), kd.abs()).masked_fill(~see, 0).amax(-1, keepdim=True)
+    lse = torch.logsumexp(s, -1, keepdim=True)
+    p = torch.exp(s - lse.masked_fill(torch.isinf(lse), 0))
+    o, A = torch.matmul(p, vd), torch.matmul(p, vd.abs())
+    tol = u * o.abs() + (u + 3 * E) * A + 2.0 ** -25
+    if q.dtype == F16:
+        tol = tol + see.sum(-1)[None, :, None] * 2.0 ** -25 * vd.abs().amax()
+    ltol = 2 * E + 2.0 ** -21 * (1 + lse.abs().nan_to_num(posinf=0))
+    return o.transpose(0, 1), lse[..., 0].t(), tol.transpose(0, 1), ltol[..., 0].t()
+
+
+def check(out, lse, q, k, v, causal):
+    o, l, tol, ltol = formula(q, k, v, causal)
+    err = (out.double() - o).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+    none = torch.isinf(l)
+    assert torch.equal(torch.isinf(lse), none) and bool((out[none] == 0).all())
+    assert bool(((lse.double() - l).abs()[~none] <= ltol[~none]).all())
+
+
+def run(rk, lq, lk, heads, kvh, hd, dtype, causal, spoil=False):
+    tq, tk = sum(lq), sum(lk)
+    q, k, v = randn(1, tq + 9, heads, hd, dtype=dtype), randn(2, tk + 70, kvh, hd, dtype=dtype), randn(3, tk + 70, kvh, hd, dtype=dtype)
+    qs, ks = [0], [0]
+    for a, b in zip(lq, lk):
+        qs.append(qs[-1] + a)
+        ks.append(ks[-1] + b)
+    if spoil:
+        # what lies behind the last key: never seen
+        k[tk:], v[tk:] = float("nan"), float("inf")
+    out, lse = torch.full_like(q, 7.0), torch.full((tq + 9, heads), 7.0, device="cuda")
+    rk.attn_prompt(q, k, v, out, q_start=ints(qs), k_start=ints(ks[:-1]), k_len=ints(lk), lse=lse, causal=causal, max_k=max(lk), timed=False)
+    assert bool((out[tq:] == 7).all()) and bool((lse[tq:] == 7).all())      # rows behind the last sequence
+    for i in range(len(lq)):
+        a, b = slice(qs[i], qs[i + 1]), slice(ks[i], ks[i + 1])
+        if lq[i]:
+            check(out[a], lse[a], q[a], k[b], v[b], causal)
+    return q, k, v, out
+
+
+# 28 sequences of 32 heads: more workgroups of 128 rows than the device has places
+MANY = [1, 0, 127, 128, 129, 33, 300, 2, 64, 65, 31, 96, 7, 260] * 2
+
+
+@pytest.mark.parametrize("hd,dtype,causal", [(32, F16, True), (64, F16, True), (64, BF16, False), (128, F16, True), (128, BF16, True), (256, F16, True),
+                                             (256, BF16, False)])
+def test_calls_that_fill_the_device(rk, hd, dtype, causal):
+    run(rk, MANY, MANY, 32, 8, hd, dtype, causal, spoil=True)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_fuller_and_emptier_contexts_than_queries(rk, hd):
+    # chunks behind a context, and more queries than keys (the first see nothing); one sequence without keys
+    past = [0, 70, -20, 500, 1, -1, 64] * 4
+    run(rk, MANY, [max(0, n + p) for n, p in zip(MANY, past)], 32, 4, hd, F16, True)
+
+
+@pytest.mark.parametrize("lq,lk,heads,kvh,hd,dtype,causal", [
+    ([400], [400], 32, 8, 32, F16, True), ([400], [400], 32, 32, 64, F16, True), ([390, 1, 0, 63], [390, 1, 0, 63], 32, 8, 64, BF16, True),
+    ([512], [512], 32, 32, 128, F16, True), ([333, 64], [340, 200], 32, 8, 128, BF16, True), ([450], [415], 32, 4, 128, F16, True),
+    ([130], [77], 32, 8, 128, F16, False), ([300], [300], 32, 8, 256, F16, True), ([257], [129], 32, 16, 256, BF16, False),
+])
+def test_calls_whose_longest_walk_counts(rk, lq, lk, heads, kvh, hd, dtype, causal):
+    run(rk, lq, lk, heads, kvh, hd, dtype, causal, spoil=True)
+
+
+@pytest.mark.parametrize("lens,hd", [([512], 128), ([400], 64), (MANY, 64), (MANY, 128)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_what_a_query_does_not_see_does_not_reach_it(rk, lens, hd, bad):
+    # the last two keys of every sequence hold no numbers: only its last two queries may show it
+    q, k, v, want = run(rk, lens, lens, 32, 8, hd, F16, True)
+    starts = [0]
+    for n in lens:
+        starts.append(starts[-1] + n)
+        if n > 1:
+            k[starts[-1] - 1], v[starts[-1] - 2:starts[-1]] = bad, bad
+    out = torch.empty_like(q)
+    rk.attn_prompt(q, k, v, out, q_start=ints(starts), k_start=ints(starts[:-1]), k_len=ints(lens), max_k=max(lens), timed=False)
+    for i, n in enumerate(lens):
+        if n > 2:
+            rows = slice(starts[i], starts[i + 1] - 2)
+            # the rows of a wave that met such a value are worked out again one after the other, in another order
+            tol = 2 * formula(*(t[rows] for t in (q, k, v)), True)[2]
+            assert bool(((out[rows].double() - want[rows].double()).abs() <= tol).all())
+            assert not bool(torch.isfinite(out[starts[i + 1] - 1]).any())
+
+
+@pytest.mark.parametrize("heads,n,hd", [(32, 400, 64), (32, 512, 128), (32, 3400, 64)])
+def test_scores_that_rise_and_fall_along_the_keys(rk, heads, n, hd):
+    # the bound is raised again and again, or never after the first step; the two halves of a step differ by far
+    q = torch.ones(n, heads, hd, dtype=F16, device="cuda")
+    v = randn(11, n, 4, hd)
+    for sign in (1, -1):
+        k = (sign * torch.linspace(-40, 40, n, device="cuda"))[:, None, None].expand(n, 4, hd).half().contiguous()
+        out, lse = torch.empty_like(q), torch.empty(n, heads, device="cuda")
+        rk.attn_prompt(q, k, v, out, lse=lse, timed=False)
+        for h in range(0, heads, 8):        # a key head's queries are all alike
+            check(out[:, h:h + 1], lse[:, h:h + 1], q[:, h:h + 1], k[:, h // 8:h // 8 + 1], v[:, h // 8:h // 8 + 1], True)
+
+
+def test_the_same_bits_again_on_another_stream_and_in_a_graph(rk):
+    for n in (512, 3000):
+        q, k, v = randn(21, n, 32, 64), randn(22, n, 8, 64), randn(23, n, 8, 64)
+        out, again = torch.empty_like(q), torch.empty_like(q)
+        rk.attn_prompt(q, k, v, out, timed=False)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            rk.attn_prompt(q, k, v, again, timed=False)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(out, again)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            rk.attn_prompt(q, k, v, again, timed=False)
+        for _ in range(3):
+            again.zero_()
+            g.replay()
+            torch.randn(1 << 20, device="cuda").sum()
+            torch.cuda.synchronize()
+            assert torch.equal(out, again)
+
+
+def test_workspace_is_asked_for(rk):
+    # few rows behind many keys are cut along the keys: their parts need room; a call without it is refused
+    import ctypes
+    lib = rk.library()
+    need = lib.rptc_attn_prompt_workspace_bytes(1, 1, 60000, 60000, 4, 2, 64)
+    assert need > 0 and lib.rptc_attn_prompt_workspace_bytes(1, 4096, 4096, 4096, 32, 8, 128) == 0
+    q, k, v = randn(1, 1, 4, 64), randn(2, 60000, 2, 64), randn(3, 60000, 2, 64)
+    out, ws = torch.full_like(q, 7.0), torch.empty(need + 16, dtype=torch.uint8, device="cuda")
+    st = rk.PromptStrides(256, 64, 128, 64, 128, 64, 256, 64)
+    call = lambda workspace, size: lib.rptc_attn_prompt(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None, None, None, None, 1, 1, 60000,
+                                                       60000, 4, 2, 64, ctypes.byref(st), 0.125, 1, 0, workspace, size, None, None)
+    assert call(None, 0) == -1 and call(ws.data_ptr(), need - 1) == -2 and call(ws.data_ptr() + 4, need) == -3
+    torch.cuda.synchronize()
+    assert bool((out == 7).all())
