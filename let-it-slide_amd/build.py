@@ -1,6 +1,8 @@
 """Build the gfx950 libraries in-tree with hipcc.
 
 librptc_hip.so        the C-ABI library of kernels (include/rptc_hip.h), from csrc/*.hip
+rptc_bindings.so      the Python entry points of the ops that run between the launches of a decode loop, from
+                      csrc/bindings.cpp (the host compiler and torch's headers; it calls the library through its C ABI)
 ../bench_aids/librptc_bench_aids.so
                       measurement aids bench.py times beside the mat-vec (an empty launch, kernels that only read,
                       instruction issue rates); beside bench.py, out of the product library, its header and its folder
@@ -10,6 +12,7 @@ import os
 import re
 import subprocess
 import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
@@ -17,6 +20,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "librptc_hip.so")
+BINDINGS = os.path.join(HERE, "rptc_bindings.so")
 AIDS_DIR = os.path.join(os.path.dirname(HERE), "bench_aids")
 AIDS_LIB = os.path.join(AIDS_DIR, "librptc_bench_aids.so")
 
@@ -126,17 +130,30 @@ def check_assembly(src, verbose=False, extra=()):
         raise RuntimeError(f"{os.path.basename(src)}: arrive() without the markers of a hand-off in the assembly")
 
 
+def build_bindings(verbose=False):
+    import torch
+    base = os.path.dirname(torch.__file__)
+    lib = os.path.join(base, "lib")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          "-isystem", os.path.join(base, "include"), "-isystem", sysconfig.get_paths()["include"],
+          os.path.join(CSRC, "bindings.cpp"), "-o", BINDINGS, f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", f"-Wl,-rpath,{lib}"], verbose)
+    return BINDINGS
+
+
 def build(verbose=False, extra=()):
     """Compiles every source (one hipcc per file, in parallel), checks the emitted assembly of the sources that hold
-    hand-written request/wait sequences, and links the two libraries."""
+    hand-written request/wait sequences, and links the two libraries; builds the Python entry points."""
     os.makedirs(OBJ, exist_ok=True)
     srcs = sources()
     objs = [os.path.join(OBJ, os.path.basename(s)[:-4] + ".o") for s in srcs]
     jobs = min(len(srcs), max(1, min(8, os.cpu_count() or 1)))
     with ThreadPoolExecutor(jobs) as pool:
+        bindings = pool.submit(build_bindings, verbose)
         list(pool.map(lambda so: _run(["hipcc", *FLAGS, *extra, "-c", so[0], "-o", so[1]], verbose), zip(srcs, objs)))
         with_asm = [s for s in srcs if re.search(r"\basm\b", open(s).read()) or "decode_asm.hpp" in open(s).read()]
         list(pool.map(lambda s: check_assembly(s, verbose, extra), with_asm))
+        bindings.result()
     _run(["hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs], verbose)
     _run(["hipcc", *FLAGS, *extra, "-shared", "-o", AIDS_LIB, os.path.join(AIDS_DIR, "probe.hip")], verbose)
     return LIB

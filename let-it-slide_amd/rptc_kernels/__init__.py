@@ -5,7 +5,8 @@ the same seven callables, positional ``torch.Tensor`` arguments, outputs written
 tensors the caller allocates, elapsed milliseconds returned as a ``float``, argument errors
 raised as ``RuntimeError`` (what ``TORCH_CHECK`` raises).  The work is done by
 ``librptc_hip.so`` through its C ABI (include/rptc_hip.h); this module only validates tensors
-and passes raw device pointers plus the current HIP stream.  There is no CPU implementation:
+and passes raw device pointers plus the current HIP stream (for the ops of a decode loop's small launches in compiled code,
+csrc/bindings.cpp).  There is no CPU implementation:
 without the library, or with CPU tensors, every op raises.
 
 Differences from the reference, all deliberate:
@@ -34,6 +35,7 @@ Sub-modules: ``packing`` (symbols -> streams), ``quantize`` (the quantizer aroun
 ``eval_ppl`` (perplexity on a token file).
 """
 import ctypes
+import importlib.util
 import os
 
 import torch
@@ -817,79 +819,27 @@ def matvec_bits_dense(compressed, codebook, out, bits):
 
 
 # ---------------------------------------------------------------- prompts, the 4-bit cache, scoring
-# These ops run between the launches of a decode loop, so their checks are plain comparisons whose messages are put together
-# only when one fails.
+# These ops run between the launches of a decode loop, where a small call is bound by the host: their checks and the call into
+# the library are compiled (csrc/bindings.cpp).
 
-_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}      # RPTC_F16, RPTC_BF16, RPTC_F32
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def _refuse(msg):
-    raise RuntimeError(msg)
+_BOUND = ("rptc_status_string", "rptc_attn_prompt_workspace_bytes", "rptc_attn_prompt", "rptc_kv4_append", "rptc_kv4_read", "rptc_kv4_rope_append",
+          "rptc_kv4_attn_decode_workspace_bytes", "rptc_kv4_attn_decode", "rptc_token_logprobs")
+_bindings = None
 
 
-def _run_on(device, timed, fn, *args):
-    """fn(*args, stream, ms) on the device's current stream; elapsed ms (0.0 when not timed)."""
-    index = device.index
-    if torch.cuda.current_device() != index:
-        with torch.cuda.device(device):
-            return _run_on(device, timed, fn, *args)
-    if _timing if timed is None else timed:
-        ms = ctypes.c_float(0.0)
-        rc = fn(*args, _raw_stream(index), ctypes.byref(ms))
-        if rc:
-            _status(rc)
-        return float(ms.value)
-    rc = fn(*args, _raw_stream(index), None)
-    if rc:
-        _status(rc)
-    return 0.0
-
-
-def _workspace(device, fn, *sizes):
-    """(tensor or None, bytes) for an op's workspace.  From torch's allocator, so it is this call's own on the current
-    stream and in a graph being captured."""
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return _workspace(device, fn, *sizes)
-    need = fn(*sizes)
-    if need < 0:
-        _status(int(need))
-    return (torch.empty(need, dtype=torch.uint8, device=device), need) if need else (None, 0)
-
-
-def _rows_ok(t, name, dtype, device):
-    # [tokens, heads, hd], any token and head strides, the head dimension contiguous
-    if not isinstance(t, torch.Tensor):
-        _refuse(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
-        _refuse(f"{name} must be a CUDA tensor")
-    if t.dim() != 3:
-        _refuse(f"{name}.dim() == 3 ([tokens, heads, head_dim])")
-    if t.dtype != dtype:
-        _refuse(f"{name} must be {str(dtype)[6:]}")
-    if t.device != device:
-        _refuse("all tensors must be on the same device")
-    a, b, c = t.stride()
-    if c != 1:
-        _refuse(f"{name} must be contiguous along the head dimension")
-    n, h, hd = t.shape
-    # the stride of a dimension of one element means nothing: any valid one will do
-    return a if n > 1 else hd, b if h > 1 else hd
-
-
-def _vector_ok(t, name, dtype, count, device):
-    if not isinstance(t, torch.Tensor):
-        _refuse(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
-        _refuse(f"{name} must be a CUDA tensor")
-    if t.dtype != dtype or t.dim() != 1 or t.size(0) != count:
-        _refuse(f"{name} must be a 1-D {str(dtype)[6:]} tensor of {count} elements")
-    if not t.is_contiguous():
-        _refuse(f"{name} must be contiguous")
-    if t.device != device:
-        _refuse("all tensors must be on the same device")
-    return t.data_ptr()
+def _load_bindings():
+    global _bindings
+    path = os.path.join(os.path.dirname(_HERE), "rptc_bindings.so")
+    if not os.path.exists(path):
+        raise RuntimeError(f"rptc_kernels: {path} is missing; build it with `python let-it-slide_amd/build.py`")
+    lib = library()
+    spec = importlib.util.spec_from_file_location("rptc_bindings", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    module.setup(tuple(ctypes.cast(getattr(lib, name), _VP).value for name in _BOUND),
+                 getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream))
+    _bindings = module
+    return module
 
 
 def attn_prompt(q, k, v, out, q_start=None, k_start=None, k_len=None, causal=True, scale=None, lse=None, max_k=None, timed=None):
@@ -903,55 +853,14 @@ def attn_prompt(q, k, v, out, q_start=None, k_start=None, k_len=None, causal=Tru
     chunk's last query sees the whole context.  ``scale`` defaults to hd ** -0.5.  ``lse`` (float32 [Tq, heads], optional)
     takes the logarithm of every row's sum.  A query that sees no key gets 0 (lse -inf); rows outside every sequence stay as
     they are.  ``max_k``: an upper bound of k_len where the key rows are many more (a cache's positions).  Returns elapsed ms."""
-    dtype = q.dtype if isinstance(q, torch.Tensor) else None
-    if dtype != torch.float16 and dtype != torch.bfloat16:
-        _refuse("q must be an fp16 or bf16 tensor")
-    device = q.device
-    st = PromptStrides(*_rows_ok(q, "q", dtype, device), *_rows_ok(k, "k", dtype, device), *_rows_ok(v, "v", dtype, device),
-                       *_rows_ok(out, "out", dtype, device))
-    (tq, heads, hd), (tk, kv_heads, k_hd) = q.shape, k.shape
-    if out.shape != q.shape:
-        _refuse("out.shape == q.shape")
-    if v.shape != k.shape or k_hd != hd:
-        _refuse("v.shape == k.shape, k.size(2) == q.size(2)")
-    if hd not in (32, 64, 128, 256):
-        _refuse("the head dimension must be 32, 64, 128 or 256")
-    if kv_heads < 1 or heads < 1 or heads % kv_heads:
-        _refuse("heads must be a multiple of kv_heads")
-    seqs, qs_ptr, ks_ptr, kl_ptr, lse_ptr = 1, None, None, None, None
-    if q_start is not None:
-        seqs = q_start.numel() - 1 if isinstance(q_start, torch.Tensor) else 0
-        if seqs < 1:
-            _refuse("q_start must hold at least two entries")
-        qs_ptr = _vector_ok(q_start, "q_start", torch.int32, seqs + 1, device)
-    if (k_start is None) != (k_len is None):
-        _refuse("k_start and k_len go together")
-    if k_start is not None:
-        ks_ptr = _vector_ok(k_start, "k_start", torch.int32, seqs, device)
-        kl_ptr = _vector_ok(k_len, "k_len", torch.int32, seqs, device)
-    elif q_start is not None and tk != tq:
-        _refuse("without k_start the keys lie as the queries do: k.size(0) == q.size(0)")
-    if lse is not None:
-        _check_input(lse, "lse")
-        if lse.dtype != torch.float32 or lse.shape != (tq, heads):
-            _refuse("lse must be float32 [Tq, heads]")
-        if lse.device != device:
-            _refuse("all tensors must be on the same device")
-        lse_ptr = lse.data_ptr()
-    if tq == 0:
-        return 0.0
-    lib = library()
-    sizes = (seqs, tq, tk, tk if max_k is None else int(max_k), heads, kv_heads, hd)
-    ws, need = _workspace(device, lib.rptc_attn_prompt_workspace_bytes, *sizes)
-    return _run_on(device, timed, lib.rptc_attn_prompt, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse_ptr, qs_ptr, ks_ptr,
-                   kl_ptr, *sizes, ctypes.byref(st), hd ** -0.5 if scale is None else float(scale), 1 if causal else 0, _DTYPES[dtype],
-                   None if ws is None else ws.data_ptr(), need)
+    return (_bindings or _load_bindings()).attn_prompt(q, k, v, out, q_start, k_start, k_len, causal, scale, lse, max_k,
+                                                       _timing if timed is None else timed)
 
 
 def kv4_row_bytes(hd):
     """Bytes of a row (one position of one head) of the 4-bit cache: hd / 2 of codes and a scale and a minimum for every 32 values."""
     if hd not in (32, 64, 128, 256):
-        _refuse("the head dimension must be 32, 64, 128 or 256")
+        raise RuntimeError("the head dimension must be 32, 64, 128 or 256")
     return hd // 2 + hd // 8
 
 
@@ -961,65 +870,18 @@ def kv4_cache(seqs, kv_heads, max_len, hd, device="cuda"):
     return torch.zeros(shape, dtype=torch.uint8, device=device), torch.zeros(shape, dtype=torch.uint8, device=device)
 
 
-def _kv4_ok(k_cache, v_cache, hd):
-    """(sequences, key heads, positions) of a pair of 4-bit caches."""
-    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        _check_input(t, name)
-        if t.dtype != torch.uint8 or t.dim() != 4:
-            _refuse(f"{name} must be uint8 [seqs, kv_heads, positions, row bytes]")
-    if k_cache.shape != v_cache.shape or k_cache.device != v_cache.device:
-        _refuse("k_cache and v_cache must be alike")
-    seqs, kv_heads, max_len, row = k_cache.shape
-    if row != kv4_row_bytes(hd):
-        _refuse("the cache's rows must have kv4_row_bytes(head dimension) bytes")
-    return seqs, kv_heads, max_len
-
-
-def _kv4_rows(k, v, k_cache, v_cache):
-    if not isinstance(k, torch.Tensor) or k.dim() != 3:
-        _refuse("k must be [tokens, kv_heads, head_dim]")
-    total, heads, hd = k.shape
-    seqs, kv_heads, max_len = _kv4_ok(k_cache, v_cache, hd)
-    device = k_cache.device
-    strides = *_rows_ok(k, "k", torch.float16, device), *_rows_ok(v, "v", torch.float16, device)
-    if v.shape != k.shape:
-        _refuse("v.shape == k.shape")
-    if heads != kv_heads:
-        _refuse("the cache must have as many heads as k and v")
-    return device, (seqs, total, kv_heads, hd, max_len), strides
-
-
 def kv4_append(k, v, k_cache, v_cache, pos, q_start=None, timed=None):
     """Put the rows k, v (fp16 [tokens, kv_heads, hd], strides as in ``attn_prompt``) into the 4-bit caches of
     ``kv4_cache``: sequence s's rows q_start[s] .. q_start[s+1] go to positions pos[s], pos[s] + 1, ... of cache s (int32 and
     int64 tensors on the device; without q_start every sequence has tokens / seqs rows).  Rows that do not fit are
     not written.  Returns elapsed ms."""
-    device, sizes, strides = _kv4_rows(k, v, k_cache, v_cache)
-    seqs, total, _, _, max_len = sizes
-    pos_ptr = _vector_ok(pos, "pos", torch.int64, seqs, device)
-    qs_ptr = None
-    if q_start is not None:
-        qs_ptr = _vector_ok(q_start, "q_start", torch.int32, seqs + 1, device)
-    elif seqs < 1 or total % seqs:
-        _refuse("without q_start the rows must divide evenly: k.size(0) % k_cache.size(0) == 0")
-    if total == 0 or max_len == 0:
-        return 0.0
-    return _run_on(device, timed, library().rptc_kv4_append, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pos_ptr,
-                   qs_ptr, *sizes, *strides)
+    return (_bindings or _load_bindings()).kv4_append(k, v, k_cache, v_cache, pos, q_start, _timing if timed is None else timed)
 
 
 def kv4_read(k_cache, v_cache, k, v, timed=None):
     """The first positions of every sequence of the 4-bit caches as fp16: k, v [seqs * rows, kv_heads, hd] (strides as in
     ``attn_prompt``) receive positions 0 .. rows-1, sequence after sequence.  Returns elapsed ms."""
-    device, (seqs, total, kv_heads, hd, max_len), strides = _kv4_rows(k, v, k_cache, v_cache)
-    if seqs < 1 or total % seqs or total // seqs > max_len:
-        _refuse("k must hold the same number of rows for every sequence, at most the cache's positions")
-    if total == 0:
-        return 0.0
-    if 0 in strides:
-        _refuse("k and v must not repeat elements")
-    return _run_on(device, timed, library().rptc_kv4_read, k_cache.data_ptr(), v_cache.data_ptr(), k.data_ptr(), v.data_ptr(), seqs,
-                   total // seqs, kv_heads, hd, max_len, *strides)
+    return (_bindings or _load_bindings()).kv4_read(k_cache, v_cache, k, v, _timing if timed is None else timed)
 
 
 def kv4_rope_append(qkv, cos, sin, pos, q_out, k_cache, v_cache, timed=None):
@@ -1027,28 +889,8 @@ def kv4_rope_append(qkv, cos, sin, pos, q_out, k_cache, v_cache, timed=None):
     [seqs, (heads + 2 kv_heads) * hd]) by cos/sin (fp16 [positions, hd/2]) at pos (int64 [seqs]), write q to q_out (fp16
     [seqs, heads, hd]) and append k and v at pos.  A sequence whose position lies outside the cache is skipped.  Returns
     elapsed ms."""
-    for t, name in ((qkv, "qkv"), (cos, "cos"), (sin, "sin"), (q_out, "q_out")):
-        _check_input(t, name)
-        if t.dtype != torch.float16:
-            _refuse(f"{name} must be fp16")
-    if q_out.dim() != 3 or qkv.dim() != 2:
-        _refuse("q_out must be [seqs, heads, head_dim], qkv [seqs, (heads + 2 kv_heads) * head_dim]")
-    seqs, heads, hd = q_out.shape
-    n, kv_heads, max_len = _kv4_ok(k_cache, v_cache, hd)
-    device = k_cache.device
-    if n != seqs or qkv.shape != (seqs, (heads + 2 * kv_heads) * hd):
-        _refuse("qkv must be [seqs, (heads + 2 kv_heads) * head_dim], the caches hold as many sequences")
-    if kv_heads < 1 or heads < 1 or heads % kv_heads:
-        _refuse("heads must be a multiple of kv_heads")
-    if cos.shape != sin.shape or cos.dim() != 2 or cos.size(0) < max_len or cos.size(1) != hd // 2:
-        _refuse("cos and sin must be [positions, head_dim / 2] with as many positions as the cache")
-    pos_ptr = _vector_ok(pos, "pos", torch.int64, seqs, device)
-    if not (qkv.device == cos.device == sin.device == q_out.device == device):
-        _refuse("all tensors must be on the same device")
-    if seqs == 0 or max_len == 0:
-        return 0.0
-    return _run_on(device, timed, library().rptc_kv4_rope_append, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), pos_ptr, q_out.data_ptr(),
-                   k_cache.data_ptr(), v_cache.data_ptr(), seqs, heads, kv_heads, hd, max_len)
+    return (_bindings or _load_bindings()).kv4_rope_append(qkv, cos, sin, pos, q_out, k_cache, v_cache,
+                                                           _timing if timed is None else timed)
 
 
 def kv4_attn_decode(q, k_cache, v_cache, pos, out, scale=None, timed=None):
@@ -1056,29 +898,7 @@ def kv4_attn_decode(q, k_cache, v_cache, pos, out, scale=None, timed=None):
     0 .. pos[s] of cache s.  q, out fp16 [seqs, heads, hd] (q's sequences may be any multiple of 8 elements apart), head h
     reading key head h // (heads // kv_heads); pos int64 [seqs] on the device.  A sequence whose pos lies outside the cache
     (a padded batch: -1) keeps what ``out`` holds.  ``scale`` defaults to hd ** -0.5.  Returns elapsed ms."""
-    if not isinstance(q, torch.Tensor) or q.dim() != 3:
-        _refuse("q must be [seqs, heads, head_dim]")
-    seqs, heads, hd = q.shape
-    n, kv_heads, max_len = _kv4_ok(k_cache, v_cache, hd)
-    device = k_cache.device
-    token, head = _rows_ok(q, "q", torch.float16, device)
-    if heads > 1 and head != hd:
-        _refuse("q must have contiguous heads")
-    _check_input(out, "out")
-    if out.dtype != torch.float16 or out.shape != q.shape or out.device != device:
-        _refuse("out must be fp16, of the shape of q and on its device")
-    if n != seqs:
-        _refuse("k_cache.size(0) == q.size(0)")
-    if kv_heads < 1 or heads < 1 or heads % kv_heads:
-        _refuse("heads must be a multiple of kv_heads")
-    pos_ptr = _vector_ok(pos, "pos", torch.int64, seqs, device)
-    if seqs == 0 or max_len == 0:
-        return 0.0
-    lib = library()
-    ws, need = _workspace(device, lib.rptc_kv4_attn_decode_workspace_bytes, seqs, heads, kv_heads, hd, max_len)
-    return _run_on(device, timed, lib.rptc_kv4_attn_decode, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pos_ptr, out.data_ptr(),
-                   seqs, heads, kv_heads, hd, max_len, token, hd ** -0.5 if scale is None else float(scale),
-                   None if ws is None else ws.data_ptr(), need)
+    return (_bindings or _load_bindings()).kv4_attn_decode(q, k_cache, v_cache, pos, out, scale, _timing if timed is None else timed)
 
 
 def token_logprobs(logits, tokens=None, logprob=None, entropy=None, top_ids=None, top_logprobs=None, timed=None):
@@ -1088,41 +908,5 @@ def token_logprobs(logits, tokens=None, logprob=None, entropy=None, top_ids=None
     entropy (float32 [rows]): of every row, in nats; top_ids (int64 [rows, k]) and top_logprobs (float32 [rows, k]): the k largest
     logits in falling order, equal ones by the lowest id, k at most 64.  Each output is optional.  A row that holds +inf or a
     not-a-number, or nothing but -inf, gives not-a-number.  Returns elapsed ms."""
-    if not isinstance(logits, torch.Tensor):
-        _refuse("logits must be a torch.Tensor")
-    if not logits.is_cuda:
-        _refuse("logits must be a CUDA tensor")
-    if logits.dim() != 2 or logits.dtype not in _DTYPES:
-        _refuse("logits must be fp16, bf16 or float32 [rows, vocab]")
-    rows, vocab = logits.shape
-    row_stride, step = logits.stride()
-    if vocab < 1:
-        _refuse("the vocabulary must not be empty")
-    if vocab > 1 and step != 1:
-        _refuse("logits must be contiguous along the vocabulary")
-    if logprob is None and entropy is None and top_ids is None and top_logprobs is None:
-        _refuse("at least one output is needed")
-    if logprob is not None and tokens is None:
-        _refuse("logprob needs tokens")
-    device = logits.device
-    tok_ptr = None if tokens is None else _vector_ok(tokens, "tokens", torch.int64, rows, device)
-    lp_ptr = None if logprob is None else _vector_ok(logprob, "logprob", torch.float32, rows, device)
-    ent_ptr = None if entropy is None else _vector_ok(entropy, "entropy", torch.float32, rows, device)
-    top = 0
-    for t, name, dtype in ((top_ids, "top_ids", torch.int64), (top_logprobs, "top_logprobs", torch.float32)):
-        if t is not None:
-            _check_input(t, name)
-            if t.dtype != dtype or t.dim() != 2 or t.size(0) != rows:
-                _refuse(f"{name} must be {str(dtype)[6:]} [rows, k]")
-            if t.device != device:
-                _refuse("all tensors must be on the same device")
-            if top not in (0, t.size(1)):
-                _refuse("top_ids and top_logprobs must have the same shape")
-            top = t.size(1)
-            if not 1 <= top <= min(64, vocab):
-                _refuse("1 <= k <= 64, k <= vocabulary")
-    if rows == 0:
-        return 0.0
-    return _run_on(device, timed, library().rptc_token_logprobs, logits.data_ptr(), _DTYPES[logits.dtype], tok_ptr, lp_ptr, ent_ptr,
-                   None if top_ids is None else top_ids.data_ptr(), None if top_logprobs is None else top_logprobs.data_ptr(), rows, vocab,
-                   row_stride if rows > 1 else vocab, top)
+    return (_bindings or _load_bindings()).token_logprobs(logits, tokens, logprob, entropy, top_ids, top_logprobs,
+                                                          _timing if timed is None else timed)
