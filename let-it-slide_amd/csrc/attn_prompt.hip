@@ -698,7 +698,7 @@ static int64_t prompt_tiles(int64_t seqs, int64_t total_q, int64_t rows) { retur
 
 // Which form, by the workgroups that 128 rows each would make for every compute unit (w) and the steps of 64 keys of the longest walk (s).
 // 128 rows read K and V least often and win where they fill the places of the compute units (3 a unit up to hd 64, 2 at 128, 1 at 256);
-// measured 128 / 64 rows, us: hd 128 w 1.5 37.2 / 36.8, w 2 52.2 / 55.9, w 3 91.8 / 107.7, w 8 520 / 609; hd 64 w 2 60.3 / 51.6, w 3
+// measured 128 / 64 rows, us: hd 128 w 1.5 37.2 / 36.8, w 1.8 (packed) 51.1 / 44.5, w 2 52.2 / 55.9, w 3 91.8 / 107.7, w 8 520 / 609; hd 64 w 2 60.3 / 51.6, w 3
 // 56.5 / 56.5, w 5 31.6 / 35.2; hd 256 w 1 104.7 / 88.5, w 1.5 143 / 175.  Below that the longest walk decides, and the two other
 // forms by the estimates that fit the measurements: 64 rows take h0 + h1 a step, more where compute units have several; the
 // narrow form, whose four waves share a walk but fetch four times the K and V a row, n0 + 2 n1 a step for its first round of
@@ -710,7 +710,7 @@ static int64_t prompt_tiles(int64_t seqs, int64_t total_q, int64_t rows) { retur
 static PromptPlan prompt_plan(int64_t seqs, int64_t total_q, int64_t heads, int64_t hd, int64_t max_k, int cus)
 {
     struct Form { double full, h0, h1, share0, share1, n0, n1; int places; };
-    static const Form forms[3] = {{3.00, 5.5, 0.47, 0.50, 0.50, 6, 0.17, 2}, {1.75, 6, 0.75, 0.45, 0.90, 8, 0.20, 1}, {1.00, 7, 2.10, 0, 1, 14, 0.35, 1}};
+    static const Form forms[3] = {{3.00, 5.5, 0.47, 0.50, 0.50, 6, 0.17, 2}, {1.85, 6, 0.75, 0.45, 0.90, 8, 0.20, 1}, {1.00, 7, 2.10, 0, 1, 14, 0.35, 1}};
     const Form &f = forms[hd <= 64 ? 0 : hd == 128 ? 1 : 2];
     PromptPlan p = {kWideRows, (int)prompt_tiles(seqs, total_q, kWideRows), 1};
     const double w = (double)p.tiles * heads / cus, s = (double)(max_k + 63) / 64;
