@@ -294,3 +294,26 @@ def test_the_same_bits_on_another_stream_and_in_two_graphs(rk):
         assert torch.equal(outs[0], out) and torch.equal(outs[1], out)
         pos.add_(1)
         rk.kv4_attn_decode(q, kc, vc, pos, out, timed=False)
+
+
+@pytest.mark.parametrize("lens", [[1, 77, 4091, 2000, 513, 2048, 3001, 333, 1024, 3777, 2500, 1666], [4096] * 3 + [5] * 9, [4096, 0, 2049], [600] * 31])
+def test_batches_of_unequal_sequences_are_cut_and_joined(rk, lens):
+    """The cut is worked out on the device from all lengths together: every sequence comes out as it does alone, within two roundings
+    of an output (its pieces, and with them the order of its sums, are others)."""
+    heads, kvh, hd, max_len = 8, 2, 64, 4096
+    n = len(lens)
+    kc, vc = rk.kv4_cache(n, kvh, max_len, hd)
+    x = randn(5, n * max_len, kvh, hd)
+    rk.kv4_append(x, randn(6, n * max_len, kvh, hd), kc, vc, torch.zeros(n, dtype=torch.int64, device="cuda"))
+    q = randn(7, n, heads, hd)
+    pos = torch.tensor(lens, device="cuda") - 1
+    out = torch.full((n, heads, hd), 7.0, dtype=torch.float16, device="cuda")
+    rk.kv4_attn_decode(q, kc, vc, pos, out)
+    for i in range(n):
+        if lens[i] == 0:
+            assert bool((out[i] == 7).all())
+            continue
+        alone = torch.empty((1, heads, hd), dtype=torch.float16, device="cuda")
+        rk.kv4_attn_decode(q[i:i + 1], kc[i:i + 1], vc[i:i + 1], pos[i:i + 1], alone)
+        # fp16's step at the output's size, and of sums whose weights (two fp16 terms) and products are rounded at 2^-21 of |v| <= 5
+        assert bool(((out[i].double() - alone[0].double()).abs() <= 2.0 ** -10 * alone[0].double().abs() + 2.0 ** -18).all())
