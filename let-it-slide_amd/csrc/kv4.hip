@@ -299,8 +299,9 @@ __device__ __forceinline__ bool kv4_find(const Kv4AttnArgs &a, int slot, bool by
         const uint32_t want = (uint32_t)a.want;
         for (int u = 0; u < 4; u++) {
             const uint32_t count = (uint32_t)__builtin_amdgcn_readlane((int)scan64(((uint32_t)(len + kKv4Tile - 1) / kKv4Tile + size - 1) / size), 63);
-            if (count <= want) break;
-            size = size / want * count + (size % want * count + want - 1) / want;            // size count / want, rounded up, in 32 bits
+            if (count <= want || size >= total / 2) break;
+            // size count / want, rounded up: in 32 bits, as size < 2^26 and count <= want + 63
+            size = min(total, size / want * count + (size % want * count + want - 1) / want);
         }
     }
     uint32_t in_front = 0;

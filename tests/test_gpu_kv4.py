@@ -317,3 +317,30 @@ def test_batches_of_unequal_sequences_are_cut_and_joined(rk, lens):
         rk.kv4_attn_decode(q[i:i + 1], kc[i:i + 1], vc[i:i + 1], pos[i:i + 1], alone)
         # fp16's step at the output's size, and of sums whose weights (two fp16 terms) and products are rounded at 2^-21 of |v| <= 5
         assert bool(((out[i].double() - alone[0].double()).abs() <= 2.0 ** -10 * alone[0].double().abs() + 2.0 ** -18).all())
+
+
+def test_more_sequences_than_pieces_wanted(rk):
+    # 7 sequences of 128 key heads: more workgroups than compute units from the sequences alone, of a cache long enough to be cut
+    seqs, kvh, hd, max_len = 7, 128, 32, 8192
+    kc, vc = rk.kv4_cache(seqs, kvh, max_len, hd)
+    lens = [8192, 8000, 1, 7000, 0, 8191, 8192]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for c in (kc, vc):
+        c[..., :hd // 2] = torch.randint(0, 256, c[..., :hd // 2].shape, generator=g, device="cuda", dtype=torch.uint8)
+        c[..., hd // 2:] = torch.tensor([0.2, -1.5], dtype=torch.float16, device="cuda").view(torch.uint8)
+    q, pos = randn(4, seqs, kvh, hd), torch.tensor(lens, device="cuda") - 1
+    out = torch.full((seqs, kvh, hd), 7.0, dtype=torch.float16, device="cuda")
+    rk.kv4_attn_decode(q, kc, vc, pos, out)
+    for i, n in enumerate(lens):
+        if n == 0:
+            assert bool((out[i] == 7).all())
+            continue
+        k, v = (torch.empty((max_len, kvh, hd), dtype=torch.float16, device="cuda") for _ in range(2))
+        rk.kv4_read(kc[i:i + 1], vc[i:i + 1], k, v)
+        kd, vd = k[:n].double(), v[:n].double()
+        s = torch.matmul(kd.transpose(0, 1), q[i].double()[:, :, None])[..., 0] * hd ** -0.5
+        p = torch.softmax(s, -1)
+        o, A = torch.matmul(p[:, None], vd.transpose(0, 1).contiguous())[:, 0], torch.matmul(p[:, None], vd.abs().transpose(0, 1).contiguous())[:, 0]
+        E = hd ** -0.5 * (hd + 4) * 2.0 ** -24 * torch.matmul(kd.abs().transpose(0, 1), q[i].double().abs()[:, :, None]).amax(1)
+        tol = 2.0 ** -11 * o.abs() + (2.0 ** -11 + 3 * E) * A + n * 2.0 ** -25 * vd.abs().amax() + 2.0 ** -25
+        assert bool(((out[i].double() - o).abs() <= tol).all())
