@@ -30,6 +30,9 @@ the reference's factorisation, quantize_hf.py:167, applied inside the kernel),
 ``sign_hadamard``, ``viterbi_pairs`` and ``viterbi_scalar`` (the quantizer's trellis search, rptc.py:13-71,
 as kernels: for the hashed pair stream and for the reference's own scalar trellis), ``lite_dequantize`` and
 ``lite_quantize`` (rptc_lite.py's decoder and search).
+Around the products of a decode loop: ``attn_prompt`` (attention of whole and packed prompts), ``kv4_cache`` / ``kv4_append`` /
+``kv4_read`` / ``kv4_rope_append`` / ``kv4_attn_decode`` (a key/value cache in 4 bits and the attention that reads it) and
+``token_logprobs`` (log probabilities, entropy and most likely tokens from logits).
 Sub-modules: ``packing`` (symbols -> streams), ``quantize`` (the quantizer around that search),
 ``linear`` (``QuantizedLinear``, ``patch_model``), ``llama_decode`` (a Llama-shaped decode loop),
 ``eval_ppl`` (perplexity on a token file).
