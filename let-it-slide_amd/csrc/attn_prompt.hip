@@ -734,7 +734,7 @@ static int prompt_sizes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t 
 {
     if (seqs < 1 || total_q < 1 || total_k < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0) return RPTC_ESHAPE;
     if (hd != 32 && hd != 64 && hd != 128 && hd != 256) return RPTC_ESHAPE;
-    if (heads > 1024 || seqs > (1 << 20) || total_q > (1 << 24) || total_k >= ((int64_t)1 << 31) - 64) return RPTC_ELIMIT;
+    if (heads > 1024 || seqs > (1 << 20) || total_q > (1 << 24) || total_k >= ((int64_t)1 << 31) - 1024) return RPTC_ELIMIT;
     if (prompt_tiles(seqs, total_q, kNarrowRows) * heads >= (int64_t)1 << 23) return RPTC_ELIMIT;      // workgroups of one launch
     return 0;
 }

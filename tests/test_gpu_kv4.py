@@ -344,3 +344,22 @@ def test_more_sequences_than_pieces_wanted(rk):
         E = hd ** -0.5 * (hd + 4) * 2.0 ** -24 * torch.matmul(kd.abs().transpose(0, 1), q[i].double().abs()[:, :, None]).amax(1)
         tol = 2.0 ** -11 * o.abs() + (2.0 ** -11 + 3 * E) * A + n * 2.0 ** -25 * vd.abs().amax() + 2.0 ** -25
         assert bool(((out[i].double() - o).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("hd", [32, 128])
+def test_codes_beside_the_middle_between_two(rk, hd):
+    # groups whose values lie on, and one fp16 step beside, the middles between two codes: the rounded quotient decides
+    g = np.random.default_rng(5)
+    n = 4096
+    lo = g.normal(0, 1, (n, hd // 32, 1)).astype(np.float16).astype(np.float32)
+    s = (2.0 ** g.integers(-12, 3, (n, hd // 32, 1))).astype(np.float32) * g.choice([1.0, 1.25, 1.5, 1.0 + 2.0 ** -10], (n, hd // 32, 1)).astype(np.float32)
+    x = (lo + s * (g.integers(0, 15, (n, hd // 32, 32)) + 0.5)).astype(np.float16)
+    step = g.integers(-1, 2, x.shape)
+    x = np.where(step == 0, x, np.nextafter(x, np.where(step > 0, np.float16(np.inf), np.float16(-np.inf)))).astype(np.float16)
+    x[..., 0], x[..., 1] = lo[..., 0].astype(np.float16), (lo + 15 * s)[..., 0].astype(np.float16)
+    rows = np.ascontiguousarray(x.reshape(n, 1, hd))
+    kc, vc = rk.kv4_cache(1, 1, n, hd)
+    t = torch.from_numpy(rows).cuda()
+    rk.kv4_append(t, t, kc, vc, torch.zeros(1, dtype=torch.int64, device="cuda"))
+    want = rows_of(rows.transpose(1, 0, 2))
+    assert np.array_equal(kc[0].cpu().numpy(), want) and np.array_equal(vc[0].cpu().numpy(), want)
