@@ -169,3 +169,94 @@ def test_scores_of_packed_texts(rk):
                     for w in windows.view(3, 64))
     assert n == n_c == 3 and abs(loss - loss_c) <= 2 * apart + 1e-4 and apart < 0.1
     assert ppl == math.exp(loss)
+
+
+def test_two_threads_on_two_streams_at_once(rk):
+    """Calls that overlap have a workspace each: split attention, cut decode attention and scores from two threads, every result the
+    bits that the call gives alone."""
+    import threading
+    g = torch.Generator(device="cuda").manual_seed(9)
+    rand = lambda *shape: torch.randn(shape, generator=g, device="cuda").half()
+    jobs = []
+    for n, past in ((7, 2500), (30, 4000)):
+        q, k, v = rand(n, 4, 64), rand(past, 2, 64), rand(past, 2, 64)
+        jobs.append((lambda out, q=q, k=k, v=v: rk.attn_prompt(q, k, v, out, timed=False), q.shape, torch.float16))
+    for lens in ((3000, 17), (4096, 2222)):
+        kc, vc = rk.kv4_cache(2, 2, 4096, 64)
+        rk.kv4_append(rand(2 * 4096, 2, 64), rand(2 * 4096, 2, 64), kc, vc, torch.zeros(2, dtype=torch.int64, device="cuda"), timed=False)
+        q, pos = rand(2, 8, 64), torch.tensor(lens, device="cuda") - 1
+        jobs.append((lambda out, q=q, kc=kc, vc=vc, pos=pos: rk.kv4_attn_decode(q, kc, vc, pos, out, timed=False), q.shape, torch.float16))
+    for rows in (3, 200):
+        x, tok = rand(rows, 5000), torch.arange(rows, device="cuda")
+        jobs.append((lambda out, x=x, tok=tok: rk.token_logprobs(x, tok, out, timed=False), (rows,), torch.float32))
+    alone = []
+    for call, shape, dtype in jobs:
+        out = torch.empty(shape, dtype=dtype, device="cuda")
+        call(out)
+        alone.append(out)
+    torch.cuda.synchronize()
+    outs = [[[torch.empty(s, dtype=d, device="cuda") for _, s, d in jobs] for _ in range(20)] for _ in range(2)]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(mine, order):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for run in mine:
+                    for i in order:
+                        jobs[i][0](run[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                      # handed to the test's own thread
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(outs[t], range(len(jobs)) if t == 0 else range(len(jobs) - 1, -1, -1))) for t in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for mine in outs:
+        for run in mine:
+            for got, want in zip(run, alone):
+                assert torch.equal(got, want)
+
+
+def test_refusals_leave_the_outputs(rk):
+    """What the entry points refuse of tensors on the device, with the outputs as they were."""
+    z = lambda *shape, dtype=torch.float16: torch.zeros(shape, dtype=dtype, device="cuda")
+    q, k, out = z(4, 4, 64), z(4, 2, 64), torch.full((4, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+    i32 = lambda *xs: torch.tensor(xs, dtype=torch.int32, device="cuda")
+    for call in (lambda: rk.attn_prompt(q, k, k, out[:3]), lambda: rk.attn_prompt(q, k, z(4, 4, 64), out), lambda: rk.attn_prompt(q, z(4, 3, 64), z(4, 3, 64), out),
+                 lambda: rk.attn_prompt(q.float(), k, k, out), lambda: rk.attn_prompt(q, k.bfloat16(), k, out), lambda: rk.attn_prompt(z(4, 4, 48), z(4, 2, 48), z(4, 2, 48), z(4, 4, 48)),
+                 lambda: rk.attn_prompt(q, k, k, q), lambda: rk.attn_prompt(q, k, k, out, q_start=i32(0)), lambda: rk.attn_prompt(q, k, k, out, k_start=i32(0)),
+                 lambda: rk.attn_prompt(q, k, k, out, q_start=i32(0, 4).long()), lambda: rk.attn_prompt(q, z(5, 2, 64), z(5, 2, 64), out, q_start=i32(0, 4)),
+                 lambda: rk.attn_prompt(q, k, k, out, lse=z(4, 4)), lambda: rk.attn_prompt(q, k, k, out, scale=0), lambda: rk.attn_prompt(q, k, k, out, max_k=-1),
+                 lambda: rk.attn_prompt(q, k, k, out.transpose(1, 2)), lambda: rk.attn_prompt(z(4, 4, 72)[..., 4:68], k, k, out),
+                 lambda: rk.attn_prompt(q, k, k, z(1, 4, 64).expand(4, 4, 64)), lambda: rk.attn_prompt(None, k, k, out)):
+        with pytest.raises(RuntimeError):
+            call()
+    kc, vc = rk.kv4_cache(1, 2, 16, 64)
+    pos = torch.zeros(1, dtype=torch.int64, device="cuda")
+    for call in (lambda: rk.kv4_append(k, k[:2], kc, vc, pos), lambda: rk.kv4_append(k, k, kc, vc, pos.int()), lambda: rk.kv4_append(k, k, kc, kc, pos),
+                 lambda: rk.kv4_append(z(4, 3, 64), z(4, 3, 64), kc, vc, pos), lambda: rk.kv4_append(k, k, kc[..., :20], vc[..., :20], pos),
+                 lambda: rk.kv4_read(kc, vc, z(17, 2, 64), z(17, 2, 64)), lambda: rk.kv4_read(kc, vc, z(1, 2, 64).expand(4, 2, 64), z(4, 2, 64)),
+                 lambda: rk.kv4_attn_decode(z(2, 4, 64), kc, vc, pos, z(2, 4, 64)), lambda: rk.kv4_attn_decode(z(1, 3, 64), kc, vc, pos, z(1, 3, 64)),
+                 lambda: rk.kv4_attn_decode(q[:1], kc, vc, pos, out[:1], scale=-1.0), lambda: rk.kv4_attn_decode(q[:1], kc, vc, pos, q[:1]),
+                 lambda: rk.kv4_rope_append(z(1, 512), z(15, 32), z(15, 32), pos, z(1, 4, 64), kc, vc), lambda: rk.kv4_rope_append(z(1, 500), z(16, 32), z(16, 32), pos, z(1, 4, 64), kc, vc)):
+        with pytest.raises(RuntimeError):
+            call()
+    x, lp = z(3, 100), torch.full((3,), 7.0, device="cuda")
+    tok = torch.zeros(3, dtype=torch.int64, device="cuda")
+    for call in (lambda: rk.token_logprobs(x), lambda: rk.token_logprobs(x, None, lp), lambda: rk.token_logprobs(x, tok[:2], lp), lambda: rk.token_logprobs(x, tok.int(), lp),
+                 lambda: rk.token_logprobs(x.t(), tok, lp), lambda: rk.token_logprobs(x, tok, z(3)), lambda: rk.token_logprobs(x.double(), tok, lp),
+                 lambda: rk.token_logprobs(x, top_ids=z(3, 65, dtype=torch.int64)), lambda: rk.token_logprobs(x, top_ids=z(3, 5, dtype=torch.int64), top_logprobs=z(3, 4, dtype=torch.float32)),
+                 lambda: rk.token_logprobs(x, top_ids=z(3, 0, dtype=torch.int64)), lambda: rk.token_logprobs(x.view(1, 3, 100), tok, lp)):
+        with pytest.raises(RuntimeError):
+            call()
+    torch.cuda.synchronize()
+    assert bool((out == 7).all()) and bool((lp == 7).all()) and not bool(kc.any()) and not bool(vc.any())
+    # empty calls are none
+    assert rk.attn_prompt(q[:0], k[:0], k[:0], out[:0]) == 0.0 and rk.token_logprobs(x[:0], tok[:0], lp[:0]) == 0.0
+    assert rk.kv4_append(k[:0], k[:0], kc, vc, pos) == 0.0 and rk.kv4_read(kc, vc, k[:0], k[:0]) == 0.0
+    # a prompt without keys
+    rk.attn_prompt(q, k[:0], k[:0], out, q_start=i32(0, 4), k_start=i32(0), k_len=i32(0))
+    assert not bool(out.any())
