@@ -182,3 +182,36 @@ def test_workspace_is_asked_for(rk):
     assert call(None, 0) == -1 and call(ws.data_ptr(), need - 1) == -2 and call(ws.data_ptr() + 4, need) == -3
     torch.cuda.synchronize()
     assert bool((out == 7).all())
+
+
+@pytest.mark.parametrize("rows,heads", [(9, 4), (512, 32), (1100, 128)])
+def test_keys_behind_four_gib(rk, rows, heads):
+    # few rows (keys split), rows whose walk counts, rows that fill the device: the keys at the end of buffers of more than 4 GiB
+    n, hd = 34_000_000, 64
+    k, v = (torch.empty((n, 1, hd), dtype=F16, device="cuda") for _ in range(2))
+    assert k.numel() * 2 > 1 << 32
+    L = rows + 700
+    k[n - L:], v[n - L:] = randn(2, L, 1, hd), randn(3, L, 1, hd)
+    q = randn(1, rows, heads, hd)
+    out, lse = torch.empty_like(q), torch.empty(rows, heads, device="cuda")
+    rk.attn_prompt(q, k, v, out, q_start=ints([0, rows]), k_start=ints([n - L]), k_len=ints([L]), lse=lse, max_k=L, timed=False)
+    for h in range(0, heads, max(1, heads // 4)):
+        check(out[:, h:h + 1], lse[:, h:h + 1], q[:, h:h + 1], k[n - L:], v[n - L:], True)
+
+
+def test_rows_behind_four_gib(rk):
+    n, heads, hd = 1 << 24, 2, 64
+    q = torch.empty((n, heads, hd), dtype=F16, device="cuda")
+    assert q.numel() * 2 >= 1 << 32
+    q[-300:] = randn(1, 300, heads, hd)
+    out = torch.full_like(q, 7.0)
+    k, v = randn(2, 50, 1, hd), randn(3, 50, 1, hd)
+    lse = torch.empty((n, heads), device="cuda")
+    # one sequence at the very end; then all rows as one sequence, not causal
+    rk.attn_prompt(q, k, v, out, q_start=ints([n - 300, n]), k_start=ints([0]), k_len=ints([50]), lse=lse, causal=False, timed=False)
+    check(out[-300:], lse[-300:], q[-300:], k, v, False)
+    assert bool((out[-301] == 7).all()) and bool((out[0] == 7).all())
+    q[:300] = q[-300:]
+    rk.attn_prompt(q, k, v, out, q_start=ints([0, n]), k_start=ints([0]), k_len=ints([50]), lse=lse, causal=False, timed=False)
+    check(out[:300], lse[:300], q[:300], k, v, False)
+    check(out[-300:], lse[-300:], q[-300:], k, v, False)

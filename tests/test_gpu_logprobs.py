@@ -157,3 +157,19 @@ def test_another_stream_and_a_graph(rk):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o[n], want[n]) for n in want)
+
+
+def test_rows_past_2_31_logits(rk):
+    rows, vocab = 17000, 128257
+    x = torch.empty((rows, vocab), dtype=BF16, device="cuda")
+    assert x.numel() > 1 << 31
+    g = torch.Generator(device="cuda").manual_seed(1)
+    part = (torch.randn((5, vocab), generator=g, device="cuda") * 2).bfloat16()
+    x.zero_()
+    x[:5], x[-5:] = part, part
+    lp, ids = torch.empty(rows, device="cuda"), torch.empty((rows, 3), dtype=torch.int64, device="cuda")
+    rk.token_logprobs(x, torch.arange(rows, device="cuda") % 5, lp, top_ids=ids, timed=False)
+    alone, alone_ids = torch.empty(5, device="cuda"), torch.empty((5, 3), dtype=torch.int64, device="cuda")
+    rk.token_logprobs(part, torch.arange(rows - 5, rows, device="cuda") % 5, alone, top_ids=alone_ids, timed=False)
+    assert torch.equal(lp[-5:], alone) and torch.equal(ids[-5:], alone_ids) and torch.equal(ids[:5], alone_ids)
+    assert torch.equal(ids[5:-5], torch.arange(3, device="cuda").expand(rows - 10, 3))       # all equal: the lowest ids
