@@ -215,3 +215,33 @@ def test_rows_behind_four_gib(rk):
     rk.attn_prompt(q, k, v, out, q_start=ints([0, n]), k_start=ints([0]), k_len=ints([50]), lse=lse, causal=False, timed=False)
     check(out[:300], lse[:300], q[:300], k, v, False)
     check(out[-300:], lse[-300:], q[-300:], k, v, False)
+
+
+@pytest.mark.parametrize("lens,hd", [([512], 128), ([400], 64), (MANY, 64), (MANY, 128), (MANY, 256)])
+def test_rows_that_are_no_numbers_beside_rows_that_only_lie_next_to_them(rk, lens, hd):
+    # a query of not-a-numbers, a key of them that half of the queries see, a value of them that the last one sees: every row
+    # by what it sees itself
+    q, k, v, want = run(rk, lens, lens, 32, 8, hd, F16, True)
+    starts = [0]
+    for n in lens:
+        starts.append(starts[-1] + n)
+        if n > 8:
+            q[starts[-2] + 3] = float("nan")
+            k[starts[-2] + n // 2] = float("nan")
+            v[starts[-1] - 1] = float("inf")
+    out = torch.empty_like(q)
+    rk.attn_prompt(q, k, v, out, q_start=ints(starts), k_start=ints(starts[:-1]), k_len=ints(lens), max_k=max(lens), timed=False)
+    for i, n in enumerate(lens):
+        rows = slice(starts[i], starts[i] + n)
+        bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+        if n > 8:
+            bad[3] = True
+            bad[n // 2:] = True
+        assert torch.equal(torch.isfinite(out[rows]).flatten(1).all(1), ~bad) and bool(torch.isnan(out[rows][bad]).all())
+        if n:
+            clean = [t[rows].clone() for t in (q, k, v)]
+            for t in clean:
+                t[~torch.isfinite(t)] = 0
+            tol = 2 * formula(*clean, True)[2][~bad] + 2.0 ** -20
+            err = (out[rows][~bad].double() - want[rows][~bad].double()).abs()
+            assert bool((err <= tol).all())
