@@ -349,7 +349,9 @@ struct PromptWave {
                 }
             }
     }
-    // whether a sum of the lane's row is infinite or not a number
+    // whether the sum of p of the lane's row is infinite or not a number
+    __device__ __forceinline__ bool odd_sum() const { return halves_max(l * 0.f != 0.f ? 1.f : 0.f) != 0.f; }
+    // whether another sum of it is
     __device__ __forceinline__ bool odd() const
     {
         float bad = 0.f;
@@ -439,7 +441,7 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
         if (k0 + kKeys < k_hi) request_v(k0 + kKeys, buf ^ 1);
         if (k0 + koff >= see_most) return;
         if (k0 + koff + kMine > see_least) {               // some row of the wave does not see all of its keys
-            if (!masked) before = halves_max(w.l * 0.f != 0.f ? 1.f : 0.f) != 0.f;
+            if (!masked) before = w.odd_sum();
             masked = true;
             w.mask(s, see - k0 - koff);
         }
@@ -461,6 +463,7 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
         }
     }
     bool odd = w.odd();
+    if (!masked) before = odd;                             // no key of the wave was masked
     float l = halves_sum(w.l);
     if (G == 2) {
         // sums of the second half's waves to the first's, a register of all lanes after the other
@@ -533,14 +536,13 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
     static_assert(kNarrowRows * kJoinRow * 4 <= 2 * kTile * 2, "a wave's sums fit where its K and V were");
     extern __shared__ __align__(16) uint16_t lds[];       // [wave][K, V][kStep][HD]
     __shared__ float s_ml[4][kNarrowRows][2];
-    __shared__ int s_odd;
+    __shared__ uint32_t s_odd[4], s_seen[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int c = lane >> 5, col = lane & 31;
     int head, tile, split;
     prompt_item(a, head, tile, split);
     PromptTile t;
     if (!find_tile<kNarrowRows>(a, tile, t)) return;
-    if (tid == 0) s_odd = 0;
     const int kvh = head / (a.heads / a.kv_heads);
     const int k_most = uniform(prompt_sees(a, t, min(t.row0 + kNarrowRows, t.q_end) - 1));
     const int per_split = ((k_most + a.splits - 1) / a.splits + kStep - 1) / kStep * kStep;
@@ -586,6 +588,7 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
     PromptWave<HD, T, kStep, 2> w;
     w.begin(a, t, row, head);
     w.settle();
+    bool masked = false, before = false;                   // as above
     for (; k0 < k_hi; k0 += kStride) {
         const bool more = k0 + kStride < k_hi;
         wait_for_lds_loads_but<kRequests>();               // K is there (V was asked for behind it)
@@ -593,7 +596,11 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
         w.scores(kt, s);
         wait_for_lds_reads();
         if (more) request_k(k0 + kStride);
-        if (k0 + kStep > see_least) w.mask(s, see - k0);
+        if (k0 + kStep > see_least) {
+            if (!masked) before = w.odd_sum();
+            masked = true;
+            w.mask(s, see - k0);
+        }
         const float off = w.bound(s, a.c);
         uint32_t p[2][kStep / 32][8];
         w.weights(s, a.c, off, p);
@@ -606,10 +613,14 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
 
     // the waves join: sums to where K and V were, row by row (four floats of padding where there is room: rows on different banks)
     float *mine = reinterpret_cast<float *>(kt);
-    const bool odd = __ballot(w.odd()) != 0;
+    const bool odd = w.odd();
+    if (!masked) before = odd;
     const float l = halves_sum(w.l);
-    __syncthreads();                                       // s_odd is cleared
-    if (odd && lane == 0) s_odd = 1;
+    const uint32_t odds = (uint32_t)__ballot(odd), seen = (uint32_t)__ballot(before);
+    if (lane == 0) {
+        s_odd[wave] = odds;
+        s_seen[wave] = seen;
+    }
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
 #pragma unroll
@@ -621,14 +632,12 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
         s_ml[wave][col][1] = l;
     }
     __syncthreads();
-    if (s_odd) {
-        prompt_rows_plain<HD, T>(a, t, t.row0 + 8 * wave, 0xFFu, head, kvh, k_lo, k_hi, split);
-        return;
-    }
+    const uint32_t redo = (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]) & ~(s_seen[0] | s_seen[1] | s_seen[2] | s_seen[3]);
     constexpr int kRowChunks = HD / 8;
     for (int i = tid; i < kNarrowRows * kRowChunks; i += kPromptThreads) {
         const int r = i / kRowChunks, d = i % kRowChunks * 8;
         if (t.row0 + r >= t.q_end) break;
+        if (redo >> r & 1) continue;
         const float M = fmaxf(fmaxf(s_ml[0][r][0], s_ml[1][r][0]), fmaxf(s_ml[2][r][0], s_ml[3][r][0]));
         float den = 0.f, num[8];
 #pragma unroll
@@ -656,6 +665,8 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
             make_uint4(T::pack(num[0] * inv, num[1] * inv), T::pack(num[2] * inv, num[3] * inv), T::pack(num[4] * inv, num[5] * inv), T::pack(num[6] * inv, num[7] * inv));
         if (a.lse && d == 0) a.lse[at] = den == 0.f ? -INFINITY : (M + log2f(den)) * 0.693147180559945f;
     }
+    const uint32_t which = uniform((int)(redo >> (8 * wave) & 0xFFu));
+    if (which) prompt_rows_plain<HD, T>(a, t, t.row0 + 8 * wave, which, head, kvh, k_lo, k_hi, split);
 }
 
 // Joins the pieces of a row, a workgroup per (row, head).  The rows are found as the kernel above found them: rows of no

@@ -245,3 +245,19 @@ def test_rows_that_are_no_numbers_beside_rows_that_only_lie_next_to_them(rk, len
             tol = 2 * formula(*clean, True)[2][~bad] + 2.0 ** -20
             err = (out[rows][~bad].double() - want[rows][~bad].double()).abs()
             assert bool((err <= tol).all())
+
+
+@pytest.mark.parametrize("n,hd", [(512, 128), (384, 64), (2560, 128)])
+def test_numbers_and_none_where_nothing_is_masked(rk, n, hd):
+    # every query sees every key: rows of a query of not-a-numbers, all others; then a key of them, which all see
+    q, k, v = randn(31, n, 32, hd), randn(32, n, 8, hd), randn(33, n, 8, hd)
+    out, again = torch.empty_like(q), torch.empty_like(q)
+    rk.attn_prompt(q, k, v, out, causal=False, timed=False)
+    q[7] = float("nan")
+    rk.attn_prompt(q, k, v, again, causal=False, timed=False)
+    assert bool(torch.isnan(again[7]).all())
+    others = [i for i in range(n) if i != 7]
+    assert torch.equal(again[others], out[others])
+    k[n - 1, 3] = float("nan")
+    rk.attn_prompt(q, k, v, again, causal=False, timed=False)
+    assert bool(torch.isnan(again[:, 12:16]).all()) and torch.equal(again[others][:, :12], out[others][:, :12])

@@ -260,3 +260,15 @@ def test_refusals_leave_the_outputs(rk):
     # a prompt without keys
     rk.attn_prompt(q, k[:0], k[:0], out, q_start=i32(0, 4), k_start=i32(0), k_len=i32(0))
     assert not bool(out.any())
+
+
+def test_the_command_scores_packed_windows(rk, capsys):
+    """``python -m rptc_kernels.eval_ppl --packed``: the windows and, to the accuracy of two fp16 paths, the loss of the command without it."""
+    import json
+    args = ["--layers", "1", "--d-model", "256", "--heads", "4", "--d-ff", "704", "--vocab", "500", "--seqlen", "48", "--windows", "5"]
+    lines = []
+    for extra in ([], ["--packed", "2"]):
+        eval_ppl.main(args + extra)
+        lines.append(json.loads(capsys.readouterr().out.strip().split("\n")[-1]))
+    assert lines[0]["windows"] == lines[1]["windows"] == 5
+    assert abs(lines[0]["avg_loss"] - lines[1]["avg_loss"]) < 1e-2 * lines[0]["avg_loss"]
