@@ -366,7 +366,7 @@ struct PromptWave {
 // Many rows: 128 query rows of a head a workgroup, 32 a wave (G = 1); all waves walk over the same keys, which are brought to
 // LDS once for the four of them, a step ahead.  G = 2: 64 query rows, two waves a row, one for the first and one for the second half of
 // a step's 64 keys, joined at the end: twice the workgroups with half the walk, where the longest walk is what the call waits
-// for (64 keys a wave and a step of 128 need twice the LDS: 1024 rows of 32 heads x 128 29.4 us instead of 21.6; G = 1 with
+// for; its keys may be cut into pieces as well (150 rows behind 8000, 32 / 8 heads x 128: 95 us whole, 46 in four) (64 keys a wave and a step of 128 need twice the LDS: 1024 rows of 32 heads x 128 29.4 us instead of 21.6; G = 1 with
 // 32 keys a step meets twice as often: 8192 rows 567 us instead of 520).
 template <int HD, int G>
 constexpr int kWaveKeys = G == 2 ? 32 : 64;    // keys of a step and wave
@@ -387,7 +387,14 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
     if (!find_tile<kRows>(a, tile, t)) return;
     const int kvh = head / (a.heads / a.kv_heads);
 
-    const int k_hi = uniform(prompt_sees(a, t, min(t.row0 + kRows, t.q_end) - 1));      // of the tile's last row: the most
+    const int k_most = uniform(prompt_sees(a, t, min(t.row0 + kRows, t.q_end) - 1));    // of the tile's last row: the most
+    // this workgroup's piece of them, whole steps
+    int k_lo = 0, k_hi = k_most;
+    if (G == 2 && a.splits > 1) {
+        const int per_split = ((k_most + a.splits - 1) / a.splits + kKeys - 1) / kKeys * kKeys;
+        k_lo = uniform((int)min((int64_t)k_most, (int64_t)split * per_split));
+        k_hi = uniform((int)min((int64_t)k_most, (int64_t)k_lo + per_split));
+    }
     const int group = G == 2 ? wave >> 1 : 0, koff = group * kMine;
     const int row_first = t.row0 + 32 * (wave & (4 / G - 1)), row = row_first + col;
     const bool wave_live = row_first < t.q_end;
@@ -421,10 +428,10 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
         for (int u = 0; u < kRequests; u++) load_to_lds(v_off[u], r, lds_base + (uint32_t)(2 + buf) * (2u * kTile) + u * 4096u);
     };
 
-    if (k_hi > 0) {
-        request_k(0, 0);
-        request_v(0, 0);
-        if (kKeys < k_hi) request_k(kKeys, 1);
+    if (k_lo < k_hi) {
+        request_k(k_lo, 0);
+        request_v(k_lo, 0);
+        if (k_lo + kKeys < k_hi) request_k(k_lo + kKeys, 1);
     }
     PromptWave<HD, T, kMine, 1> w;
     w.begin(a, t, row, head);
@@ -451,12 +458,12 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
         w.weights(s, a.c, off, p);
         w.product(lds + (2 + buf) * kTile + koff * HD, p);
     };
-    if (k_hi > 0) {
+    if (k_lo < k_hi) {
         float16_t sa[kMine / 32], sb[kMine / 32];
         wait_for_lds_loads();
         __syncthreads();
         w.scores(lds + koff * HD, sa);
-        for (int k0 = 0; k0 < k_hi; k0 += 2 * kKeys) {
+        for (int k0 = k_lo; k0 < k_hi; k0 += 2 * kKeys) {
             step(k0, 0, sa, sb);
             if (k0 + kKeys >= k_hi) break;
             step(k0 + kKeys, 1, sb, sa);
@@ -502,6 +509,21 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
     }
     if (!wave_live) return;
     const bool redo = odd && !before;
+    const uint32_t which = (uint32_t)__ballot(redo);
+    if (G == 2 && a.splits > 1) {
+        if (row < t.q_end && !redo) {
+            const int64_t pa = ((int64_t)row * a.heads + head) * a.splits + split;
+            float *part = a.part_acc + pa * HD + 4 * c;
+#pragma unroll
+            for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+                for (int b = 0; b < 4; b++)
+                    *reinterpret_cast<float4 *>(part + 32 * d + 8 * b) = make_float4(w.acc[d][4 * b], w.acc[d][4 * b + 1], w.acc[d][4 * b + 2], w.acc[d][4 * b + 3]);
+            if (c == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * pa) = make_float2(l == 0.f ? -INFINITY : w.m, l);
+        }
+        if (which) prompt_rows_plain<HD, T>(a, t, row_first, which, head, kvh, k_lo, k_hi, split);
+        return;
+    }
     const float inv = l == 0.f ? 0.f : 1.f / l;            // a row that sees nothing: zeros
     uint16_t *o = a.out + (int64_t)min(row, t.q_end - 1) * a.st.out_token + (int64_t)head * a.st.out_head + 8 * c;
 #pragma unroll
@@ -518,7 +540,6 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
                 *reinterpret_cast<uint4 *>(o + 32 * d + 8 * b) = make_uint4((uint32_t)w0[0], (uint32_t)w1[0], (uint32_t)w0[1], (uint32_t)w1[1]);
         }
     if (a.lse && c == 0 && row < t.q_end && !redo) a.lse[(int64_t)row * a.heads + head] = l == 0.f ? -INFINITY : (w.m + log2f(l)) * 0.693147180559945f;
-    const uint32_t which = (uint32_t)__ballot(redo);
     if (which) prompt_rows_plain<HD, T>(a, t, row_first, which, head, kvh, 0, k_hi, 0);
 }
 
@@ -669,7 +690,7 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
     if (which) prompt_rows_plain<HD, T>(a, t, t.row0 + 8 * wave, which, head, kvh, k_lo, k_hi, split);
 }
 
-// Joins the pieces of a row, a workgroup per (row, head).  The rows are found as the kernel above found them: rows of no
+// Joins the pieces of a row, a workgroup per (row, head), for more pieces than the kernel below takes.  The rows are found as the kernel above found them: rows of no
 // sequence have no pieces and stay as they are.
 template <int HD, class T>
 __global__ __launch_bounds__(kJoinThreads) void attn_prompt_merge_kernel(const PromptArgs a)
@@ -685,6 +706,66 @@ __global__ __launch_bounds__(kJoinThreads) void attn_prompt_merge_kernel(const P
     if (threadIdx.x < HD)
         a.out[(int64_t)row * a.st.out_token + (int64_t)head * a.st.out_head + threadIdx.x] = (uint16_t)T::pack(l == 0.f ? 0.f : num / l, 0.f);
     if (a.lse && threadIdx.x == 0) a.lse[at] = l == 0.f ? -INFINITY : (M + log2f(l)) * 0.693147180559945f;
+}
+
+// The same for at most kFewPieces pieces: a wave per (row, head), eight pieces asked for at once (2300 rows of 8 heads in two pieces: 6 us
+// where a workgroup a row took 28; a branch a piece in place of the clamped index: 45).
+constexpr int kFewPieces = 16;
+template <int HD, class T>
+__global__ __launch_bounds__(256) void attn_prompt_merge_few_kernel(const PromptArgs a)
+{
+    constexpr int kEach = HD / 64 < 1 ? 1 : HD / 64;       // dimensions of a lane (hd 32: the lanes from 32 on repeat the others)
+    typedef float vec __attribute__((ext_vector_type(kEach)));
+    const int lane = threadIdx.x & 63, head = blockIdx.y * 4 + uniform((int)threadIdx.x >> 6);
+    if (head >= a.heads) return;
+    PromptTile t;
+    if (!find_tile<kNarrowRows>(a, blockIdx.x / kNarrowRows, t)) return;
+    const int row = t.row0 + blockIdx.x % kNarrowRows;
+    if (row >= t.q_end) return;
+    const int64_t at = (int64_t)row * a.heads + head;
+    const int dim = kEach * lane % HD;
+    const float *acc = a.part_acc + at * a.splits * HD + dim;
+    vec v[8];
+    auto ask = [&](int i0) {                               // (a piece past the last: the last once more, with factor 0)
+#pragma unroll
+        for (int u = 0; u < 8; u++) v[u] = *reinterpret_cast<const vec *>(acc + min(i0 + u, a.splits - 1) * HD);
+    };
+    ask(0);
+    float m = -INFINITY, l = 0.f;
+    if (lane < a.splits) {
+        const float2 w = reinterpret_cast<const float2 *>(a.part_ml)[at * a.splits + lane];
+        m = w.x;
+        l = w.y;
+    }
+    float M = m;
+#pragma unroll
+    for (int off = kFewPieces / 2; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+    // a sum of 0 takes part in nothing (its sums are 0); a bound of -inf with a sum is a row of not-a-numbers
+    const float f = l == 0.f ? 0.f : m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - M);
+    vec num = (vec)(0.f);
+    float den = l * f;
+#pragma unroll
+    for (int off = kFewPieces / 2; off > 0; off >>= 1) den += __shfl_xor(den, off, 64);
+    den = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, den)));   // (of the first 16 lanes)
+    for (int i0 = 0;; i0 += 8) {
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i0 + u));
+            num += i0 + u < a.splits ? v[u] * fi : (vec)(0.f);
+        }
+        if (i0 + 8 >= a.splits) break;
+        ask(i0 + 8);
+    }
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    uint16_t *o = a.out + (int64_t)row * a.st.out_token + (int64_t)head * a.st.out_head + dim;
+    if (kEach * lane < HD) {
+        if (kEach == 1) *o = (uint16_t)T::pack(num[0] * inv, 0.f);
+        else {
+#pragma unroll
+            for (int u = 0; u + 1 < kEach; u += 2) *reinterpret_cast<uint32_t *>(o + u) = T::pack(num[u] * inv, num[(u + 1) % kEach] * inv);
+        }
+    }
+    if (a.lse && lane == 0) a.lse[at] = den == 0.f ? -INFINITY : (M + log2f(den)) * 0.693147180559945f;
 }
 
 template <int HD, int G>
@@ -721,38 +802,42 @@ struct PromptPlan {
 // sequences cut into tiles: at most so many (whatever the sequences' lengths are)
 static int64_t prompt_tiles(int64_t seqs, int64_t total_q, int64_t rows) { return (total_q + seqs * (rows - 1)) / rows; }
 
-// Which form, by the workgroups that 128 rows each would make for every compute unit (w) and the steps of 64 keys of the longest walk (s).
-// 128 rows read K and V least often and win where they fill the places of the compute units (3 a unit up to hd 64, 2 at 128, 1 at 256);
-// measured 128 / 64 rows, us: hd 128 w 1.5 37.2 / 36.8, w 1.8 (packed) 51.1 / 44.5, w 2 52.2 / 55.9, w 3 91.8 / 107.7, w 8 520 / 609; hd 64 w 2 60.3 / 51.6, w 3
-// 56.5 / 56.5, w 5 31.6 / 35.2; hd 256 w 1 104.7 / 88.5, w 1.5 143 / 175.  Below that the longest walk decides, and the two other
-// forms by the estimates that fit the measurements: 64 rows take h0 + h1 a step, more where compute units have several; the
-// narrow form, whose four waves share a walk but fetch four times the K and V a row, n0 + 2 n1 a step for its first round of
-// workgroups (r of them, shorter and shorter as the walk of a causal prompt does).  Measured 64 / 32 rows, us: hd 128 300 rows
-// of 8 heads 9.8 / 10.9, 1000 rows of 8 17.9 / 15.9, of 16 18.6 / 24.3, 2300 rows of 2 30.9 / 23.0; hd 64 400 rows of 32
-// 8.6 / 8.8, 1000 rows of 16 13.1 / 12.2, 2400 rows of 4 23.0 / 18.4, 2000 rows of 16 21.6 / 27.7; hd 256 700 rows of 8
-// 30.5 / 22.5, 300 rows of 32 19.1 / 26.8; 32 rows of 32 heads x 128 behind 8000 91 / 30 (keys split).  The keys of a call that
-// leaves compute units without a workgroup are split, not below 512 a piece, and a second launch joins the pieces.
-static PromptPlan prompt_plan(int64_t seqs, int64_t total_q, int64_t heads, int64_t hd, int64_t max_k, int cus)
+// Which form and how many pieces of the keys: the cheapest by an estimate (us) that fits the measurements below.  A workgroup takes
+// `alone` a step of 64 keys by itself; w workgroups a compute unit take `busy` a step and workgroup (the walks of a causal prompt are
+// half as long on average, those of a chunk behind a long context all alike: `even`), the first round of them (`places` run on a unit
+// at once) costs `start`, the others half of it where the steps of another place hide them.  Pieces (of 512 keys and more) shorten the walk, but their sums go to memory and back and a second launch joins them.
+// Measured 128 / 64 / 32 rows a workgroup, us: hd 128: 1024 rows of 32 heads 25.8 / 21.6 / 42, 2048 rows 52.2 / 55.9 / 117, 8192 rows of
+// 32 / 8 520 / 609 / 1153, 2300 rows of 8 heads 44 / 34 / 43, of 2 heads 43 / 31 / 24; hd 64: 2000 rows of 16 heads 30 / 22 / 28, 2400
+// of 4 33 / 23 / 18, 8192 of 16 177 / 188 / 287; hd 256: 2000 rows of 16 heads 105 / 88 / 113, 3000 143 / 175 / 195, 700 of 8 40 / 31 / 23.  Behind 8000
+// keys, 32 / 8 heads x 128, 1 / 2 / 4 / 8 pieces: 150 rows in 64s 95 / 60 / 46 / 46, 512 rows 103 / 96 / 100 / 116, 8 rows in 32s
+// 64 / 40 / 26 / 20.
+static PromptPlan prompt_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t heads, int64_t hd, int64_t max_k, int cus)
 {
-    struct Form { double full, h0, h1, share0, share1, n0, n1; int places; };
-    static const Form forms[3] = {{3.00, 5.5, 0.47, 0.50, 0.50, 6, 0.17, 2}, {1.85, 6, 0.75, 0.45, 0.90, 8, 0.20, 1}, {1.00, 7, 2.10, 0, 1, 14, 0.35, 1}};
-    const Form &f = forms[hd <= 64 ? 0 : hd == 128 ? 1 : 2];
-    PromptPlan p = {kWideRows, (int)prompt_tiles(seqs, total_q, kWideRows), 1};
-    const double w = (double)p.tiles * heads / cus, s = (double)(max_k + 63) / 64;
-    if (w > f.full) return p;
-    const int64_t tiles = prompt_tiles(seqs, total_q, kNarrowRows), slots = (int64_t)cus * f.places;
-    const double share = f.share0 + f.share1 * w, r = (double)tiles * heads / (double)slots;
-    if (f.h0 + f.h1 * s * (share < 1 ? 1 : share) <= f.n0 * (r < 1 ? 1 : r) + f.n1 * s * (1 + (r < 1 ? 1 : r))) {
-        p.rows = kWideRows / 2;
-        p.tiles = (int)prompt_tiles(seqs, total_q, p.rows);
-        return p;
+    struct Form { int rows, places; double start, alone, busy; };
+    static const Form forms[3][3] = {{{kWideRows, 3, 6, 0.73, 0.56}, {kWideRows / 2, 4, 5.5, 0.47, 0.32}, {kNarrowRows, 2, 6, 0.34, 0.25}},
+                                     {{kWideRows, 2, 6, 1.10, 0.92}, {kWideRows / 2, 2, 6, 0.75, 0.60}, {kNarrowRows, 1, 8, 0.43, 0.43}},
+                                     {{kWideRows, 1, 6, 2.90, 2.10}, {kWideRows / 2, 1, 7, 2.10, 1.75}, {kNarrowRows, 1, 14, 0.70, 0.90}}};
+    static const int pieces[12] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+    // the longest walk: no longer than max_k, and where that is no more than all rows, likely not over twice the average sequence's
+    const double longest = (double)(max_k < 2 * total_k / seqs ? max_k : 2 * total_k / seqs), s = (longest + 63) / 64;
+    const double even = total_k > total_q ? 1 - 0.5 * (double)total_q / (double)total_k : 0.5;
+    PromptPlan best = {kWideRows, 0, 1};
+    double least = 0;
+    for (const Form &f : forms[hd <= 64 ? 0 : hd == 128 ? 1 : 2]) {
+        const int64_t tiles = prompt_tiles(seqs, total_q, f.rows);
+        for (const int n : pieces) {
+            // (128 rows a workgroup: whole walks; 64: what the join of few pieces takes)
+            if (n > 1 && (f.rows == kWideRows || s < 8 * n || (f.rows != kNarrowRows && n > kFewPieces))) break;
+            const double w = (double)tiles * heads * n / cus, rounds = w <= f.places ? 1 : f.places == 1 ? w : 0.5 + 0.5 * w / f.places;
+            const double busy = f.busy * (even * w + 1 - even);
+            double us = f.start * rounds + s / n * (busy > f.alone ? busy : f.alone);
+            if (n > 1) us += 3.5 + (double)total_q * heads * n * hd * (8 / 4.5e6);
+            if (best.tiles && us >= least) continue;
+            best = {f.rows, (int)tiles, n};
+            least = us;
+        }
     }
-    p.rows = kNarrowRows;
-    p.tiles = (int)tiles;
-    int64_t n = slots / (tiles * heads);
-    if (n > max_k / 512) n = max_k / 512;
-    p.splits = n < 1 ? 1 : n > 64 ? 64 : (int)n;
-    return p;
+    return best;
 }
 
 static int prompt_sizes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads, int64_t hd)
@@ -772,13 +857,12 @@ static void launch_prompt(const PromptArgs &a, int rows, hipStream_t s)
         hipLaunchKernelGGL((attn_prompt_kernel<HD, T, 1>), grid, dim3(kPromptThreads), (prompt_lds<HD, 1>()), s, a);
         return;
     }
-    if (rows == kWideRows / 2) {
-        hipLaunchKernelGGL((attn_prompt_kernel<HD, T, 2>), grid, dim3(kPromptThreads), (prompt_lds<HD, 2>()), s, a);
-        return;
-    }
-    hipLaunchKernelGGL((attn_prompt_narrow_kernel<HD, T>), grid, dim3(kPromptThreads), narrow_lds<HD>(), s, a);
-    if (a.splits > 1)
-        hipLaunchKernelGGL((attn_prompt_merge_kernel<HD, T>), dim3((unsigned)a.tiles * kNarrowRows, (unsigned)a.heads), dim3(kJoinThreads), 0, s, a);
+    if (rows == kWideRows / 2) hipLaunchKernelGGL((attn_prompt_kernel<HD, T, 2>), grid, dim3(kPromptThreads), (prompt_lds<HD, 2>()), s, a);
+    else hipLaunchKernelGGL((attn_prompt_narrow_kernel<HD, T>), grid, dim3(kPromptThreads), narrow_lds<HD>(), s, a);
+    if (a.splits == 1) return;
+    const unsigned rows32 = (unsigned)prompt_tiles(a.seqs, a.total_q, kNarrowRows) * kNarrowRows;
+    if (a.splits <= kFewPieces) hipLaunchKernelGGL((attn_prompt_merge_few_kernel<HD, T>), dim3(rows32, (unsigned)(a.heads + 3) / 4), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_prompt_merge_kernel<HD, T>), dim3(rows32, (unsigned)a.heads), dim3(kJoinThreads), 0, s, a);
 }
 
 }  // namespace rptc
@@ -792,7 +876,7 @@ extern "C" int64_t rptc_attn_prompt_workspace_bytes(int64_t seqs, int64_t total_
     if (rc) return rc;
     DeviceInfo *dev;
     if ((rc = device_info(&dev))) return rc < 0 ? rc : RPTC_EDEVICE;
-    const int splits = prompt_plan(seqs, total_q, heads, hd, max_k < total_k ? max_k : total_k, dev->cus).splits;
+    const int splits = prompt_plan(seqs, total_q, total_k, heads, hd, max_k < total_k ? max_k : total_k, dev->cus).splits;
     return splits > 1 ? (int64_t)splits * total_q * heads * (hd + 2) * 4 : 0;
 }
 
@@ -835,7 +919,7 @@ extern "C" int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint
     a.total_k = (int)total_k;
     a.heads = (int)heads;
     a.kv_heads = (int)kv_heads;
-    const PromptPlan plan = prompt_plan(seqs, total_q, heads, hd, max_k < total_k ? max_k : total_k, dev->cus);
+    const PromptPlan plan = prompt_plan(seqs, total_q, total_k, heads, hd, max_k < total_k ? max_k : total_k, dev->cus);
     a.tiles = plan.tiles;
     a.splits = plan.splits;
     a.causal = causal ? 1 : 0;

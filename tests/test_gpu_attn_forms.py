@@ -261,3 +261,65 @@ def test_numbers_and_none_where_nothing_is_masked(rk, n, hd):
     k[n - 1, 3] = float("nan")
     rk.attn_prompt(q, k, v, again, causal=False, timed=False)
     assert bool(torch.isnan(again[:, 12:16]).all()) and torch.equal(again[others][:, :12], out[others][:, :12])
+
+
+@pytest.mark.parametrize("hd,dtype", [(32, F16), (64, F16), (64, BF16)])
+def test_long_and_short_sequences_together(rk, hd, dtype):
+    lens = [700, 1, 0, 333, 900, 129, 64, 1000, 1300]
+    run(rk, lens, lens, 32, 8, hd, dtype, True, spoil=True)
+
+
+# rows behind a context long enough for its keys to be cut, too many rows for a workgroup of 32
+CHUNKS = [([150], [3150], 8, 128, F16, True), ([150], [3150], 8, 128, BF16, True), ([300], [5000], 8, 64, F16, True), ([300], [5000], 8, 32, F16, True),
+          ([100, 0, 30], [3000, 7, 2000], 8, 128, F16, True), ([70], [6000], 4, 128, F16, False), ([70], [2001], 32, 128, BF16, True)]
+
+
+@pytest.mark.parametrize("lq,lk,kvh,hd,dtype,causal", CHUNKS)
+def test_chunks_behind_a_long_context(rk, lq, lk, kvh, hd, dtype, causal):
+    run(rk, lq, lk, 32, kvh, hd, dtype, causal, spoil=True)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_pieces_and_values_that_are_no_numbers(rk, bad):
+    # what the last two queries see alone, a query of its own, and at last a key in the middle of a piece, which all see
+    lq, lk, hd = 150, 3150, 128
+    q, k, v, want = run(rk, [lq], [lk], 32, 8, hd, F16, True)
+    k[lk - 1], v[lk - 2:lk], q[5] = bad, bad, float("nan")
+    out = torch.empty_like(q)
+    call = lambda: rk.attn_prompt(q, k, v, out, q_start=ints([0, lq]), k_start=ints([0]), k_len=ints([lk]), max_k=lk, timed=False)
+    call()
+    rows = [i for i in range(lq - 2) if i != 5]
+    tol = 2 * formula(q[:lq][rows[-1:]], k[:lk - 2], v[:lk - 2], False)[2].amax()
+    assert bool(((out[rows].double() - want[rows].double()).abs() <= tol).all())
+    assert bool(torch.isnan(out[5]).all()) and not bool(torch.isfinite(out[lq - 1]).any())
+    k[1000, 3] = float("nan")
+    call()
+    assert bool(torch.isnan(out[:lq, 12:16]).all())
+    assert bool(((out[rows][:, :12].double() - want[rows][:, :12].double()).abs() <= tol).all())
+
+
+def test_pieces_in_two_graphs_and_on_another_stream(rk):
+    q, k, v = randn(41, 150, 32, 128), randn(42, 3150, 8, 128), randn(43, 3150, 8, 128)
+    args = dict(q_start=ints([0, 150]), k_start=ints([0]), k_len=ints([3150]), max_k=3150, timed=False)
+    out, again = torch.empty_like(q), torch.empty_like(q)
+    rk.attn_prompt(q, k, v, out, **args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        rk.attn_prompt(q, k, v, again, **args)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, again)
+    graphs, outs = [], []
+    for _ in range(2):
+        g, o = torch.cuda.CUDAGraph(), torch.empty_like(q)
+        with torch.cuda.graph(g):
+            rk.attn_prompt(q, k, v, o, **args)
+        graphs.append(g)
+        outs.append(o)
+    for _ in range(3):
+        for g, o in zip(graphs, outs):
+            o.zero_()
+            g.replay()
+        torch.randn(1 << 20, device="cuda").sum()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], out) and torch.equal(outs[1], out)
