@@ -19,7 +19,7 @@
 // What bounds it: a SIMD's matrix and vector instructions hardly overlap (a step of 32 rows and 64 keys at hd 128: 0.47 us of one, 0.25 of
 // the other, of 0.9 together), at the clock the power leaves.  8192 causal rows of 32 / 8 heads x 128, bf16: 497 to 512 us, 1.09
 // PFLOP/s, the matrix unit busy for 62 % of it (a library product of 8192^3 1.22 PFLOP/s).  32 rows behind 8000, 32 heads x 128: 30 us
-// for 132 MB, 4.4 TB/s, and 4.6 for joining the pieces.
+// for 132 MB, 4.4 TB/s, and 4 for joining the pieces.
 #include "join.hpp"
 #include "lds_load.hpp"
 
@@ -366,8 +366,9 @@ struct PromptWave {
 // Many rows: 128 query rows of a head a workgroup, 32 a wave (G = 1); all waves walk over the same keys, which are brought to
 // LDS once for the four of them, a step ahead.  G = 2: 64 query rows, two waves a row, one for the first and one for the second half of
 // a step's 64 keys, joined at the end: twice the workgroups with half the walk, where the longest walk is what the call waits
-// for; its keys may be cut into pieces as well (150 rows behind 8000, 32 / 8 heads x 128: 95 us whole, 46 in four) (64 keys a wave and a step of 128 need twice the LDS: 1024 rows of 32 heads x 128 29.4 us instead of 21.6; G = 1 with
-// 32 keys a step meets twice as often: 8192 rows 567 us instead of 520).
+// for; its keys may be cut into pieces as well (150 rows behind 8000, 32 / 8 heads x 128: 95 us whole, 46 in four).  64 keys a wave
+// and a step of 128 need twice the LDS: 1024 rows of 32 heads x 128 29.4 us instead of 21.6; G = 1 with 32 keys a step meets
+// twice as often: 8192 rows 567 us instead of 520.
 template <int HD, int G>
 constexpr int kWaveKeys = G == 2 ? 32 : 64;    // keys of a step and wave
 
