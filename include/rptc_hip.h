@@ -408,10 +408,10 @@ int64_t rptc_lite_viterbi_scratch_bytes(int L, int R, int64_t rows, int64_t step
  *   q_start int32 [seqs + 1], k_start, k_len int32 [seqs], device memory.  q_start NULL: one sequence of all query rows.
  *   k_start and k_len NULL (both or neither): the keys lie as the queries do (total_k == total_q), or, without q_start, are
  *   all key rows.  max_k an upper bound of k_len (total_k will do:
- *   it only decides how far the keys of a call with few rows are split)
+ *   it only decides which form of the kernel runs and into how many pieces the keys are cut)
  *   workspace  rptc_attn_prompt_workspace_bytes(...) bytes (a negative status for sizes the call does not take) of device
- *              memory, 16-byte aligned (0: may be NULL); no initialisation, calls that may overlap need one each.  At most 2^24 query rows, 1024 heads, 2^20 sequences,
- *              (total_q / 32 + seqs) * heads below 2^23.
+ *              memory, 16-byte aligned (0: may be NULL); no initialisation, calls that may overlap need one each.
+ * At most 2^24 query rows, 1024 heads, 2^20 sequences, (total_q / 32 + seqs) * heads below 2^23.
  */
 typedef struct rptc_prompt_strides {
     int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
