@@ -215,11 +215,22 @@ __global__ __launch_bounds__(kScoreThreads) void token_logprobs_kernel(const Sco
     }
     const float base = M == -INFINITY ? 0.f : M;
     const bool none = l == 0.f;                // a row of -inf only
-    const float ln_l = none ? __builtin_nanf("") : log2f(l) * kLn2;
-    auto logp = [&](float v) { return (v - base) - ln_l; };
+    // The results are differences of numbers of their own size, so ln l is held in two parts: with l = 2^k f, k ln 2 to 15 bits
+    // (exact) and the rest, and a difference is rounded once, at its end (the error falls from 3.4e-8 of a log probability to 2.5e-8).
+    const float k = (float)__builtin_amdgcn_frexp_expf(l);
+    const float ln_hi = none ? __builtin_nanf("") : k * 0x1.62e4p-1f, ln_lo = fmaf(k, 0x1.7f7d1cp-20f, log2f(__builtin_amdgcn_frexp_mantf(l)) * kLn2);
+    auto less_ln_l = [&](float d, float rest) {            // d + rest - ln l
+        const float s = d - ln_hi, b = s - d;
+        const float lost = (d - (s - b)) + (-ln_hi - b);
+        return d == -INFINITY ? d - (ln_hi + ln_lo) : s + (lost + (rest - ln_lo));
+    };
+    auto logp = [&](float v) { return less_ln_l(v - base, 0.f); };
     if (tid == 0) {
         if (wants_token) a.logprob[row] = tok_ok ? logp(x_tok) : __builtin_nanf("");
-        if (a.entropy) a.entropy[row] = ln_l - t / l;
+        if (a.entropy) {
+            const float mean = t / l;                      // of d; what its rounding left is added as well
+            a.entropy[row] = -less_ln_l(mean, fmaf(-mean, l, t) / l);
+        }
     }
     if (a.top == 0) return;
 

@@ -5,6 +5,8 @@ c = 2^-23 (1.45 |d| + 2) (the product with log2 e, the instruction's unit in the
 weigh less than 2^-100; the sums have at most n roundings in a thread and log2(threads) over them: with n = 150 additions a thread
 l is off by at most (150 + 24) 2^-24 + max c (weighted): together below 2^-15 for the sizes here.  A log probability is
 then off by 2^-24 |d| + 2^-15 + 2^-23 |ln l|; the entropy by 2^-15 (1 + |t| / l) and its roundings."""
+import math
+
 import pytest
 import torch
 
@@ -173,3 +175,24 @@ def test_rows_past_2_31_logits(rk):
     rk.token_logprobs(part, torch.arange(rows - 5, rows, device="cuda") % 5, alone, top_ids=alone_ids, timed=False)
     assert torch.equal(lp[-5:], alone) and torch.equal(ids[-5:], alone_ids) and torch.equal(ids[:5], alone_ids)
     assert torch.equal(ids[5:-5], torch.arange(3, device="cuda").expand(rows - 10, 3))       # all equal: the lowest ids
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_tokens_without_probability_and_far_ones(rk, dtype):
+    # a token at -inf, at the type's lowest value below a large one, and beside the largest of a flat row
+    low = torch.finfo(dtype).min
+    x = torch.zeros((5, 300), dtype=dtype, device="cuda")
+    x[0, 7], x[1, 7], x[2] = float("-inf"), low, low
+    x[3, 5], x[3, 7] = -low, low                      # their difference is beyond fp32 in the wide types
+    x[4, 7] = float("nan")
+    lp, en = torch.empty(5, device="cuda"), torch.empty(5, device="cuda")
+    rk.token_logprobs(x, torch.full((5,), 7, device="cuda"), lp, en, timed=False)
+    want = torch.log_softmax(x.double(), -1)[:, 7]
+    assert lp[0] == float("-inf") and bool(torch.isnan(lp[4])) and bool(torch.isnan(en[4]))
+    assert abs(float(lp[2]) + math.log(300)) < 1e-6 * math.log(300) and abs(float(en[2]) - math.log(300)) < 1e-6 * math.log(300)
+    assert abs(float(en[0]) - math.log(299)) < 1e-6 * math.log(299)
+    for i in (1, 3):
+        # what rounds to fp32's range (-FLT_MAX - ln 299 does: half a step there is 1e31) is a number, what does not is -inf
+        w = float(want[i].float())
+        assert float(lp[i]) == w if math.isinf(w) else abs(float(lp[i]) / w - 1) < 1e-6
+    assert float(en[3]) == 0.0
