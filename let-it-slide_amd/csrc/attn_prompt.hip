@@ -49,6 +49,12 @@ struct TypeF16 {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, half2_t));
     }
     static __device__ __forceinline__ float to_float(uint16_t b) { return half_bits_to_float(b); }
+    static constexpr short kExponent = 0x7C00;
+    // sum + 0 x for two values x: not a number where one of them is no finite number
+    static __device__ __forceinline__ float zero_of(uint32_t w, float sum)
+    {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, w), (half2_t)((_Float16)0.f), sum, false);
+    }
 };
 struct TypeBf16 {
     static __device__ __forceinline__ float16_t mfma(short8_t a, short8_t b, float16_t c)
@@ -61,6 +67,11 @@ struct TypeBf16 {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));
     }
     static __device__ __forceinline__ float to_float(uint16_t b) { return __builtin_bit_cast(float, (uint32_t)b << 16); }
+    static constexpr short kExponent = 0x7F80;
+    static __device__ __forceinline__ float zero_of(uint32_t w, float sum)
+    {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), (bf16x2_t)((__bf16)0.f), sum, false);
+    }
 };
 
 struct PromptArgs {
@@ -176,63 +187,45 @@ __device__ __forceinline__ int swizzle_v(int row)
     return HD >= 128 ? (row & 3) << 2 : HD == 64 ? (row >> 1 & 1) << 2 : 0;
 }
 
-// Rows in plain fp32, one after the other (bit i of `which`: row row_first + i), keys [k_lo, k_hi) of those a row sees.  Taken when a
-// sum of the matrix path came out infinite or not a number: that is right where the row sees such a value, and wrong where only a
-// masked key or a masked row of V held it (0 * NaN is NaN), so the rows are worked out again without the masked ones.
+// Values of V that are no finite numbers in a step where some row does not see some key (the last one or two of a walk): the weight is 0
+// there, but 0 times infinity or not-a-number is none, and would reach a row that must not show it.  Where a wave's sums came out odd
+// and its steps with masked keys hold such values, the walk is taken three times more: with a 1 in place of every value that is +infinity or
+// not-a-number, a 0 of every other and equal weights, which marks the elements that see one; so for -infinity or not-a-number; and
+// with 0 in place of all of them, in the first walk's order.  The elements then get what they saw, and one that saw none has the bits it
+// has with zeros in V.  At most five times the time of a call without them (2000 rows of 32 heads x 128: 54 us, with an infinity in the
+// first and the last values 244, nothing but not-a-numbers 275; the odd rows one after the other, with plain loads, took 11.5 ms and grew
+// with the square of the rows).
+enum { kUps, kDowns, kFiniteOnly, kWalks };
+// whether rows [k0, k1) of V hold such values
 template <int HD, class T>
-__device__ __forceinline__ void prompt_rows_plain(const PromptArgs &a, const PromptTile &t, int row_first, uint32_t which, int head, int kvh,
-                                                  int k_lo, int k_hi, int split)
+__device__ __forceinline__ bool values_odd(const uint16_t *v, int64_t token, int k0, int k1)
 {
-    const int lane = threadIdx.x & 63;
-    constexpr int kOut = (HD + 63) / 64;
-    for (; which; which &= which - 1) {
-        const int row = row_first + __builtin_ctz(which);
-        if (row >= t.q_end) break;
-        const int end = min(prompt_sees(a, t, row), k_hi);
-        const uint16_t *q = a.q + (int64_t)row * a.st.q_token + (int64_t)head * a.st.q_head;
-        auto score = [&](int j) {
-            const uint16_t *k = a.k + (int64_t)(t.k_first + j) * a.st.k_token + (int64_t)kvh * a.st.k_head;
-            float s = 0.f;
-            for (int d = 0; d < HD; d += 8) {
-                const short8_t qv = *reinterpret_cast<const short8_t *>(q + d), kv = *reinterpret_cast<const short8_t *>(k + d);
-#pragma unroll
-                for (int u = 0; u < 8; u++) s = fmaf(T::to_float((uint16_t)qv[u]), T::to_float((uint16_t)kv[u]), s);
-            }
-            return s;
-        };
-        float m = -INFINITY;
-        for (int j = k_lo + lane; j < end; j += 64) m = fmaxf(m, score(j));
-        for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-        const float mc = m == -INFINITY ? 0.f : m * a.c;
-        float l = 0.f, acc[kOut];
-        for (int u = 0; u < kOut; u++) acc[u] = 0.f;
-        for (int j0 = k_lo; j0 < end; j0 += 64) {
-            const float p = j0 + lane < end ? __builtin_amdgcn_exp2f(fmaf(score(j0 + lane), a.c, -mc)) : 0.f;
-            l += p;
-            for (int i = 0; i < min(64, end - j0); i++) {
-                const float pi = __shfl(p, i, 64);
-                const uint16_t *v = a.v + (int64_t)(t.k_first + j0 + i) * a.st.v_token + (int64_t)kvh * a.st.v_head;
-                for (int u = 0; u < kOut; u++)
-                    if (lane + 64 * u < HD) acc[u] = fmaf(pi, T::to_float(v[lane + 64 * u]), acc[u]);
-            }
-        }
-        for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
-        const int64_t at = (int64_t)row * a.heads + head;
-        if (a.splits > 1) {
-            const int64_t pa = at * a.splits + split;
-            for (int u = 0; u < kOut; u++)
-                if (lane + 64 * u < HD) a.part_acc[pa * HD + lane + 64 * u] = acc[u];
-            if (lane == 0) {
-                a.part_ml[2 * pa] = l == 0.f ? -INFINITY : mc;
-                a.part_ml[2 * pa + 1] = l;
-            }
-            continue;
-        }
-        uint16_t *o = a.out + (int64_t)row * a.st.out_token + (int64_t)head * a.st.out_head;
-        for (int u = 0; u < kOut; u++)
-            if (lane + 64 * u < HD) o[lane + 64 * u] = (uint16_t)T::pack(l == 0.f ? 0.f : acc[u] / l, 0.f);
-        if (a.lse && lane == 0) a.lse[at] = l == 0.f ? -INFINITY : (mc + log2f(l)) * 0.693147180559945f;
+    float none = 0.f;
+    for (int i = 8 * (threadIdx.x & 63); i < (k1 - k0) * HD; i += 512) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(v + (k0 + i / HD) * token + i % HD);
+        none = T::zero_of(w.w, T::zero_of(w.z, T::zero_of(w.y, T::zero_of(w.x, none))));
     }
+    return __ballot(none != 0.f) != 0;
+}
+template <class T>
+__device__ __forceinline__ void change_values(uint16_t *v, int walk)
+{
+    uint4 w = *reinterpret_cast<uint4 *>(v);
+    uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    const uint32_t one = T::pack(1.f, 1.f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int b = 0; b < 32; b += 16) {
+            const uint32_t half = 0xFFFFu << b, value = x[i] & half, least = (uint32_t)T::kExponent << b, minus = least | 0x8000u << b;
+            const bool finite = (value & least) != least;
+            if (walk == kFiniteOnly) r |= finite ? value : 0u;
+            else r |= !finite && value != (walk == kUps ? minus : least) ? one & half : 0u;
+        }
+        x[i] = r;
+    }
+    *reinterpret_cast<uint4 *>(v) = make_uint4(x[0], x[1], x[2], x[3]);
 }
 
 // What a wave holds of 32 query rows, and the parts of a step over KEYS keys (a multiple of 32).  Lane (col, c): row col; of
@@ -242,6 +235,7 @@ __device__ __forceinline__ void prompt_rows_plain(const PromptArgs &a, const Pro
 template <int HD, class T, int KEYS, int TERMS>
 struct PromptWave {
     static constexpr int kSteps = HD / 16, kDims = HD / 32, kBlocks = KEYS / 32;
+    int tid;                               // the thread in its workgroup
     short8_t qf[kSteps];
     float16_t acc[kDims];
     float m, l;                            // running bound of c * score (log2 units), sum of p over the lane's keys
@@ -249,7 +243,7 @@ struct PromptWave {
     __device__ __forceinline__ void begin(const PromptArgs &a, const PromptTile &t, int row, int head)
     {
         // a lane without a row of its own takes the sequence's last (its results go nowhere)
-        const uint16_t *q = a.q + (int64_t)min(row, t.q_end - 1) * a.st.q_token + (int64_t)head * a.st.q_head + 8 * ((threadIdx.x & 63) >> 5);
+        const uint16_t *q = a.q + (int64_t)min(row, t.q_end - 1) * a.st.q_token + (int64_t)head * a.st.q_head + 8 * ((tid & 63) >> 5);
 #pragma unroll
         for (int i = 0; i < kSteps; i++) qf[i] = *reinterpret_cast<const short8_t *>(q + 16 * i);
 #pragma unroll
@@ -266,7 +260,7 @@ struct PromptWave {
     // S^T of the keys in LDS at kt
     __device__ __forceinline__ void scores(const uint16_t *kt, float16_t (&s)[kBlocks]) const
     {
-        const int lane = threadIdx.x & 63, c = lane >> 5, col = lane & 31;
+        const int lane = tid & 63, c = lane >> 5, col = lane & 31;
 #pragma unroll
         for (int h = 0; h < kBlocks; h++) {
             s[h] = (float16_t)(0.f);
@@ -278,10 +272,18 @@ struct PromptWave {
             }
         }
     }
-    // keys from `left` on (counted from the step's first) are not the row's
-    static __device__ __forceinline__ void mask(float16_t (&s)[kBlocks], int left)
+    // the same for a walk taken again: where it marks, every key weighs the same
+    __device__ __forceinline__ void scores_of(const uint16_t *kt, int walk, float16_t (&s)[kBlocks]) const
     {
-        left -= 4 * ((threadIdx.x & 63) >> 5);
+        scores(kt, s);
+        if (walk == kFiniteOnly) return;
+#pragma unroll
+        for (int h = 0; h < kBlocks; h++) s[h] = (float16_t)(0.f);
+    }
+    // keys from `left` on (counted from the step's first) are not the row's
+    __device__ __forceinline__ void mask(float16_t (&s)[kBlocks], int left) const
+    {
+        left -= 4 * ((tid & 63) >> 5);
 #pragma unroll
         for (int h = 0; h < kBlocks; h++)
 #pragma unroll
@@ -328,7 +330,7 @@ struct PromptWave {
     __device__ __forceinline__ void product(const uint16_t *vt, const uint32_t (&p)[TERMS][kBlocks][8])
     {
         typedef __attribute__((address_space(3))) short4_t lds_short4;
-        const int lane = threadIdx.x & 63, c = lane >> 5, g16 = lane >> 4, rr = (lane & 15) >> 2, piece = lane & 3;
+        const int lane = tid & 63, c = lane >> 5, g16 = lane >> 4, rr = (lane & 15) >> 2, piece = lane & 3;
 #pragma unroll
         for (int h = 0; h < kBlocks; h++)
 #pragma unroll
@@ -349,9 +351,7 @@ struct PromptWave {
                 }
             }
     }
-    // whether the sum of p of the lane's row is infinite or not a number
-    __device__ __forceinline__ bool odd_sum() const { return halves_max(l * 0.f != 0.f ? 1.f : 0.f) != 0.f; }
-    // whether another sum of it is
+    // whether a sum came out infinite or not a number, in any of the rows
     __device__ __forceinline__ bool odd() const
     {
         float bad = 0.f;
@@ -359,7 +359,39 @@ struct PromptWave {
         for (int d = 0; d < kDims; d++)
 #pragma unroll
             for (int r = 0; r < 16; r++) bad = fmaf(acc[d][r], 0.f, bad);
-        return halves_max(bad != 0.f ? 1.f : 0.f) != 0.f;      // (not-a-number compares unequal)
+        return __ballot(bad != 0.f) != 0;                  // (not-a-number compares unequal)
+    }
+    // which elements are above 0, a bit each
+    static constexpr int kMarks = HD < 64 ? 1 : HD / 64;
+    __device__ __forceinline__ void take_marks(uint32_t *marks) const
+    {
+#pragma unroll
+        for (int i = 0; i < kMarks; i++) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int d = 2 * i; d < 2 * i + 2 && d < kDims; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) bits = bits << 1 | (acc[d][r] > 0.f ? 1u : 0u);
+            marks[i * kPromptThreads] = bits;
+        }
+    }
+    // the infinities (not-a-number where it is both) that the elements see
+    __device__ __forceinline__ void put_marks(const uint32_t *ups, const uint32_t *downs)
+    {
+#pragma unroll
+        for (int i = 0; i < kMarks; i++) {
+            uint32_t up = ups[i * kPromptThreads], down = downs[i * kPromptThreads];
+#pragma unroll
+            for (int d = 2 * i + 1; d >= 2 * i; d--)
+#pragma unroll
+                for (int r = 15; r >= 0; r--) {
+                    if (d >= kDims) continue;
+                    if (up & 1u) acc[d][r] += INFINITY;
+                    if (down & 1u) acc[d][r] -= INFINITY;
+                    up >>= 1;
+                    down >>= 1;
+                }
+        }
     }
 };
 
@@ -372,16 +404,22 @@ struct PromptWave {
 template <int HD, int G>
 constexpr int kWaveKeys = G == 2 ? 32 : 64;    // keys of a step and wave
 
+// workgroups that a compute unit holds at once (by their registers; LDS has room for as many): said to the compiler as least and
+// most, so that it uses the registers for operands asked for early instead of for more of them
+template <int HD, int G>
+constexpr int kPlaces = HD > 128 ? 1 : HD == 128 ? 2 : HD == 64 && G == 1 ? 3 : 4;
+
 template <int HD, class T, int G>
-__global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_kernel(const PromptArgs a)
+__global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(kPlaces<HD, G>, kPlaces<HD, G>))) void attn_prompt_kernel(const PromptArgs a)
 {
     extern __shared__ __align__(16) uint16_t lds[];       // two buffers of K, two of V, [kKeys][HD] each
     constexpr int kMine = kWaveKeys<HD, G>, kKeys = G * kMine, kTile = kKeys * HD, kRows = kWideRows / G;
     static_assert(G == 1 || 2 * 32 * HD * 4 <= 4 * kTile * 2, "the sums of two waves fit where K and V were");
     __shared__ float s_ml[2][32][2];
-    __shared__ int s_odd[2][32];
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-    const int c = lane >> 5, col = lane & 31;
+    __shared__ uint32_t s_marks[2][PromptWave<HD, T, kMine, 1>::kMarks * kPromptThreads];
+    __shared__ int s_again;
+    int tid = threadIdx.x, lane = tid & 63, c = lane >> 5, col = lane & 31;
+    const int wave = uniform(tid >> 6);
     int head, tile, split;
     prompt_item(a, head, tile, split);
     PromptTile t;
@@ -397,9 +435,10 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
         k_hi = uniform((int)min((int64_t)k_most, (int64_t)k_lo + per_split));
     }
     const int group = G == 2 ? wave >> 1 : 0, koff = group * kMine;
-    const int row_first = t.row0 + 32 * (wave & (4 / G - 1)), row = row_first + col;
+    const int row_first = t.row0 + 32 * (wave & (4 / G - 1));
+    int row = row_first + col;
     const bool wave_live = row_first < t.q_end;
-    const int see = row < t.q_end ? prompt_sees(a, t, row) : 0;
+    int see = row < t.q_end ? prompt_sees(a, t, row) : 0;
     // what all rows of the wave see, and what one of them sees
     const int see_least = uniform(wave_live ? prompt_sees(a, t, row_first) : 0);
     const int see_most = uniform(wave_live ? prompt_sees(a, t, min(row_first + 31, t.q_end - 1)) : 0);
@@ -435,11 +474,11 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
         if (k_lo + kKeys < k_hi) request_k(k_lo + kKeys, 1);
     }
     PromptWave<HD, T, kMine, 1> w;
+    w.tid = tid;
     w.begin(a, t, row, head);
     w.settle();
-    // A row whose sum of p is odd before a key of its wave is masked sees the key that made it so: it stays as it is (a prompt full of
-    // not-a-numbers takes no longer than any other; 2000 rows of them 0.29 ms instead of 11.7; asking the sums of V as well cost 2 %).
-    bool masked = false, before = false;
+    if (tid == 0) s_again = 0;
+    int masked_from = 0x7FFFFFFF;                          // the first step with a key that some row of the wave does not see
     // One step: the softmax of the scores s of the keys from k0 on and their product with V, while the matrix unit forms the
     // next step's scores (behind the last step these are of whatever the buffer holds, and nobody looks at them).
     auto step = [&](int k0, int buf, float16_t (&s)[kMine / 32], float16_t (&next)[kMine / 32]) {
@@ -448,9 +487,9 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
         if (k0 + 2 * kKeys < k_hi) request_k(k0 + 2 * kKeys, buf);
         if (k0 + kKeys < k_hi) request_v(k0 + kKeys, buf ^ 1);
         if (k0 + koff >= see_most) return;
-        if (k0 + koff + kMine > see_least) {               // some row of the wave does not see all of its keys
-            if (!masked) before = w.odd_sum();
-            masked = true;
+        const bool masked = k0 + koff + kMine > see_least; // some row of the wave does not see all of its keys
+        if (masked) {
+            masked_from = min(masked_from, k0 + koff);
             w.mask(s, see - k0 - koff);
         }
         const float off = w.bound(s, a.c);
@@ -469,79 +508,117 @@ __global__ __launch_bounds__(kPromptThreads, HD > 128 ? 1 : 2) void attn_prompt_
             if (k0 + kKeys >= k_hi) break;
             step(k0 + kKeys, 1, sb, sa);
         }
+        // what is known of the lane is worked out again for what follows: kept over the walk it would cost the registers that let
+        // the loop ask for its operands early
+        asm volatile("" : "+v"(tid));
+        w.tid = tid;
+        lane = tid & 63;
+        c = lane >> 5;
+        col = lane & 31;
+        row = row_first + col;
+        see = row < t.q_end ? prompt_sees(a, t, row) : 0;
+        if (masked_from < k_hi && w.odd() && values_odd<HD, T>(v_base, a.st.v_token, masked_from, min(t.k_len, see_most + kMine))) s_again = 1;
     }
-    bool odd = w.odd();
-    if (!masked) before = odd;                             // no key of the wave was masked
-    float l = halves_sum(w.l);
-    if (G == 2) {
-        // sums of the second half's waves to the first's, a register of all lanes after the other
-        float4 *sums = reinterpret_cast<float4 *>(lds) + (wave & 1) * (HD * 8) + lane;
-        __syncthreads();                                   // nobody reads K or V now
-        if (group == 1) {
+    auto finish = [&]() {
+        float l = halves_sum(w.l);
+        if (G == 2) {
+            // sums of the second half's waves to the first's, a register of all lanes after the other
+            float4 *sums = reinterpret_cast<float4 *>(lds) + (wave & 1) * (HD * 8) + lane;
+            if (group == 1) {
+#pragma unroll
+                for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+                    for (int b = 0; b < 4; b++)
+                        sums[64 * (4 * d + b)] = make_float4(w.acc[d][4 * b], w.acc[d][4 * b + 1], w.acc[d][4 * b + 2], w.acc[d][4 * b + 3]);
+                if (c == 0) {
+                    s_ml[wave & 1][col][0] = w.m;
+                    s_ml[wave & 1][col][1] = l;
+                }
+            }
+            __syncthreads();
+            if (group == 1) return;
+            const float m1 = s_ml[wave][col][0], M = fmaxf(w.m, m1);
+            const float f0 = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - M), f1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - M);
+            l = l * f0 + s_ml[wave][col][1] * f1;
+            w.m = M;
 #pragma unroll
             for (int d = 0; d < HD / 32; d++)
 #pragma unroll
-                for (int b = 0; b < 4; b++)
-                    sums[64 * (4 * d + b)] = make_float4(w.acc[d][4 * b], w.acc[d][4 * b + 1], w.acc[d][4 * b + 2], w.acc[d][4 * b + 3]);
-            if (c == 0) {
-                s_ml[wave & 1][col][0] = w.m;
-                s_ml[wave & 1][col][1] = l;
-                s_odd[wave & 1][col] = (odd ? 1 : 0) | (before ? 2 : 0);
-            }
+                for (int b = 0; b < 4; b++) {
+                    const float4 o = sums[64 * (4 * d + b)];
+                    w.acc[d][4 * b] = fmaf(o.x, f1, w.acc[d][4 * b] * f0);
+                    w.acc[d][4 * b + 1] = fmaf(o.y, f1, w.acc[d][4 * b + 1] * f0);
+                    w.acc[d][4 * b + 2] = fmaf(o.z, f1, w.acc[d][4 * b + 2] * f0);
+                    w.acc[d][4 * b + 3] = fmaf(o.w, f1, w.acc[d][4 * b + 3] * f0);
+                }
         }
-        __syncthreads();
-        if (group == 1) return;
-        odd = odd || (s_odd[wave][col] & 1);
-        before = before || (s_odd[wave][col] & 2);
-        const float m1 = s_ml[wave][col][0], M = fmaxf(w.m, m1);
-        const float f0 = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(w.m - M), f1 = m1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m1 - M);
-        l = l * f0 + s_ml[wave][col][1] * f1;
-        w.m = M;
+        if (!wave_live) return;
+        if (G == 2 && a.splits > 1) {
+            if (row < t.q_end) {
+                const int64_t pa = ((int64_t)row * a.heads + head) * a.splits + split;
+                float *part = a.part_acc + pa * HD + 4 * c;
+#pragma unroll
+                for (int d = 0; d < HD / 32; d++)
+#pragma unroll
+                    for (int b = 0; b < 4; b++)
+                        *reinterpret_cast<float4 *>(part + 32 * d + 8 * b) = make_float4(w.acc[d][4 * b], w.acc[d][4 * b + 1], w.acc[d][4 * b + 2], w.acc[d][4 * b + 3]);
+                if (c == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * pa) = make_float2(l == 0.f ? -INFINITY : w.m, l);
+            }
+            return;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;            // a row that sees nothing: zeros
+        uint16_t *o = a.out + (int64_t)min(row, t.q_end - 1) * a.st.out_token + (int64_t)head * a.st.out_head + 8 * c;
 #pragma unroll
         for (int d = 0; d < HD / 32; d++)
 #pragma unroll
-            for (int b = 0; b < 4; b++) {
-                const float4 o = sums[64 * (4 * d + b)];
-                w.acc[d][4 * b] = fmaf(o.x, f1, w.acc[d][4 * b] * f0);
-                w.acc[d][4 * b + 1] = fmaf(o.y, f1, w.acc[d][4 * b + 1] * f0);
-                w.acc[d][4 * b + 2] = fmaf(o.z, f1, w.acc[d][4 * b + 2] * f0);
-                w.acc[d][4 * b + 3] = fmaf(o.w, f1, w.acc[d][4 * b + 3] * f0);
+            for (int b = 0; b < 4; b += 2) {
+                // the lane's four dimensions of blocks b and b + 1 (8 dimensions each, the halves of the wave four): a swap of
+                // the halves leaves eight consecutive ones of block b + c in each lane
+                const float16_t &x = w.acc[d];
+                uint32_t x0 = T::pack(x[4 * b] * inv, x[4 * b + 1] * inv), x1 = T::pack(x[4 * b + 2] * inv, x[4 * b + 3] * inv);
+                uint32_t y0 = T::pack(x[4 * b + 4] * inv, x[4 * b + 5] * inv), y1 = T::pack(x[4 * b + 6] * inv, x[4 * b + 7] * inv);
+                const auto w0 = __builtin_amdgcn_permlane32_swap(x0, y0, false, false), w1 = __builtin_amdgcn_permlane32_swap(x1, y1, false, false);
+                if (row < t.q_end)
+                    *reinterpret_cast<uint4 *>(o + 32 * d + 8 * b) = make_uint4((uint32_t)w0[0], (uint32_t)w1[0], (uint32_t)w0[1], (uint32_t)w1[1]);
             }
-    }
-    if (!wave_live) return;
-    const bool redo = odd && !before;
-    const uint32_t which = (uint32_t)__ballot(redo);
-    if (G == 2 && a.splits > 1) {
-        if (row < t.q_end && !redo) {
-            const int64_t pa = ((int64_t)row * a.heads + head) * a.splits + split;
-            float *part = a.part_acc + pa * HD + 4 * c;
-#pragma unroll
-            for (int d = 0; d < HD / 32; d++)
-#pragma unroll
-                for (int b = 0; b < 4; b++)
-                    *reinterpret_cast<float4 *>(part + 32 * d + 8 * b) = make_float4(w.acc[d][4 * b], w.acc[d][4 * b + 1], w.acc[d][4 * b + 2], w.acc[d][4 * b + 3]);
-            if (c == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * pa) = make_float2(l == 0.f ? -INFINITY : w.m, l);
+        if (a.lse && c == 0 && row < t.q_end) a.lse[(int64_t)row * a.heads + head] = l == 0.f ? -INFINITY : (w.m + log2f(l)) * 0.693147180559945f;
+    };
+    // every wave has said whether to go again, and nobody reads K or V any more; one that need not wait for that has stored its rows
+    if (G == 1) finish();
+    __syncthreads();
+    if (k_lo < k_hi && s_again) {
+#pragma unroll 1
+        for (int walk = kUps; walk < kWalks; walk++) {
+            request_k(k_lo, 0);
+            request_v(k_lo, 0);
+            w.begin(a, t, row, head);
+            w.settle();
+#pragma unroll 1
+            for (int k0 = k_lo, buf = 0; k0 < k_hi; k0 += kKeys, buf ^= 1) {
+                wait_for_lds_loads();
+                __syncthreads();
+                if (k0 + kKeys < k_hi) {
+                    request_k(k0 + kKeys, buf ^ 1);
+                    request_v(k0 + kKeys, buf ^ 1);
+                }
+#pragma unroll 1
+                for (int i = 8 * tid; i < kTile; i += 8 * kPromptThreads) change_values<T>(lds + (2 + buf) * kTile + i, walk);
+                __syncthreads();
+                if (k0 + koff >= see_most) continue;
+                float16_t s[kMine / 32];
+                uint32_t p[1][kMine / 32][8];
+                w.scores_of(lds + buf * kTile + koff * HD, walk, s);
+                if (k0 + koff + kMine > see_least) w.mask(s, see - k0 - koff);
+                w.weights(s, a.c, w.bound(s, a.c), p);
+                w.product(lds + (2 + buf) * kTile + koff * HD, p);
+            }
+            if (walk != kFiniteOnly) w.take_marks(s_marks[walk - kUps] + tid);
+            __syncthreads();                               // nobody reads K or V now
         }
-        if (which) prompt_rows_plain<HD, T>(a, t, row_first, which, head, kvh, k_lo, k_hi, split);
-        return;
+        w.put_marks(s_marks[0] + tid, s_marks[1] + tid);
+        if (G == 1) finish();
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;            // a row that sees nothing: zeros
-    uint16_t *o = a.out + (int64_t)min(row, t.q_end - 1) * a.st.out_token + (int64_t)head * a.st.out_head + 8 * c;
-#pragma unroll
-    for (int d = 0; d < HD / 32; d++)
-#pragma unroll
-        for (int b = 0; b < 4; b += 2) {
-            // the lane's four dimensions of blocks b and b + 1 (8 dimensions each, the halves of the wave four): a swap of
-            // the halves leaves eight consecutive ones of block b + c in each lane
-            const float16_t &x = w.acc[d];
-            uint32_t x0 = T::pack(x[4 * b] * inv, x[4 * b + 1] * inv), x1 = T::pack(x[4 * b + 2] * inv, x[4 * b + 3] * inv);
-            uint32_t y0 = T::pack(x[4 * b + 4] * inv, x[4 * b + 5] * inv), y1 = T::pack(x[4 * b + 6] * inv, x[4 * b + 7] * inv);
-            const auto w0 = __builtin_amdgcn_permlane32_swap(x0, y0, false, false), w1 = __builtin_amdgcn_permlane32_swap(x1, y1, false, false);
-            if (row < t.q_end && !redo)
-                *reinterpret_cast<uint4 *>(o + 32 * d + 8 * b) = make_uint4((uint32_t)w0[0], (uint32_t)w1[0], (uint32_t)w0[1], (uint32_t)w1[1]);
-        }
-    if (a.lse && c == 0 && row < t.q_end && !redo) a.lse[(int64_t)row * a.heads + head] = l == 0.f ? -INFINITY : (w.m + log2f(l)) * 0.693147180559945f;
-    if (which) prompt_rows_plain<HD, T>(a, t, row_first, which, head, kvh, 0, k_hi, 0);
+    if (G == 2) finish();
 }
 
 // Few rows: 32 query rows of a head a workgroup; the four waves hold the same rows and take the steps over the keys (of this
@@ -558,9 +635,9 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
     static_assert(kNarrowRows * kJoinRow * 4 <= 2 * kTile * 2, "a wave's sums fit where its K and V were");
     extern __shared__ __align__(16) uint16_t lds[];       // [wave][K, V][kStep][HD]
     __shared__ float s_ml[4][kNarrowRows][2];
-    __shared__ uint32_t s_odd[4], s_seen[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-    const int c = lane >> 5, col = lane & 31;
+    __shared__ uint32_t s_marks[2][PromptWave<HD, T, kStep, 2>::kMarks * kPromptThreads];
+    int tid = threadIdx.x, lane = tid & 63, c = lane >> 5, col = lane & 31;
+    const int wave = uniform(tid >> 6);
     int head, tile, split;
     prompt_item(a, head, tile, split);
     PromptTile t;
@@ -570,8 +647,8 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
     const int per_split = ((k_most + a.splits - 1) / a.splits + kStep - 1) / kStep * kStep;
     const int k_lo = uniform((int)min((int64_t)k_most, (int64_t)split * per_split));
     const int k_hi = uniform((int)min((int64_t)k_most, (int64_t)k_lo + per_split));
-    const int row = t.row0 + col;
-    const int see = min(row < t.q_end ? prompt_sees(a, t, row) : 0, k_hi);
+    int row = t.row0 + col;
+    int see = min(row < t.q_end ? prompt_sees(a, t, row) : 0, k_hi);
     const int see_least = uniform(min(prompt_sees(a, t, t.row0), k_hi));
 
     // a request is 1024 bytes: 512 / HD rows; the swizzles repeat every 16 rows (K) and every 4 (V)
@@ -602,25 +679,26 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
     };
 
     constexpr int kStride = 4 * kStep;
-    int k0 = k_lo + wave * kStep;
-    if (k0 < k_hi) {
-        request_k(k0);
-        request_v(k0);
+    const int k_first = k_lo + wave * kStep;
+    if (k_first < k_hi) {
+        request_k(k_first);
+        request_v(k_first);
     }
     PromptWave<HD, T, kStep, 2> w;
+    w.tid = tid;
     w.begin(a, t, row, head);
     w.settle();
-    bool masked = false, before = false;                   // as above
-    for (; k0 < k_hi; k0 += kStride) {
+    int masked_from = 0x7FFFFFFF;                          // as above
+    for (int k0 = k_first; k0 < k_hi; k0 += kStride) {
         const bool more = k0 + kStride < k_hi;
         wait_for_lds_loads_but<kRequests>();               // K is there (V was asked for behind it)
         float16_t s[kStep / 32];
         w.scores(kt, s);
         wait_for_lds_reads();
         if (more) request_k(k0 + kStride);
-        if (k0 + kStep > see_least) {
-            if (!masked) before = w.odd_sum();
-            masked = true;
+        const bool masked = k0 + kStep > see_least;        // some row does not see all of the step's keys
+        if (masked) {
+            masked_from = min(masked_from, k0);
             w.mask(s, see - k0);
         }
         const float off = w.bound(s, a.c);
@@ -632,17 +710,42 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
         wait_for_lds_reads();
         if (more) request_v(k0 + kStride);
     }
+    asm volatile("" : "+v"(tid));                        // as above
+    w.tid = tid;
+    lane = tid & 63;
+    c = lane >> 5;
+    col = lane & 31;
+    row = t.row0 + col;
+    see = min(row < t.q_end ? prompt_sees(a, t, row) : 0, k_hi);
+    if (masked_from < k_hi && w.odd() && values_odd<HD, T>(v_base, a.st.v_token, masked_from, min(t.k_len, k_hi + kStep))) {
+#pragma unroll 1
+        for (int walk = kUps; walk < kWalks; walk++) {
+            w.begin(a, t, row, head);
+            w.settle();
+#pragma unroll 1
+            for (int k0 = k_first; k0 < k_hi; k0 += kStride) {
+                request_k(k0);
+                request_v(k0);
+                wait_for_lds_loads();
+#pragma unroll 1
+                for (int i = 8 * lane; i < kTile; i += 512) change_values<T>(vt + i, walk);
+                wait_for_lds_reads();
+                float16_t s[kStep / 32];
+                uint32_t p[2][kStep / 32][8];
+                w.scores_of(kt, walk, s);
+                if (k0 + kStep > see_least) w.mask(s, see - k0);
+                w.weights(s, a.c, w.bound(s, a.c), p);
+                w.product(vt, p);
+                wait_for_lds_reads();
+            }
+            if (walk != kFiniteOnly) w.take_marks(s_marks[walk - kUps] + tid);
+        }
+        w.put_marks(s_marks[0] + tid, s_marks[1] + tid);
+    }
 
     // the waves join: sums to where K and V were, row by row (four floats of padding where there is room: rows on different banks)
     float *mine = reinterpret_cast<float *>(kt);
-    const bool odd = w.odd();
-    if (!masked) before = odd;
     const float l = halves_sum(w.l);
-    const uint32_t odds = (uint32_t)__ballot(odd), seen = (uint32_t)__ballot(before);
-    if (lane == 0) {
-        s_odd[wave] = odds;
-        s_seen[wave] = seen;
-    }
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
 #pragma unroll
@@ -654,12 +757,10 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
         s_ml[wave][col][1] = l;
     }
     __syncthreads();
-    const uint32_t redo = (s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3]) & ~(s_seen[0] | s_seen[1] | s_seen[2] | s_seen[3]);
     constexpr int kRowChunks = HD / 8;
     for (int i = tid; i < kNarrowRows * kRowChunks; i += kPromptThreads) {
         const int r = i / kRowChunks, d = i % kRowChunks * 8;
         if (t.row0 + r >= t.q_end) break;
-        if (redo >> r & 1) continue;
         const float M = fmaxf(fmaxf(s_ml[0][r][0], s_ml[1][r][0]), fmaxf(s_ml[2][r][0], s_ml[3][r][0]));
         float den = 0.f, num[8];
 #pragma unroll
@@ -687,8 +788,6 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
             make_uint4(T::pack(num[0] * inv, num[1] * inv), T::pack(num[2] * inv, num[3] * inv), T::pack(num[4] * inv, num[5] * inv), T::pack(num[6] * inv, num[7] * inv));
         if (a.lse && d == 0) a.lse[at] = den == 0.f ? -INFINITY : (M + log2f(den)) * 0.693147180559945f;
     }
-    const uint32_t which = uniform((int)(redo >> (8 * wave) & 0xFFu));
-    if (which) prompt_rows_plain<HD, T>(a, t, t.row0 + 8 * wave, which, head, kvh, k_lo, k_hi, split);
 }
 
 // Joins the pieces of a row, a workgroup per (row, head), for more pieces than the kernel below takes.  The rows are found as the kernel above found them: rows of no
