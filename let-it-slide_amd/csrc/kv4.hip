@@ -397,7 +397,7 @@ __global__ __launch_bounds__(64 * kKv4Waves<HD>, HD > 128 ? 2 : 4) void kv4_attn
     uint8_t *ring = lds4 + wave * (kKv4Stages * 2 * kStage);
     const uint32_t ring_to = lds_address(ring);
     auto request = [&](int i) {
-        const int j0 = first + i * kWaves * kKv4Tile, bytes = min(kStage, (hi - j0) * kRow);
+        const int j0 = first + i * kWaves * kKv4Tile, bytes = min(kKv4Tile, hi - j0) * kRow;
         const int4_t kr = buffer_resource(k_base + (int64_t)j0 * kRow, bytes), vr = buffer_resource(v_base + (int64_t)j0 * kRow, bytes);
         const uint32_t to = ring_to + (uint32_t)(i % kKv4Stages) * (2u * kStage);
 #pragma unroll
