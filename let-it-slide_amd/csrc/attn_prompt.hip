@@ -299,8 +299,9 @@ struct PromptWave {
 #pragma unroll
             for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[h][r]);
         mx = halves_max(mx) * scale;
-        if (__ballot(mx > m + kLazy)) {
-            const float up = fmaxf(m, mx);
+        const bool raise = mx > m + kLazy;                 // (each row by itself: its bits do not depend on the wave's others)
+        if (__ballot(raise)) {
+            const float up = raise ? mx : m;
             const float f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - up);
             l *= f;
 #pragma unroll
