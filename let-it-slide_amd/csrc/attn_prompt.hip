@@ -4,7 +4,8 @@
 //   o_i = sum_j p_ij v_j / l_i,   p_ij = exp2(c q_i.k_j - m_i),   l_i = sum_j p_ij,   lse_i = (m_i + log2 l_i) ln 2
 //
 // with c = scale log2(e), over the keys j that query i sees, in one pass over the keys: m_i is a running bound of
-// c q_i.k_j (raised, and the sums rescaled, only where a score exceeds it by more than 2^8, so p stays below 256).
+// c q_i.k_j (raised, and the sums rescaled, only where a score exceeds it by more than 2^8, so p stays below 256; in fp16 all of
+// them times 2^7, which the quotient takes off again).
 // Scores, m, l and the output sums are fp32; p is rounded to the inputs' type for the matrix unit (by at most
 // 2^-11 of it in fp16, 2^-8 in bf16: the products need two operands of one type), l adds the unrounded p.
 //
@@ -50,6 +51,9 @@ struct TypeF16 {
     }
     static __device__ __forceinline__ float to_float(uint16_t b) { return half_bits_to_float(b); }
     static constexpr short kExponent = 0x7C00;
+    // weights carry a factor 2^7: a weight far below the largest is held to 2^-31 of it instead of 2^-24 (many such ones behind one that outweighs
+    // them would otherwise be lost), and the largest, 2^15, stays below 65504.  bf16 has fp32's exponents
+    static constexpr float kWeightLog2 = 7.f, kWeightInverse = 0x1p-7f;
     // sum + 0 x for two values x: not a number where one of them is no finite number
     static __device__ __forceinline__ float zero_of(uint32_t w, float sum)
     {
@@ -68,6 +72,7 @@ struct TypeBf16 {
     }
     static __device__ __forceinline__ float to_float(uint16_t b) { return __builtin_bit_cast(float, (uint32_t)b << 16); }
     static constexpr short kExponent = 0x7F80;
+    static constexpr float kWeightLog2 = 0.f, kWeightInverse = 1.f;
     static __device__ __forceinline__ float zero_of(uint32_t w, float sum)
     {
         return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), (bf16x2_t)((__bf16)0.f), sum, false);
@@ -308,7 +313,7 @@ struct PromptWave {
             for (int d = 0; d < kDims; d++) acc[d] *= f;
             m = up;
         }
-        return m == -INFINITY ? 0.f : m;
+        return (m == -INFINITY ? 0.f : m) - T::kWeightLog2;
     }
     // p = exp2(c s - bound), packed in pairs of keys
     __device__ __forceinline__ void weights(const float16_t (&s)[kBlocks], float scale, float off, uint32_t (&p)[TERMS][kBlocks][8])
@@ -582,7 +587,7 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
                 if (row < t.q_end)
                     *reinterpret_cast<uint4 *>(o + 32 * d + 8 * b) = make_uint4((uint32_t)w0[0], (uint32_t)w1[0], (uint32_t)w0[1], (uint32_t)w1[1]);
             }
-        if (a.lse && c == 0 && row < t.q_end) a.lse[(int64_t)row * a.heads + head] = l == 0.f ? -INFINITY : (w.m + log2f(l)) * 0.693147180559945f;
+        if (a.lse && c == 0 && row < t.q_end) a.lse[(int64_t)row * a.heads + head] = l == 0.f ? -INFINITY : (w.m + log2f(l * T::kWeightInverse)) * 0.693147180559945f;
     };
     // every wave has said whether to go again, and nobody reads K or V any more; one that need not wait for that has stored its rows
     if (G == 1) finish();
@@ -787,7 +792,7 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
         const float inv = den == 0.f ? 0.f : 1.f / den;
         *reinterpret_cast<uint4 *>(a.out + (int64_t)(t.row0 + r) * a.st.out_token + (int64_t)head * a.st.out_head + d) =
             make_uint4(T::pack(num[0] * inv, num[1] * inv), T::pack(num[2] * inv, num[3] * inv), T::pack(num[4] * inv, num[5] * inv), T::pack(num[6] * inv, num[7] * inv));
-        if (a.lse && d == 0) a.lse[at] = den == 0.f ? -INFINITY : (M + log2f(den)) * 0.693147180559945f;
+        if (a.lse && d == 0) a.lse[at] = den == 0.f ? -INFINITY : (M + log2f(den * T::kWeightInverse)) * 0.693147180559945f;
     }
 }
 
@@ -806,7 +811,7 @@ __global__ __launch_bounds__(kJoinThreads) void attn_prompt_merge_kernel(const P
     const float num = join_pieces(a.part_acc + at * a.splits * HD, a.part_ml + 2 * at * a.splits, a.splits, HD, M, l);
     if (threadIdx.x < HD)
         a.out[(int64_t)row * a.st.out_token + (int64_t)head * a.st.out_head + threadIdx.x] = (uint16_t)T::pack(l == 0.f ? 0.f : num / l, 0.f);
-    if (a.lse && threadIdx.x == 0) a.lse[at] = l == 0.f ? -INFINITY : (M + log2f(l)) * 0.693147180559945f;
+    if (a.lse && threadIdx.x == 0) a.lse[at] = l == 0.f ? -INFINITY : (M + log2f(l * T::kWeightInverse)) * 0.693147180559945f;
 }
 
 // The same for at most kFewPieces pieces: a wave per (row, head), eight pieces asked for at once (2300 rows of 8 heads in two pieces: 6 us
@@ -866,7 +871,7 @@ __global__ __launch_bounds__(256) void attn_prompt_merge_few_kernel(const Prompt
             for (int u = 0; u + 1 < kEach; u += 2) *reinterpret_cast<uint32_t *>(o + u) = T::pack(num[u] * inv, num[(u + 1) % kEach] * inv);
         }
     }
-    if (a.lse && lane == 0) a.lse[at] = den == 0.f ? -INFINITY : (M + log2f(den)) * 0.693147180559945f;
+    if (a.lse && lane == 0) a.lse[at] = den == 0.f ? -INFINITY : (M + log2f(den * T::kWeightInverse)) * 0.693147180559945f;
 }
 
 template <int HD, int G>

@@ -53,3 +53,22 @@ def test_a_row_keeps_its_bits_whatever_the_others_are(rk, n, L, heads, kvh, hd, 
         out2, lse2 = attend(q2)
         others = torch.arange(n, device="cuda") % 8 != 3
         assert torch.equal(out[others], out2[others]) and torch.equal(lse[others], lse2[others])
+
+
+@pytest.mark.parametrize("n,L,heads,kvh,hd", [(7, 16384, 4, 4, 64), (64, 16384, 32, 32, 64), (2048, 16384, 16, 16, 64), (300, 8192, 8, 8, 128)])
+def test_many_weights_far_below_the_largest(rk, n, L, heads, kvh, hd):
+    """The first key outweighs each other one by 2^26 (as the first token of a trained model's context may) and has a value of 0, the others
+    of 1: an output is what those weigh together, m / (2^26 + m) with m of them seen.  The scores are hd (exact) and 0, the scale makes the
+    one 26 ln 2 to 26 * 2^-23.  fp16 weights are multiples of 2^-24; with the largest at 2^7 at least the others are 32 of those.  Tolerance: the output's half step, the scores' fp32 roundings
+    (3 E of the output, E = 18.1 (hd + 4) 2^-24), fp32 sums of at most 2^14 terms of which a lane adds 2^13 (2^-11)."""
+    scale = 26 * math.log(2) / hd
+    q = torch.ones(n, heads, hd, dtype=F16, device="cuda")
+    k, v = torch.zeros(L, kvh, hd, dtype=F16, device="cuda"), torch.ones(L, kvh, hd, dtype=F16, device="cuda")
+    k[0], v[0] = 1, 0
+    out, lse = torch.empty_like(q), torch.empty(n, heads, device="cuda")
+    rk.attn_prompt(q, k, v, out, q_start=ints([0, n]), k_start=ints([0]), k_len=ints([L]), scale=scale, lse=lse, timed=False)
+    rest = (torch.arange(n, device="cuda", dtype=torch.float64) + L - n) * 2.0 ** -26
+    want = (rest / (1 + rest))[:, None, None]
+    E = 18.1 * (hd + 4) * 2.0 ** -24
+    assert bool(((out.double() - want).abs() <= want * (2.0 ** -11 + 3 * E + 2.0 ** -11) + 2.0 ** -25).all()), float(((out.double() - want).abs() / want).max())
+    assert bool(((lse.double() - hd * scale - torch.log1p(rest)[:, None]).abs() <= 2 * E + 2.0 ** -21 * 20).all())
