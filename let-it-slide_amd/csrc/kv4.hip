@@ -356,6 +356,9 @@ __device__ __forceinline__ float rows_sum(float x)
 
 constexpr int kKv4Stages = 2;               // of them on their way or in LDS
 constexpr float kKv4Lazy = 8.f;
+// weights carry a factor 2^7, which the quotient takes off again: one far below the largest is held to 2^-31 of it instead of 2^-24 (many such
+// ones behind one that outweighs them would otherwise be lost), and the largest, 2^15, stays below 65504
+constexpr float kKv4WeightLog2 = 7.f;
 template <int HD>
 constexpr int kKv4Waves = HD > 128 ? 4 : 8;
 template <int HD>
@@ -488,7 +491,7 @@ __global__ __launch_bounds__(64 * kKv4Waves<HD>, HD > 128 ? 2 : 4) void kv4_attn
             for (int e = 0; e < kE; e++) acc[e] *= f;
             m = up;
         }
-        const float mc = m == -INFINITY ? 0.f : m;
+        const float mc = (m == -INFINITY ? 0.f : m) - kKv4WeightLog2;
         half2_t p2[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {

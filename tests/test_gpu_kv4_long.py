@@ -1,4 +1,6 @@
 """rptc_kernels.kv4_attn_decode over caches of very many positions."""
+import math
+
 import pytest
 import torch
 
@@ -52,3 +54,22 @@ def test_pieces_of_more_than_four_gib_behind_a_tile(rk):
     for s in range(2):
         for i in range(2):
             assert torch.equal(out[s, i::2], want[2 * i + s].expand(heads // 2, hd)), (s, i)
+
+
+@pytest.mark.parametrize("heads,kvh,seqs", [(4, 4, 256), (32, 2, 512)])
+def test_many_weights_far_below_the_largest(rk, heads, kvh, seqs):
+    """A key in front that outweighs each other one by 2^26, as the first token of a trained model's context may, with a value of 0, and
+    values of 1 behind it: the output is what the others weigh together, (n - 1) / (2^26 + n - 1).  The scores are hd (exact) and 0, the
+    scale makes the one 26 ln 2 to 26 * 2^-23.  An fp16 weight is a multiple of 2^-24; with the largest at 2^7 at least, the
+    others are 32 of those.  Tolerance: the output's half step, the scores' fp32 roundings (E = 18.1 (hd + 4) 2^-24, 3 E of the output),
+    fp32 sums of 2^11 terms behind each other (2^-13)."""
+    hd, n = 64, 16384
+    kc, vc = rk.kv4_cache(seqs, kvh, n, hd)
+    par = torch.tensor([0.0, 1.0], dtype=torch.float16, device="cuda").view(torch.uint8).repeat(hd // 32)      # scale 0, minimum 1
+    kc[:, :, 0, hd // 2:], vc[:, :, 1:, hd // 2:] = par, par
+    q = torch.ones(seqs, heads, hd, dtype=torch.float16, device="cuda")
+    out = torch.empty_like(q)
+    rk.kv4_attn_decode(q, kc, vc, i64([n - 1] * seqs), out, scale=26 * math.log(2) / hd, timed=False)
+    rest = (n - 1) * 2.0 ** -26
+    want = rest / (1 + rest)
+    assert bool(((out.double() - want).abs() <= want * (2.0 ** -11 + 3 * 18.1 * (hd + 4) * 2.0 ** -24 + 2.0 ** -13) + 2.0 ** -25).all()), (want, float(out.min()), float(out.max()))
