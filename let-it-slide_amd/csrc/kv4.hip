@@ -230,8 +230,10 @@ __global__ __launch_bounds__(256) void kv4_rope_append_kernel(const uint16_t *__
 // words as the row operand; its result has, in a lane, scores of one head for four positions of each of two tiles, which is,
 // with the positions renumbered accordingly, the operand P of O^T = V^T P^T; V^T's operand wants eight positions of one
 // dimension in a lane, so the lane reads one word (eight dimensions) of its eight rows and pairs the positions up with byte
-// permutes.  Values are formed in fp16, as stored; p enters the product rounded to fp16, and, where half of the
-// columns are free, what that left enters through them.
+// permutes.  Values are formed in fp16, as stored; p enters the product rounded to fp16, and what that left enters as well:
+// through the free columns with at most eight heads, by a second product with more (one term alone: error 1.32 to 1.39 times that of the
+// output's own rounding instead of 1.00, for
+// 0 to 6 % of the time: 32 sequences of 3000, 32 / 2 heads x 128, 19.9 us, 8 of 2000, 48 / 4 x 256, 30.1 -> 31.6).
 // The 32 rows are a run of memory, and come straight into LDS, two stages a wave in flight (10 KB of them at hd 128, up to
 // 160 KB a compute unit); the row length in words (20 at hd 128) puts the lanes of every LDS read on different banks.
 // The matrix unit is mostly idle (15 of 16 columns with one query head a key head); what counts is the vector unit's work of
@@ -492,7 +494,7 @@ __global__ __launch_bounds__(64 * kKv4Waves<HD>, HD > 128 ? 2 : 4) void kv4_attn
             m = up;
         }
         const float mc = (m == -INFINITY ? 0.f : m) - kKv4WeightLog2;
-        half2_t p2[4];
+        half2_t p2[4], rest[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int r = 2 * j;
@@ -502,7 +504,8 @@ __global__ __launch_bounds__(64 * kKv4Waves<HD>, HD > 128 ? 2 : 4) void kv4_attn
             const float2v_t xy = {x, y};
             p2[j] = __builtin_convertvector(xy, half2_t);
             const float2v_t left_over = {x - (float)p2[j].x, y - (float)p2[j].y};
-            p2[j] = second ? __builtin_convertvector(left_over, half2_t) : p2[j];
+            rest[j] = __builtin_convertvector(left_over, half2_t);
+            p2[j] = second ? rest[j] : p2[j];
         }
         const half8v_t p = as_half8(p2);
         // V: the same byte of two positions' words side by side, then the nibbles of a dimension of both in one register
@@ -538,6 +541,11 @@ __global__ __launch_bounds__(64 * kKv4Waves<HD>, HD > 128 ? 2 : 4) void kv4_attn
         }
 #pragma unroll
         for (int e = 0; e < kE; e++) acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(val[e]), p, acc[e], 0, 0, 0);
+        if (!twice) {                                      // no free columns: a second product
+            const half8v_t left_over = as_half8(rest);
+#pragma unroll
+            for (int e = 0; e < kE; e++) acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_half8(val[e]), left_over, acc[e], 0, 0, 0);
+        }
     }
 
     // The waves join through LDS: lane (column n, quarter c) holds the dimensions 4 kE c .. 4 kE (c + 1) of its column, a run of
