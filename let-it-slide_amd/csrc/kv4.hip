@@ -316,7 +316,7 @@ __device__ __forceinline__ bool kv4_find(const Kv4AttnArgs &a, int slot, bool by
     r.len = r.pieces = r.slot0 = 0;
     for (int s0 = 0; s0 < a.seqs; s0 += 64) {
         if (a.seqs > 64) len = kv4_length(a, s0 + lane);
-        const uint32_t n = min(((uint32_t)(len + kKv4Tile - 1) / kKv4Tile + size - 1) / size, (uint32_t)kJoinMost);
+        const uint32_t n = ((uint32_t)(len + kKv4Tile - 1) / kKv4Tile + size - 1) / size;      // at most a.want of one sequence
         const uint32_t incl = scan64(n);
         const uint64_t hit = __ballot(by_seq ? s0 + lane == slot : in_front + incl > (uint32_t)slot);
         if (hit) {
@@ -644,12 +644,15 @@ struct Kv4Plan {
 // 4 steps of its waves, 2 us) with fewer sequences and heads than compute units, and of 8192 and more up to four times as
 // many, for what one long sequence among short ones would cost.  Pieces are no shorter than 512 positions.  Measured, uncut /
 // cut, heads x 128: one sequence of 1024, 32 heads: 10.4 / 11.3 us; of 8192, 32 heads: 34 / 18; 32 of 2000, 8 heads x 64: 14.4 / 17.3.
+// One key head would take a piece a compute unit, but joining more than 128 costs more than the shorter walks give: one sequence of 131072, one
+// head x 128, 128 / 256 pieces: 19.3 / 22.9 us.
 static Kv4Plan kv4_plan(int64_t seqs, int64_t groups, int64_t max_len, int cus)
 {
     Kv4Plan p = {(int)seqs, 1, 512 / kKv4Tile};
     if (max_len < 2048 || seqs > 1024 || seqs * groups >= (max_len >= 8192 ? 4 : 1) * (int64_t)cus) return p;
     p.want = (int)((cus + groups - 1) / groups);
     if (p.want < 2) p.want = 2;
+    if (p.want > kJoinMost) p.want = kJoinMost;
     p.slots = (int)seqs + p.want - 1;          // pieces of one length: fewer than want whole ones and one more a sequence
     return p;
 }

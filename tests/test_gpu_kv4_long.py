@@ -73,3 +73,25 @@ def test_many_weights_far_below_the_largest(rk, heads, kvh, seqs):
     rest = (n - 1) * 2.0 ** -26
     want = rest / (1 + rest)
     assert bool(((out.double() - want).abs() <= want * (2.0 ** -11 + 3 * 18.1 * (hd + 4) * 2.0 ** -24 + 2.0 ** -13) + 2.0 ** -25).all()), (want, float(out.min()), float(out.max()))
+
+
+@pytest.mark.parametrize("hd,L", [(64, 131072), (128, 140001)])
+def test_one_key_head_in_as_many_pieces_as_are_joined(rk, hd, L):
+    """One long sequence of one key head, cut into as many pieces as are joined, against the formula in 64 bits.  Tolerance: the
+    output's rounding (u |o|, u = 2^-11), the weights' in two fp16 terms (2^-21 A, A = sum p |v|), the scores' (E = scale (hd + 4)
+    2^-24 max sum |q k|, 3 E A), and fp32 sums of n positive terms in groups of at most 2^10 behind each other (2^-13 A)."""
+    heads, most = 4, 128                                      # room for as many pieces as there can be, no more workgroups than these
+    assert rk.library().rptc_kv4_attn_decode_workspace_bytes(1, heads, 1, hd, L) <= heads * most * (hd + 2) * 4
+    kc, vc = rk.kv4_cache(1, 1, L, hd)
+    k, v = randn(1, L, 1, hd), randn(2, L, 1, hd)
+    rk.kv4_append(k, v, kc, vc, i64([0]), timed=False)
+    rk.kv4_read(kc, vc, k, v, timed=False)
+    q = randn(3, 1, heads, hd)
+    for pos in (L - 1, L - 77, 40000):
+        out = torch.empty_like(q)
+        rk.kv4_attn_decode(q, kc, vc, i64([pos]), out, timed=False)
+        kd, vd, qd = k[:pos + 1, 0].double(), v[:pos + 1, 0].double(), q[0].double()
+        p = torch.softmax(qd @ kd.t().contiguous() * hd ** -0.5, -1)
+        o, A = p @ vd, p @ vd.abs()
+        E = hd ** -0.5 * (hd + 4) * 2.0 ** -24 * (qd.abs() @ kd.abs().t().contiguous()).amax(-1, keepdim=True)
+        assert bool(((out[0].double() - o).abs() <= 2.0 ** -11 * o.abs() + (2.0 ** -21 + 3 * E + 2.0 ** -13) * A + 2.0 ** -25).all()), pos
