@@ -427,10 +427,10 @@ int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint16_t *v, ui
 /*
  * A key/value cache held in 4 bits.  No counterpart in the reference (it generates with transformers, quantize_hf.py:229-236).
  * k_cache, v_cache: uint8 [seqs][kv_heads][max_len][rptc_kv4_row_bytes(hd)], hd in {32, 64, 128, 256} (a negative status for others).  A row holds hd fp16
- * values in groups of 32: m = min x, s = fp16((max x - min x) / 15), code = clamp(rint((x - m) / s), 0, 15) (0 where s = 0; the
- * quotients in fp32), and stands for fp16(code * s + m).  A group with a value that is no finite number reads as
- * not-a-number.  hd / 2 bytes of codes (word w: values 8w .. 8w+7, nibble t the value 8w + 2t, nibble t + 4 the value
- * 8w + 2t + 1), then (s, m) of every group.
+ * values in groups of 32: m = min x, s = fp16((max x - min x) / 15), or the number below it where fp16(15 s + m) would be infinite, code =
+ * clamp(rint((x - m) / s), 0, 15) (0 where s = 0; the quotients in fp32), and stands for fp16(code * s + m): finite where the group is; a
+ * group with a value that is no finite number reads as not-a-number.  hd / 2 bytes of codes (word w: values 8w .. 8w+7, nibble t the value
+ * 8w + 2t, nibble t + 4 the value 8w + 2t + 1), then (s, m) of every group.
  *   rptc_kv4_append       k, v fp16 [total][kv_heads][hd] by token and head strides (elements, multiples of 8): row t of sequence
  *                         s goes to position pos[s] + t - q_start[s] of cache s.  q_start int32 [seqs + 1] (rows of
  *                         no sequence are skipped), or NULL: total / seqs rows a sequence; pos int64 [seqs]; both device memory.

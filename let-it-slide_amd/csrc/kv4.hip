@@ -2,8 +2,8 @@
 // (No counterpart in the reference, which generates with transformers on dense weights and caches, quantize_hf.py:229-236.)
 //
 // A row is one position of one head, hd fp16 values in groups of 32:
-//   m = min x,  s = fp16((max x - min x) / 15),  code = clamp(rint((x - m) / s), 0, 15) (0 where s = 0),
-//   the value a code stands for = fp16(code * s + m), one rounding
+//   m = min x,  s = fp16((max x - min x) / 15), or the number below it where fp16(15 s + m) would be infinite,
+//   code = clamp(rint((x - m) / s), 0, 15) (0 where s = 0),  the value a code stands for = fp16(code * s + m), one rounding
 // (the quotients in fp32, correctly rounded; a group that holds a value which is no finite number reads as not-a-number).
 // hd / 2 bytes of codes, then s and m of every group: hd / 2 + hd / 8 bytes, 80 against 256 at hd = 128.  Word w of a row
 // holds the values 8w .. 8w+7, nibble t the value 8w + 2t and nibble t + 4 the value 8w + 2t + 1: one mask of a word gives a
@@ -73,9 +73,13 @@ __device__ __forceinline__ void quantize_word(const float (&x)[8], uint32_t &cod
         par = 0x7E007E00u;
         return;
     }
-    const uint16_t sb = float_to_half_bits((hi - lo) / 15.f);
+    uint16_t sb = float_to_half_bits((hi - lo) / 15.f);
+    const uint16_t mb = float_to_half_bits(lo);
+    // the scale's rounding may take the largest code past 65504: the scale below it does not
+    const _Float16 top = __builtin_elementwise_fma((_Float16)15.f, __builtin_bit_cast(_Float16, sb), __builtin_bit_cast(_Float16, mb));
+    if (__builtin_bit_cast(uint16_t, top) == 0x7C00u) sb--;
     const float s = half_bits_to_float(sb);
-    par = (uint32_t)float_to_half_bits(lo) << 16 | sb;
+    par = (uint32_t)mb << 16 | sb;
     if (s == 0.f) return;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
