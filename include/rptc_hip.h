@@ -400,7 +400,8 @@ int64_t rptc_lite_viterbi_scratch_bytes(int L, int R, int64_t rows, int64_t step
  * rows [q_start[s], q_start[s+1]) and the key rows [k_start[s], k_start[s] + k_len[s]); with causal != 0 query i of Lq sees
  * the keys j <= i + Lk - Lq (the last query sees all: a chunk at the end of a context), else all Lk.
  *   out[i] = softmax(scale * q[i] . K^T) V,  lse[i] = log sum exp(scale * q[i] . K^T)  (lse float [total_q][heads], may be NULL)
- * A query that sees no key gets out = 0, lse = -inf.  What a query does not see does not reach it, not-a-number included.
+ * A query that sees no key, or none with a score above -inf, gets out = 0, lse = -inf.  What a query does not see does not reach
+ * it, not-a-number included.
  * Rows of q outside every sequence, and sequences whose rows lie outside q or k (checked on the device), are left unwritten.
  *   q [total_q][heads][hd], k, v [total_k][kv_heads][hd], out as q, by token and head strides in elements (multiples of
  *   8, tokens at most 2^23 apart; a key cache [kv_heads][positions][hd] has k_token = hd, k_head = positions * hd); head h reads
@@ -434,7 +435,7 @@ int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint16_t *v, ui
  *   rptc_kv4_append       k, v fp16 [total][kv_heads][hd] by token and head strides (elements, multiples of 8): row t of sequence
  *                         s goes to position pos[s] + t - q_start[s] of cache s.  q_start int32 [seqs + 1] (rows of
  *                         no sequence are skipped), or NULL: total / seqs rows a sequence; pos int64 [seqs]; both device memory.
- *                         Rows whose position lies outside [0, max_len) are not written.
+ *                         Rows whose position is max_len or more are not written; of a sequence with a negative pos (padding) none is.
  *   rptc_kv4_read         the first `rows` positions of every sequence as fp16: k, v [seqs * rows][kv_heads][hd] by strides
  *   rptc_kv4_rope_append  one token per sequence: qkv [seqs][(heads + 2 kv_heads) * hd] = [q | k | v]; rotates the (2i, 2i+1)
  *                         pairs of q and k by cos/sin [max_len][hd/2] at pos[s] as rptc_rope_cache does, writes q_out

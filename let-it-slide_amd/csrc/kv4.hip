@@ -127,7 +127,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4AppendArgs a)
         start = seq * a.rows_each;
     }
     const int64_t first = a.pos[seq];
-    // a position outside the cache is not written
+    // a sequence that begins outside the cache is not written, nor what lies past its end
     if (first < 0 || first >= a.max_len) return;
     const int64_t p = first + ((int64_t)token - start);
     if (p >= a.max_len) return;

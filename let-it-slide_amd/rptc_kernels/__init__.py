@@ -854,8 +854,9 @@ def attn_prompt(q, k, v, out, q_start=None, k_start=None, k_len=None, causal=Tru
     k_len[s] key rows from k_start[s] on (int32 tensors on the device).  Without k_start / k_len the keys lie as the
     queries do; without q_start there is one sequence.  ``causal``: query i of Lq sees the keys j <= i + Lk - Lq, so a
     chunk's last query sees the whole context.  ``scale`` defaults to hd ** -0.5.  ``lse`` (float32 [Tq, heads], optional)
-    takes the logarithm of every row's sum.  A query that sees no key gets 0 (lse -inf); rows outside every sequence stay as
-    they are.  ``max_k``: an upper bound of k_len where the key rows are many more (a cache's positions).  Returns elapsed ms."""
+    takes the logarithm of every row's sum.  A query that sees no key, or none with a score above -inf, gets 0 (lse -inf);
+    rows outside every sequence stay as they are.  ``max_k``: an upper bound of k_len where the key rows are many more (a
+    cache's positions).  Returns elapsed ms."""
     return (_bindings or _load_bindings()).attn_prompt(q, k, v, out, q_start, k_start, k_len, causal, scale, lse, max_k,
                                                        _timing if timed is None else timed)
 
@@ -877,7 +878,7 @@ def kv4_append(k, v, k_cache, v_cache, pos, q_start=None, timed=None):
     """Put the rows k, v (fp16 [tokens, kv_heads, hd], strides as in ``attn_prompt``) into the 4-bit caches of
     ``kv4_cache``: sequence s's rows q_start[s] .. q_start[s+1] go to positions pos[s], pos[s] + 1, ... of cache s (int32 and
     int64 tensors on the device; without q_start every sequence has tokens / seqs rows).  Rows that do not fit are
-    not written.  Returns elapsed ms."""
+    not written, nor any of a sequence whose pos is negative (padding).  Returns elapsed ms."""
     return (_bindings or _load_bindings()).kv4_append(k, v, k_cache, v_cache, pos, q_start, _timing if timed is None else timed)
 
 

@@ -72,3 +72,20 @@ def test_many_weights_far_below_the_largest(rk, n, L, heads, kvh, hd):
     E = 18.1 * (hd + 4) * 2.0 ** -24
     assert bool(((out.double() - want).abs() <= want * (2.0 ** -11 + 3 * E + 2.0 ** -11) + 2.0 ** -25).all()), float(((out.double() - want).abs() / want).max())
     assert bool(((lse.double() - hd * scale - torch.log1p(rest)[:, None]).abs() <= 2 * E + 2.0 ** -21 * 20).all())
+
+
+@pytest.mark.parametrize("n,L,heads,kvh,hd", FORMS)
+def test_rows_whose_scores_are_all_minus_infinity(rk, n, L, heads, kvh, hd):
+    # every key a row sees has a product of -infinity with it: no weight at all, as for a row that sees no key; its neighbours as ever
+    q, k, v = randn(1, n, heads, hd), randn(2, L, kvh, hd), randn(3, L, kvh, hd)
+    k[..., 0] = k[..., 0].abs() + 0.1
+    q[..., 0] = 0
+    out, lse = torch.empty_like(q), torch.empty(n, heads, device="cuda")
+    args = dict(q_start=ints([0, n]), k_start=ints([0]), k_len=ints([L]), timed=False)
+    rk.attn_prompt(q, k, v, out, lse=lse, **args)
+    q2, out2, lse2 = q.clone(), torch.empty_like(q), torch.empty_like(lse)
+    q2[5::8, :, 0] = -math.inf
+    rk.attn_prompt(q2, k, v, out2, lse=lse2, **args)
+    none = torch.arange(n, device="cuda") % 8 == 5
+    assert bool((out2[none] == 0).all()) and bool((lse2[none] == -math.inf).all())
+    assert torch.equal(out2[~none], out[~none]) and torch.equal(lse2[~none], lse[~none])
