@@ -85,8 +85,10 @@ struct PromptArgs {
     float *lse;                        // [total_q][heads], may be null
     const int32_t *q_start, *k_start, *k_len;
     float *part_acc, *part_ml;         // splits > 1: [total_q][heads][split][hd] sums, [..][2] bound and sum of p
+    int32_t *first_tile;               // [seqs], may be null: the tiles of the sequences in front of each
     rptc_prompt_strides st;
     int seqs, total_q, total_k, heads, kv_heads, tiles, splits, causal;
+    int row_bits;                      // a tile has 2^row_bits query rows
     float c;                           // scale * log2(e)
 };
 
@@ -95,56 +97,112 @@ struct PromptTile {
     int k_first, k_len;                // and its keys
 };
 
-// The sequence that holds tile `tile` when every sequence is cut into tiles of ROWS query rows: 64 sequences at a time, a
-// lane each.  A sequence's tiles are taken from its end (the longest rows of a causal prompt first).  The starts come from
-// device memory: a sequence that does not lie inside the query rows has no tiles; false for a tile past the last, and
-// for one whose keys do not lie inside k and v (its rows are left as they are).
-template <int ROWS>
+// Sequence s as device memory has it.  One that does not lie inside the query rows has no tiles.
+struct PromptSequence {
+    int begin, end, tiles, k_first, k_len;
+};
+__device__ __forceinline__ PromptSequence prompt_sequence(const PromptArgs &a, int s)
+{
+    PromptSequence r = {0, 0, 0, 0, 0};
+    if (s >= a.seqs) return r;
+    r.begin = a.q_start ? a.q_start[s] : 0;
+    r.end = a.q_start ? a.q_start[s + 1] : a.total_q;
+    r.k_first = a.k_start ? a.k_start[s] : a.q_start ? r.begin : 0;
+    r.k_len = a.k_len ? a.k_len[s] : a.q_start ? r.end - r.begin : a.total_k;
+    if (r.begin >= 0 && r.end > r.begin && r.end <= a.total_q) r.tiles = (r.end - r.begin + (1 << a.row_bits) - 1) >> a.row_bits;
+    return r;
+}
+
+// The sequence that holds tile `tile` when every sequence is cut into tiles of 2^row_bits query rows: 64 sequences at a time, a
+// lane each; of very many sequences by a search for the tile among their first ones, 64 of them at a time.  A sequence's
+// tiles are taken from its end (the longest rows of a causal prompt first).  False for a tile past the last, and for one whose
+// keys do not lie inside k and v (its rows are left as they are).
 __device__ __forceinline__ bool find_tile(const PromptArgs &a, int tile, PromptTile &t)
 {
     const int lane = threadIdx.x & 63;
     t.seq = -1;
     t.q_begin = t.q_end = t.row0 = t.k_first = t.k_len = 0;
-    int in_front = 0;                      // tiles of the sequences in front (they do not overlap: at most a.tiles)
-    for (int s0 = 0; s0 < a.seqs; s0 += 64) {
-        const int s = s0 + lane;
-        int begin = 0, end = 0, kf = 0, kl = 0;
-        if (s < a.seqs) {
-            begin = a.q_start ? a.q_start[s] : 0;
-            end = a.q_start ? a.q_start[s + 1] : a.total_q;
-            kf = a.k_start ? a.k_start[s] : a.q_start ? begin : 0;
-            kl = a.k_len ? a.k_len[s] : a.q_start ? end - begin : a.total_k;
+    int in_front = 0, n = 0;               // tiles of the sequences in front (they do not overlap: at most a.tiles), of the sequence
+    if (a.first_tile) {
+        int s = 0;                         // first_tile[s] <= tile, the last such one in [s, s + range)
+        for (int range = a.seqs; range > 1;) {
+            const int stride = (range + 63) >> 6, at = lane * stride;
+            const bool up_to = at < range && a.first_tile[s + at] <= tile;
+            const int passed = (__builtin_popcountll(__ballot(up_to)) - 1) * stride;
+            s += passed;
+            range = min(stride, range - passed);
         }
-        const bool ok = begin >= 0 && end > begin && end <= a.total_q;
-        const int n = ok ? (end - begin + ROWS - 1) / ROWS : 0;
+        const PromptSequence r = prompt_sequence(a, s);
+        in_front = a.first_tile[s];
+        if (tile - in_front < r.tiles) {
+            t.seq = s;
+            t.q_begin = r.begin;
+            t.q_end = r.end;
+            t.k_first = r.k_first;
+            t.k_len = r.k_len;
+            n = r.tiles;
+        }
+    } else {
+        for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+            const PromptSequence r = prompt_sequence(a, s0 + lane);
+            int incl = r.tiles;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const int o = __shfl_up(incl, off, 64);
+                if (lane >= off) incl += o;
+            }
+            const uint64_t hit = __ballot(in_front + incl > tile);
+            if (hit) {
+                const int f = __builtin_ctzll(hit);
+                n = __builtin_amdgcn_readlane(r.tiles, f);
+                in_front += __builtin_amdgcn_readlane(incl, f) - n;
+                t.seq = s0 + f;
+                t.q_begin = __builtin_amdgcn_readlane(r.begin, f);
+                t.q_end = __builtin_amdgcn_readlane(r.end, f);
+                t.k_first = __builtin_amdgcn_readlane(r.k_first, f);
+                t.k_len = __builtin_amdgcn_readlane(r.k_len, f);
+                break;
+            }
+            in_front += __builtin_amdgcn_readlane(incl, 63);
+        }
+    }
+    if (t.seq < 0) return false;
+    t.seq = uniform(t.seq);
+    t.q_begin = uniform(t.q_begin);
+    t.q_end = uniform(t.q_end);
+    t.row0 = uniform(t.q_begin + ((n - 1 - (tile - in_front)) << a.row_bits));
+    t.k_first = uniform(t.k_first);
+    t.k_len = uniform(t.k_len);
+    return t.k_first >= 0 && t.k_len >= 0 && (int64_t)t.k_first + t.k_len <= a.total_k;
+}
+
+// The tiles of the sequences in front of each, for calls of very many sequences: one workgroup, a thread a sequence at a time.  No more than
+// a.tiles, the tiles there are room for (sequences that overlap, which is not a valid call, may have more).
+constexpr int kTableThreads = 1024;
+__global__ __launch_bounds__(kTableThreads) void attn_prompt_table_kernel(const PromptArgs a)
+{
+    __shared__ int s_waves[kTableThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int in_front = 0;
+    for (int s0 = 0; s0 < a.seqs; s0 += kTableThreads) {
+        const int n = prompt_sequence(a, s0 + tid).tiles;
         int incl = n;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
             const int o = __shfl_up(incl, off, 64);
             if (lane >= off) incl += o;
         }
-        const uint64_t hit = __ballot(in_front + incl > tile);
-        if (hit) {
-            const int f = __builtin_ctzll(hit);
-            const int nf = __builtin_amdgcn_readlane(n, f);
-            const int local = tile - (in_front + __builtin_amdgcn_readlane(incl, f) - nf);
-            t.seq = s0 + f;
-            t.q_begin = __builtin_amdgcn_readlane(begin, f);
-            t.q_end = __builtin_amdgcn_readlane(end, f);
-            t.row0 = t.q_begin + (nf - 1 - local) * ROWS;
-            t.k_first = __builtin_amdgcn_readlane(kf, f);
-            t.k_len = __builtin_amdgcn_readlane(kl, f);
-            break;
+        if (lane == 63) s_waves[wave] = incl;
+        __syncthreads();
+        int before = in_front, all = 0;
+        for (int w = 0; w < kTableThreads / 64; w++) {
+            if (w < wave) before += s_waves[w];
+            all += s_waves[w];
         }
-        in_front += __builtin_amdgcn_readlane(incl, 63);
+        if (s0 + tid < a.seqs) a.first_tile[s0 + tid] = min(before + incl - n, a.tiles);
+        in_front = min(in_front + all, a.tiles);
+        __syncthreads();
     }
-    t.seq = uniform(t.seq);
-    t.q_begin = uniform(t.q_begin);
-    t.q_end = uniform(t.q_end);
-    t.row0 = uniform(t.row0);
-    t.k_first = uniform(t.k_first);
-    t.k_len = uniform(t.k_len);
-    return t.seq >= 0 && t.k_first >= 0 && t.k_len >= 0 && (int64_t)t.k_first + t.k_len <= a.total_k;
 }
 
 // keys a row sees: [0, sees)
@@ -429,7 +487,7 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
     int head, tile, split;
     prompt_item(a, head, tile, split);
     PromptTile t;
-    if (!find_tile<kRows>(a, tile, t)) return;
+    if (!find_tile(a, tile, t)) return;
     const int kvh = head / (a.heads / a.kv_heads);
 
     const int k_most = uniform(prompt_sees(a, t, min(t.row0 + kRows, t.q_end) - 1));    // of the tile's last row: the most
@@ -647,7 +705,7 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
     int head, tile, split;
     prompt_item(a, head, tile, split);
     PromptTile t;
-    if (!find_tile<kNarrowRows>(a, tile, t)) return;
+    if (!find_tile(a, tile, t)) return;
     const int kvh = head / (a.heads / a.kv_heads);
     const int k_most = uniform(prompt_sees(a, t, min(t.row0 + kNarrowRows, t.q_end) - 1));
     const int per_split = ((k_most + a.splits - 1) / a.splits + kStep - 1) / kStep * kStep;
@@ -803,8 +861,8 @@ __global__ __launch_bounds__(kJoinThreads) void attn_prompt_merge_kernel(const P
 {
     const int head = blockIdx.y;
     PromptTile t;
-    if (!find_tile<kNarrowRows>(a, blockIdx.x / kNarrowRows, t)) return;
-    const int row = t.row0 + blockIdx.x % kNarrowRows;
+    if (!find_tile(a, blockIdx.x >> a.row_bits, t)) return;
+    const int row = t.row0 + (blockIdx.x & ((1 << a.row_bits) - 1));
     if (row >= t.q_end) return;
     const int64_t at = (int64_t)row * a.heads + head;
     float M, l;
@@ -825,8 +883,8 @@ __global__ __launch_bounds__(256) void attn_prompt_merge_few_kernel(const Prompt
     const int lane = threadIdx.x & 63, head = blockIdx.y * 4 + uniform((int)threadIdx.x >> 6);
     if (head >= a.heads) return;
     PromptTile t;
-    if (!find_tile<kNarrowRows>(a, blockIdx.x / kNarrowRows, t)) return;
-    const int row = t.row0 + blockIdx.x % kNarrowRows;
+    if (!find_tile(a, blockIdx.x >> a.row_bits, t)) return;
+    const int row = t.row0 + (blockIdx.x & ((1 << a.row_bits) - 1));
     if (row >= t.q_end) return;
     const int64_t at = (int64_t)row * a.heads + head;
     const int dim = kEach * lane % HD;
@@ -946,6 +1004,21 @@ static PromptPlan prompt_plan(int64_t seqs, int64_t total_q, int64_t total_k, in
     return best;
 }
 
+// More sequences than this are looked up in a table that a launch in front works out: a workgroup's walk over all of them grows with their
+// square.  Walk / table, us: 128 sequences of 5 rows, 32 / 8 heads x 128: 46 / 45; 200 of 30, 8 heads x 64: 14.2 / 14.7; 256 of 30, 32 / 8
+// heads x 128: 114 / 93; 4096 of 30, 8 heads x 64: 1082 / 223.
+constexpr int64_t kTableSeqs = 128;
+
+// The workspace: the pieces' sums and bounds, then the table.
+struct PromptRoom {
+    int64_t sums, bounds, table;           // bytes, multiples of 16
+};
+static PromptRoom prompt_room(const PromptPlan &plan, int64_t seqs, int64_t total_q, int64_t heads, int64_t hd)
+{
+    const int64_t parts = plan.splits > 1 ? plan.splits * total_q * heads : 0;
+    return {parts * hd * 4, (parts * 8 + 15) / 16 * 16, seqs > kTableSeqs ? (seqs * 4 + 15) / 16 * 16 : 0};
+}
+
 static int prompt_sizes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads, int64_t hd)
 {
     if (seqs < 1 || total_q < 1 || total_k < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0) return RPTC_ESHAPE;
@@ -958,6 +1031,7 @@ static int prompt_sizes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t 
 template <int HD, class T>
 static void launch_prompt(const PromptArgs &a, int rows, hipStream_t s)
 {
+    if (a.first_tile) hipLaunchKernelGGL(attn_prompt_table_kernel, dim3(1), dim3(kTableThreads), 0, s, a);
     const dim3 grid((unsigned)(a.heads * a.tiles * a.splits));
     if (rows == kWideRows) {
         hipLaunchKernelGGL((attn_prompt_kernel<HD, T, 1>), grid, dim3(kPromptThreads), (prompt_lds<HD, 1>()), s, a);
@@ -966,9 +1040,9 @@ static void launch_prompt(const PromptArgs &a, int rows, hipStream_t s)
     if (rows == kWideRows / 2) hipLaunchKernelGGL((attn_prompt_kernel<HD, T, 2>), grid, dim3(kPromptThreads), (prompt_lds<HD, 2>()), s, a);
     else hipLaunchKernelGGL((attn_prompt_narrow_kernel<HD, T>), grid, dim3(kPromptThreads), narrow_lds<HD>(), s, a);
     if (a.splits == 1) return;
-    const unsigned rows32 = (unsigned)prompt_tiles(a.seqs, a.total_q, kNarrowRows) * kNarrowRows;
-    if (a.splits <= kFewPieces) hipLaunchKernelGGL((attn_prompt_merge_few_kernel<HD, T>), dim3(rows32, (unsigned)(a.heads + 3) / 4), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attn_prompt_merge_kernel<HD, T>), dim3(rows32, (unsigned)a.heads), dim3(kJoinThreads), 0, s, a);
+    const unsigned tile_rows = (unsigned)a.tiles << a.row_bits;
+    if (a.splits <= kFewPieces) hipLaunchKernelGGL((attn_prompt_merge_few_kernel<HD, T>), dim3(tile_rows, (unsigned)(a.heads + 3) / 4), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_prompt_merge_kernel<HD, T>), dim3(tile_rows, (unsigned)a.heads), dim3(kJoinThreads), 0, s, a);
 }
 
 }  // namespace rptc
@@ -982,8 +1056,9 @@ extern "C" int64_t rptc_attn_prompt_workspace_bytes(int64_t seqs, int64_t total_
     if (rc) return rc;
     DeviceInfo *dev;
     if ((rc = device_info(&dev))) return rc < 0 ? rc : RPTC_EDEVICE;
-    const int splits = prompt_plan(seqs, total_q, total_k, heads, hd, max_k < total_k ? max_k : total_k, dev->cus).splits;
-    return splits > 1 ? (int64_t)splits * total_q * heads * (hd + 2) * 4 : 0;
+    const PromptPlan plan = prompt_plan(seqs, total_q, total_k, heads, hd, max_k < total_k ? max_k : total_k, dev->cus);
+    const PromptRoom room = prompt_room(plan, seqs, total_q, heads, hd);
+    return room.sums + room.bounds + room.table;
 }
 
 extern "C" int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint16_t *v, uint16_t *out, float *lse,
@@ -1030,14 +1105,20 @@ extern "C" int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint
     a.splits = plan.splits;
     a.causal = causal ? 1 : 0;
     a.c = scale * 1.44269504088896f;
+    a.row_bits = __builtin_ctz((unsigned)plan.rows);
     a.part_acc = a.part_ml = nullptr;
-    if (a.splits > 1) {
-        const int64_t n = (int64_t)a.splits * total_q * heads;
+    a.first_tile = nullptr;
+    const PromptRoom room = prompt_room(plan, seqs, total_q, heads, hd);
+    if (const int64_t need = room.sums + room.bounds + room.table) {
         if (!workspace) return RPTC_ENULL;
         if (!aligned16(workspace)) return RPTC_EALIGN;
-        if (workspace_bytes < n * (hd + 2) * 4) return RPTC_ESHAPE;
-        a.part_acc = static_cast<float *>(workspace);
-        a.part_ml = a.part_acc + n * hd;
+        if (workspace_bytes < need) return RPTC_ESHAPE;
+        char *p = static_cast<char *>(workspace);
+        if (room.sums) {
+            a.part_acc = reinterpret_cast<float *>(p);
+            a.part_ml = reinterpret_cast<float *>(p + room.sums);
+        }
+        if (room.table) a.first_tile = reinterpret_cast<int32_t *>(p + room.sums + room.bounds);
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
     Timer timer;
