@@ -471,7 +471,7 @@ int rptc_kv4_attn_decode(const uint16_t *q, const uint8_t *k_cache, const uint8_
  *   entropy       float [rows], nats
  *   top_ids       int64 [rows][top], top_logprobs float [rows][top]: the `top` largest logits of a row in falling order, equal
  *                 ones by the lowest id (a not-a-number counts as -inf); top <= 64 and <= vocab
- * Each output may be NULL (top == 0 without the last two), none may overlap the logits.  fp32 inside.  A row that holds +inf or a not-a-number, or nothing
+ * Each output may be NULL (top == 0 without the last two), none may overlap the logits, the tokens or another one.  fp32 inside.  A row that holds +inf or a not-a-number, or nothing
  * but -inf, has not-a-number for probabilities and entropy.
  */
 int rptc_token_logprobs(const void *logits, int dtype, const int64_t *tokens, float *logprob, float *entropy, int64_t *top_ids,

@@ -354,12 +354,14 @@ extern "C" int rptc_token_logprobs(const void *logits, int dtype, const int64_t 
     if (rows >= (int64_t)1 << 22 || vocab >= (int64_t)1 << 30 || row_stride >= (int64_t)1 << 34 || top > kScoreGroups) return RPTC_ELIMIT;
     const int64_t width = dtype == RPTC_F32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(logits) % width != 0) return RPTC_EALIGN;
-    const int64_t bytes = ((rows - 1) * row_stride + vocab) * width;
-    auto inside = [&](const void *out, int64_t out_bytes) {
-        const char *lo = static_cast<const char *>(logits), *o = static_cast<const char *>(out);
-        return out && o < lo + bytes && lo < o + out_bytes;
-    };
-    if (inside(logprob, rows * 4) || inside(entropy, rows * 4) || inside(top_ids, rows * top * 8) || inside(top_logprobs, rows * top * 4)) return RPTC_EALIAS;
+    // what is read, then what is written: an output overlaps neither the one nor another
+    const struct { const void *p; int64_t bytes; } part[6] = {{logits, ((rows - 1) * row_stride + vocab) * width}, {tokens, rows * 8},
+                                                              {logprob, rows * 4}, {entropy, rows * 4}, {top_ids, rows * top * 8}, {top_logprobs, rows * top * 4}};
+    for (int i = 2; i < 6; i++)
+        for (int j = 0; j < i; j++) {
+            const char *x = static_cast<const char *>(part[i].p), *y = static_cast<const char *>(part[j].p);
+            if (x && y && x < y + part[j].bytes && y < x + part[i].bytes) return RPTC_EALIAS;
+        }
     DeviceInfo *dev;
     int rc = device_info(&dev);
     if (rc) return rc;

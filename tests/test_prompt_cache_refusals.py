@@ -1,0 +1,33 @@
+"""Calls of the prompt attention, the 4-bit cache and the token log probabilities that are refused, or are not, before a device is
+touched: by the C ABI's statuses (no pointer here is ever read)."""
+import ctypes
+
+import pytest
+import torch
+
+import rptc_kernels as rk
+
+ESHAPE, EALIAS = -2, -7
+REFUSED = (-1, -2, -3, -4, -5, -7)              # every status of the checks in front of the device's
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return rk.library()
+
+
+def logprobs(lib, logits=1 << 16, tokens=1 << 30, logprob=None, entropy=None, ids=None, tops=None, rows=4, vocab=1000, top=0):
+    return lib.rptc_token_logprobs(logits, 0, tokens, logprob, entropy, ids, tops, rows, vocab, vocab, top, None, None)
+
+
+def test_scores_over_the_tokens_or_over_each_other(lib):
+    t, a = 1 << 30, 1 << 31
+    assert logprobs(lib, tokens=t, logprob=t) == EALIAS and logprobs(lib, tokens=t, logprob=t + 28) == EALIAS
+    assert logprobs(lib, tokens=t, logprob=a, entropy=t - 12) == EALIAS and logprobs(lib, tokens=t, ids=t, top=1) == EALIAS
+    assert logprobs(lib, logprob=a, entropy=a) == EALIAS and logprobs(lib, logprob=a, entropy=a + 12) == EALIAS
+    assert logprobs(lib, logprob=a, ids=a - 8 * 4 * 3 + 4, top=3) == EALIAS and logprobs(lib, entropy=a, tops=a + 15, top=2) == EALIAS
+    assert logprobs(lib, ids=a, tops=a + 8 * 4 * 2 - 4, top=2) == EALIAS
+    # side by side they are not
+    for call in (dict(tokens=t, logprob=t + 32), dict(tokens=t, logprob=t - 16), dict(logprob=a, entropy=a + 16), dict(ids=a, tops=a + 64, top=2)):
+        if not torch.cuda.is_available():
+            assert logprobs(lib, **call) not in (0,) + REFUSED
