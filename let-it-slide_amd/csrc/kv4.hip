@@ -720,6 +720,7 @@ extern "C" int rptc_kv4_read(const uint8_t *k_cache, const uint8_t *v_cache, uin
     int rc = kv4_sizes(seqs, kv_heads, hd, max_len);
     if (rc) return rc;
     if (rows < 1 || rows > max_len || k_token < 0 || k_head < 0 || v_token < 0 || v_head < 0) return RPTC_ESHAPE;
+    if ((seqs * rows > 1 && (k_token == 0 || v_token == 0)) || (kv_heads > 1 && (k_head == 0 || v_head == 0))) return RPTC_ESHAPE;      // rows over rows
     if (!aligned16(k) || !aligned16(v) || !aligned16(k_cache) || !aligned16(v_cache)) return RPTC_EALIGN;
     if (k_token % 8 || k_head % 8 || v_token % 8 || v_head % 8) return RPTC_EALIGN;
     auto cache = [&](const void *o) { return o == k_cache || o == v_cache; };

@@ -31,3 +31,17 @@ def test_scores_over_the_tokens_or_over_each_other(lib):
     for call in (dict(tokens=t, logprob=t + 32), dict(tokens=t, logprob=t - 16), dict(logprob=a, entropy=a + 16), dict(ids=a, tops=a + 64, top=2)):
         if not torch.cuda.is_available():
             assert logprobs(lib, **call) not in (0,) + REFUSED
+
+
+def test_rows_read_back_over_each_other(lib):
+    kc, vc, k, v = 1 << 22, 1 << 23, 1 << 20, 1 << 21
+
+    def read(seqs=1, rows=4, kv_heads=2, st=(128, 64, 128, 64)):
+        return lib.rptc_kv4_read(kc, vc, k, v, seqs, rows, kv_heads, 64, 16, *st, None, None)
+    for i in range(4):
+        st = [128, 64, 128, 64]
+        st[i] = 0
+        assert read(st=st) == ESHAPE
+        if not torch.cuda.is_available():       # one row, one head: its stride means nothing
+            assert read(rows=1, kv_heads=1, st=st) not in (0,) + REFUSED
+    assert read(seqs=2, rows=1, st=(0, 64, 128, 64)) == ESHAPE
