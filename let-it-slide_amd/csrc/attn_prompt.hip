@@ -1078,7 +1078,7 @@ extern "C" int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint
     const int64_t st[8] = {strides->q_token, strides->q_head, strides->k_token, strides->k_head,
                            strides->v_token, strides->v_head, strides->out_token, strides->out_head};
     for (int i = 0; i < 8; i++) {
-        if (st[i] < 0 || (i != 4 && i != 5 && i != 2 && i != 3 && st[i] == 0)) return RPTC_ESHAPE;
+        if (st[i] < 0 || (i >= 6 && st[i] == 0)) return RPTC_ESHAPE;     // (what is read may repeat)
         if (st[i] % 8 != 0) return RPTC_EALIGN;
         if (i % 2 == 0 && st[i] > (1 << 23)) return RPTC_ELIMIT;     // 64 rows of a step inside 32-bit offsets
     }

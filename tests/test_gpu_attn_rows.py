@@ -89,3 +89,15 @@ def test_rows_whose_scores_are_all_minus_infinity(rk, n, L, heads, kvh, hd):
     none = torch.arange(n, device="cuda") % 8 == 5
     assert bool((out2[none] == 0).all()) and bool((lse2[none] == -math.inf).all())
     assert torch.equal(out2[~none], out[~none]) and torch.equal(lse2[~none], lse[~none])
+
+
+@pytest.mark.parametrize("n,L,heads,kvh,hd", FORMS)
+def test_one_query_for_all_heads_or_rows(rk, n, L, heads, kvh, hd):
+    # a query that is repeated by a stride of 0 gives the bits of its copies
+    k, v = randn(2, L, kvh, hd), randn(3, L, kvh, hd)
+    args = dict(q_start=ints([0, n]), k_start=ints([0]), k_len=ints([L]), timed=False)
+    for q in (randn(1, n, 1, hd).expand(n, heads, hd), randn(1, 1, heads, hd).expand(n, heads, hd), randn(1, 1, 1, hd).expand(n, heads, hd)):
+        out, want = torch.empty(n, heads, hd, dtype=F16, device="cuda"), torch.empty(n, heads, hd, dtype=F16, device="cuda")
+        rk.attn_prompt(q, k, v, out, **args)
+        rk.attn_prompt(q.contiguous(), k, v, want, **args)
+        assert torch.equal(out, want)

@@ -45,3 +45,13 @@ def test_rows_read_back_over_each_other(lib):
         if not torch.cuda.is_available():       # one row, one head: its stride means nothing
             assert read(rows=1, kv_heads=1, st=st) not in (0,) + REFUSED
     assert read(seqs=2, rows=1, st=(0, 64, 128, 64)) == ESHAPE
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="with a device the call would read its pointers")
+def test_one_query_for_all_rows_or_heads_is_not_refused(lib):
+    # strides of 0 repeat what is read; what is written may not repeat
+    for st, refused in (((0, 64, 128, 64, 128, 64, 256, 64), False), ((256, 0, 128, 64, 128, 64, 256, 64), False), ((0, 0, 0, 0, 0, 0, 256, 64), False),
+                        ((256, 64, 128, 64, 128, 64, 0, 64), True), ((256, 64, 128, 64, 128, 64, 256, 0), True)):
+        rc = lib.rptc_attn_prompt(16, 1 << 20, 1 << 21, 1 << 22, None, None, None, None, 1, 8, 8, 8, 4, 2, 64, ctypes.byref(rk.PromptStrides(*st)),
+                                  0.125, 1, 0, None, 0, None, None)
+        assert (rc == ESHAPE) if refused else rc not in (0,) + REFUSED
