@@ -172,6 +172,8 @@ class QuantizedLlama(torch.nn.Module):
             raise ValueError(f"a prompt of {max(lens)} tokens exceeds the model's max_len {sh.max_len}")
         if store and len(lens) != 1:
             raise ValueError("store takes one sequence: the cache holds one")
+        if int(tokens.min()) < 0 or int(tokens.max()) >= sh.vocab:
+            raise ValueError("token ids outside the model's vocabulary")
         dev = self.embed.device
         pos = torch.cat([torch.arange(n) for n in lens]).to(dev)
         ends = torch.tensor(lens).cumsum(0)
