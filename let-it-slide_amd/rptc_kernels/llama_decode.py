@@ -109,7 +109,12 @@ class QuantizedLlama(torch.nn.Module):
         x = self.embed[tokens]                                                     # [T, d]
         if self.cache_bits == 4:
             # the rows a chunk reads back (one token: none, the attention reads the cache itself)
-            rows = 1 if T == 1 else int(pos[-1]) + 1
+            rows = 1
+            if T > 1:
+                p = pos.tolist()
+                if p != list(range(p[0], p[0] + T)) or p[0] < 0 or p[-1] >= sh.max_len:
+                    raise ValueError("a chunk on a 4-bit cache takes consecutive positions inside the cache")
+                rows = p[-1] + 1
             attend = lambda i, q, k, v: self._attend_kv4(i, q, k, v, pos, rows)
         else:
             key_pos = torch.arange(sh.max_len, device=x.device)
