@@ -400,6 +400,8 @@ int64_t rptc_lite_viterbi_scratch_bytes(int L, int R, int64_t rows, int64_t step
  * rows [q_start[s], q_start[s+1]) and the key rows [k_start[s], k_start[s] + k_len[s]); with causal != 0 query i of Lq sees
  * the keys j <= i + Lk - Lq (the last query sees all: a chunk at the end of a context), else all Lk.
  *   out[i] = softmax(scale * q[i] . K^T) V,  lse[i] = log sum exp(scale * q[i] . K^T)  (lse float [total_q][heads], may be NULL)
+ * The weights enter the product with V rounded to dtype, where the device is at most half full or query rows few in two terms: the error is 1.00 to
+ * 1.33 times that of the output's own rounding.
  * A query that sees no key, or none with a score above -inf, gets out = 0, lse = -inf.  What a query does not see does not reach
  * it, not-a-number included.
  * Rows of q outside every sequence, and sequences whose rows lie outside q or k (checked on the device), are left unwritten.

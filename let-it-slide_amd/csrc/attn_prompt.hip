@@ -7,7 +7,8 @@
 // c q_i.k_j (raised, and the sums rescaled, only where a score exceeds it by more than 2^8, so p stays below 256; in fp16 all of
 // them times 2^7, which the quotient takes off again).
 // Scores, m, l and the output sums are fp32; p is rounded to the inputs' type for the matrix unit (by at most
-// 2^-11 of it in fp16, 2^-8 in bf16: the products need two operands of one type), l adds the unrounded p.
+// 2^-11 of it in fp16, 2^-8 in bf16: the products need two operands of one type), l adds the unrounded p.  Calls that leave the matrix unit
+// idle put what the rounding left in as well (see prompt_plan).
 //
 // A workgroup of four waves owns 128 query rows of one head (64 or 32 in the forms for fewer rows), 32 a wave, and walks over its
 // keys 64 at a time.
@@ -294,7 +295,7 @@ __device__ __forceinline__ void change_values(uint16_t *v, int walk)
 // What a wave holds of 32 query rows, and the parts of a step over KEYS keys (a multiple of 32).  Lane (col, c): row col; of
 // every eight keys and of every eight dimensions the four from 4c on.
 // TERMS = 2: p enters the product as the sum of two numbers of the type (its rounding and what that left), so that
-// the output's own rounding is what is left: for the calls that leave the matrix unit idle.
+// the output's own rounding is what is left: for the calls that leave the matrix unit idle (see prompt_plan).
 template <int HD, class T, int KEYS, int TERMS>
 struct PromptWave {
     static constexpr int kSteps = HD / 16, kDims = HD / 32, kBlocks = KEYS / 32;
@@ -473,14 +474,14 @@ constexpr int kWaveKeys = G == 2 ? 32 : 64;    // keys of a step and wave
 template <int HD, int G>
 constexpr int kPlaces = HD > 128 ? 1 : HD == 128 ? 2 : HD == 64 && G == 1 ? 3 : 4;
 
-template <int HD, class T, int G>
+template <int HD, class T, int G, int TERMS>
 __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(kPlaces<HD, G>, kPlaces<HD, G>))) void attn_prompt_kernel(const PromptArgs a)
 {
     extern __shared__ __align__(16) uint16_t lds[];       // two buffers of K, two of V, [kKeys][HD] each
     constexpr int kMine = kWaveKeys<HD, G>, kKeys = G * kMine, kTile = kKeys * HD, kRows = kWideRows / G;
     static_assert(G == 1 || 2 * 32 * HD * 4 <= 4 * kTile * 2, "the sums of two waves fit where K and V were");
     __shared__ float s_ml[2][32][2];
-    __shared__ uint32_t s_marks[2][PromptWave<HD, T, kMine, 1>::kMarks * kPromptThreads];
+    __shared__ uint32_t s_marks[2][PromptWave<HD, T, kMine, TERMS>::kMarks * kPromptThreads];
     __shared__ int s_again;
     int tid = threadIdx.x, lane = tid & 63, c = lane >> 5, col = lane & 31;
     const int wave = uniform(tid >> 6);
@@ -537,7 +538,7 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
         request_v(k_lo, 0);
         if (k_lo + kKeys < k_hi) request_k(k_lo + kKeys, 1);
     }
-    PromptWave<HD, T, kMine, 1> w;
+    PromptWave<HD, T, kMine, TERMS> w;
     w.tid = tid;
     w.begin(a, t, row, head);
     w.settle();
@@ -558,7 +559,7 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
         }
         const float off = w.bound(s, a.c);
         w.scores(lds + (buf ^ 1) * kTile + koff * HD, next);
-        uint32_t p[1][kMine / 32][8];
+        uint32_t p[TERMS][kMine / 32][8];
         w.weights(s, a.c, off, p);
         w.product(lds + (2 + buf) * kTile + koff * HD, p);
     };
@@ -670,7 +671,7 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
                 __syncthreads();
                 if (k0 + koff >= see_most) continue;
                 float16_t s[kMine / 32];
-                uint32_t p[1][kMine / 32][8];
+                uint32_t p[TERMS][kMine / 32][8];
                 w.scores_of(lds + buf * kTile + koff * HD, walk, s);
                 if (k0 + koff + kMine > see_least) w.mask(s, see - k0 - koff);
                 w.weights(s, a.c, w.bound(s, a.c), p);
@@ -940,9 +941,11 @@ static constexpr size_t narrow_lds() { return (size_t)4 * 2 * kNarrowKeys<HD> * 
 template <int HD, class T>
 static int prepare_prompt()
 {
-    int rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<HD, T, 1>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<HD, 1>());
+    int rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<HD, T, 1, 1>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<HD, 1>());
     if (rc) return rc;
-    rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<HD, T, 2>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<HD, 2>());
+    rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<HD, T, 2, 1>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<HD, 2>());
+    if (rc) return rc;
+    rc = (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_kernel<HD, T, 2, 2>), hipFuncAttributeMaxDynamicSharedMemorySize, prompt_lds<HD, 2>());
     if (rc) return rc;
     return (int)hipFuncSetAttribute(reinterpret_cast<const void *>(&attn_prompt_narrow_kernel<HD, T>), hipFuncAttributeMaxDynamicSharedMemorySize, narrow_lds<HD>());
 }
@@ -961,6 +964,7 @@ int prepare_attn_prompt()
 struct PromptPlan {
     int rows;                              // query rows of a workgroup: 128 or 64 (the wide kernel), 32 (the narrow one)
     int tiles, splits;
+    int terms;                             // of a weight in the second product
 };
 
 // sequences cut into tiles: at most so many (whatever the sequences' lengths are)
@@ -975,6 +979,10 @@ static int64_t prompt_tiles(int64_t seqs, int64_t total_q, int64_t rows) { retur
 // of 4 33 / 23 / 18, 8192 of 16 177 / 188 / 287; hd 256: 2000 rows of 16 heads 105 / 88 / 113, 3000 143 / 175 / 195, 700 of 8 40 / 31 / 23.  Behind 8000
 // keys, 32 / 8 heads x 128, 1 / 2 / 4 / 8 pieces: 150 rows in 64s 95 / 60 / 46 / 46, 512 rows 103 / 96 / 100 / 116, 8 rows in 32s
 // 64 / 40 / 26 / 20.
+// Two terms a weight (the output's own rounding is then what is left, 1.00 times it, with one term 1.2 to 1.33) in the 32-row form, and in the
+// 64-row form where at most half of the compute units have a workgroup: the matrix unit idles there.  One / two, us: 37 rows of 32 heads x 128
+// 7.1 / 7.2, 130 of 32 / 8 8.1 / 8.4; with more it is the time of the products: 512 rows of 32 heads 12.7 / 14.0, 200 behind 4000 38 / 44,
+// packed 1 .. 2049 rows of 16 heads x 64 29 / 36, and in the 128-row form 2048 rows of 32 heads 51 / 65, 8192 of 32 / 8 508 / 688.
 static PromptPlan prompt_plan(int64_t seqs, int64_t total_q, int64_t total_k, int64_t heads, int64_t hd, int64_t max_k, int cus)
 {
     struct Form { int rows, places; double start, alone, busy; };
@@ -985,7 +993,7 @@ static PromptPlan prompt_plan(int64_t seqs, int64_t total_q, int64_t total_k, in
     // the longest walk: no longer than max_k, and where that is no more than all rows, likely not over twice the average sequence's
     const double longest = (double)(max_k < 2 * total_k / seqs ? max_k : 2 * total_k / seqs), s = (longest + 63) / 64;
     const double even = total_k > total_q ? 1 - 0.5 * (double)total_q / (double)total_k : 0.5;
-    PromptPlan best = {kWideRows, 0, 1};
+    PromptPlan best = {kWideRows, 0, 1, 1};
     double least = 0;
     for (const Form &f : forms[hd <= 64 ? 0 : hd == 128 ? 1 : 2]) {
         const int64_t tiles = prompt_tiles(seqs, total_q, f.rows);
@@ -997,7 +1005,7 @@ static PromptPlan prompt_plan(int64_t seqs, int64_t total_q, int64_t total_k, in
             double us = f.start * rounds + s / n * (busy > f.alone ? busy : f.alone);
             if (n > 1) us += 3.5 + (double)total_q * heads * n * hd * (8 / 4.5e6);
             if (best.tiles && us >= least) continue;
-            best = {f.rows, (int)tiles, n};
+            best = {f.rows, (int)tiles, n, f.rows == kNarrowRows || (f.rows < kWideRows && 2 * tiles * heads * n <= cus) ? 2 : 1};
             least = us;
         }
     }
@@ -1029,16 +1037,15 @@ static int prompt_sizes(int64_t seqs, int64_t total_q, int64_t total_k, int64_t 
 }
 
 template <int HD, class T>
-static void launch_prompt(const PromptArgs &a, int rows, hipStream_t s)
+static void launch_prompt(const PromptArgs &a, const PromptPlan &plan, hipStream_t s)
 {
     if (a.first_tile) hipLaunchKernelGGL(attn_prompt_table_kernel, dim3(1), dim3(kTableThreads), 0, s, a);
     const dim3 grid((unsigned)(a.heads * a.tiles * a.splits));
-    if (rows == kWideRows) {
-        hipLaunchKernelGGL((attn_prompt_kernel<HD, T, 1>), grid, dim3(kPromptThreads), (prompt_lds<HD, 1>()), s, a);
-        return;
-    }
-    if (rows == kWideRows / 2) hipLaunchKernelGGL((attn_prompt_kernel<HD, T, 2>), grid, dim3(kPromptThreads), (prompt_lds<HD, 2>()), s, a);
-    else hipLaunchKernelGGL((attn_prompt_narrow_kernel<HD, T>), grid, dim3(kPromptThreads), narrow_lds<HD>(), s, a);
+    const dim3 block(kPromptThreads);
+    if (plan.rows == kWideRows) hipLaunchKernelGGL((attn_prompt_kernel<HD, T, 1, 1>), grid, block, (prompt_lds<HD, 1>()), s, a);
+    else if (plan.rows == kNarrowRows) hipLaunchKernelGGL((attn_prompt_narrow_kernel<HD, T>), grid, block, narrow_lds<HD>(), s, a);
+    else if (plan.terms == 2) hipLaunchKernelGGL((attn_prompt_kernel<HD, T, 2, 2>), grid, block, (prompt_lds<HD, 2>()), s, a);
+    else hipLaunchKernelGGL((attn_prompt_kernel<HD, T, 2, 1>), grid, block, (prompt_lds<HD, 2>()), s, a);
     if (a.splits == 1) return;
     const unsigned tile_rows = (unsigned)a.tiles << a.row_bits;
     if (a.splits <= kFewPieces) hipLaunchKernelGGL((attn_prompt_merge_few_kernel<HD, T>), dim3(tile_rows, (unsigned)(a.heads + 3) / 4), dim3(256), 0, s, a);
@@ -1125,10 +1132,10 @@ extern "C" int rptc_attn_prompt(const uint16_t *q, const uint16_t *k, const uint
     if ((rc = timer.begin(dev, s, ms))) return rc;
     const bool f16 = dtype == RPTC_F16;
     switch (hd) {
-    case 32: f16 ? launch_prompt<32, TypeF16>(a, plan.rows, s) : launch_prompt<32, TypeBf16>(a, plan.rows, s); break;
-    case 64: f16 ? launch_prompt<64, TypeF16>(a, plan.rows, s) : launch_prompt<64, TypeBf16>(a, plan.rows, s); break;
-    case 128: f16 ? launch_prompt<128, TypeF16>(a, plan.rows, s) : launch_prompt<128, TypeBf16>(a, plan.rows, s); break;
-    default: f16 ? launch_prompt<256, TypeF16>(a, plan.rows, s) : launch_prompt<256, TypeBf16>(a, plan.rows, s); break;
+    case 32: f16 ? launch_prompt<32, TypeF16>(a, plan, s) : launch_prompt<32, TypeBf16>(a, plan, s); break;
+    case 64: f16 ? launch_prompt<64, TypeF16>(a, plan, s) : launch_prompt<64, TypeBf16>(a, plan, s); break;
+    case 128: f16 ? launch_prompt<128, TypeF16>(a, plan, s) : launch_prompt<128, TypeBf16>(a, plan, s); break;
+    default: f16 ? launch_prompt<256, TypeF16>(a, plan, s) : launch_prompt<256, TypeBf16>(a, plan, s); break;
     }
     return timer.end();
 }

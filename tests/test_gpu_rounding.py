@@ -55,6 +55,7 @@ def formula(q, k, v, scale):
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("n,L,heads,hd,bound", [
     (30, 600, 4, 128, 1.1), (32, 4000, 8, 64, 1.1), (20, 3000, 4, 256, 1.1),      # few rows: two terms a weight
+    (37, 37, 32, 128, 1.1), (130, 130, 8, 128, 1.1), (250, 250, 16, 64, 1.1), (100, 100, 4, 256, 1.1), (200, 200, 4, 32, 1.1),   # short prompts: too
     (512, 512, 32, 128, 1.5), (2600, 2600, 16, 64, 1.5),                          # one term, as documented: 1.2 to 1.4
 ])
 def test_prompt_attention(rk, n, L, heads, hd, bound, dtype):
