@@ -354,8 +354,8 @@ struct PromptWave {
             for (int r = 0; r < 16; r++)
                 if (32 * h + 8 * (r / 4) + r % 4 >= left) s[h][r] = -INFINITY;
     }
-    // raises the bound where a score exceeds it by more than 2^kLazy; returns the bound to take off
-    __device__ __forceinline__ float bound(const float16_t (&s)[kBlocks], float scale)
+    // raises the bound where a score exceeds it by more than 2^kLazy; returns what to take off of the scores times `scale`
+    __device__ __forceinline__ float bound(float16_t (&s)[kBlocks], float &scale)
     {
         float mx = s[0][0];
 #pragma unroll
@@ -372,7 +372,24 @@ struct PromptWave {
             for (int d = 0; d < kDims; d++) acc[d] *= f;
             m = up;
         }
-        return (m == -INFINITY ? 0.f : m) - T::kWeightLog2;
+        float off = (m == -INFINITY ? 0.f : m) - T::kWeightLog2;
+        // the bound is a rounded product, and what the rounding left a factor of all weights: within 2^(1/32) of 1 below 2^20, but up to 2^32
+        // at 2^30.  From 2^20 on the scores are multiplied and rounded as the bound was, and their differences to it taken
+        const uint32_t size = __builtin_bit_cast(uint32_t, m) & 0x7FFFFFFFu;
+        const bool far = size - 0x49800000u < 0x7F800000u - 0x49800000u;      // 2^20 <= |m| < infinity
+        if (__ballot(far)) {
+#pragma clang fp contract(off)
+#pragma unroll
+            for (int h = 0; h < kBlocks; h++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const float product = s[h][r] * scale;
+                    s[h][r] = far ? product - m : s[h][r];
+                }
+            scale = far ? 1.f : scale;
+            off = far ? -T::kWeightLog2 : off;
+        }
+        return off;
     }
     // p = exp2(c s - bound), packed in pairs of keys
     __device__ __forceinline__ void weights(const float16_t (&s)[kBlocks], float scale, float off, uint32_t (&p)[TERMS][kBlocks][8])
@@ -471,11 +488,12 @@ constexpr int kWaveKeys = G == 2 ? 32 : 64;    // keys of a step and wave
 
 // workgroups that a compute unit holds at once (by their registers; LDS has room for as many): said to the compiler as least and
 // most, so that it uses the registers for operands asked for early instead of for more of them
-template <int HD, int G>
-constexpr int kPlaces = HD > 128 ? 1 : HD == 128 ? 2 : HD == 64 && G == 1 ? 3 : 4;
+// (two terms a weight: for calls that leave places free)
+template <int HD, int G, int TERMS>
+constexpr int kPlaces = HD > 128 ? 1 : HD == 128 || TERMS == 2 ? 2 : HD == 64 && G == 1 ? 3 : 4;
 
 template <int HD, class T, int G, int TERMS>
-__global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(kPlaces<HD, G>, kPlaces<HD, G>))) void attn_prompt_kernel(const PromptArgs a)
+__global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(kPlaces<HD, G, TERMS>, kPlaces<HD, G, TERMS>))) void attn_prompt_kernel(const PromptArgs a)
 {
     extern __shared__ __align__(16) uint16_t lds[];       // two buffers of K, two of V, [kKeys][HD] each
     constexpr int kMine = kWaveKeys<HD, G>, kKeys = G * kMine, kTile = kKeys * HD, kRows = kWideRows / G;
@@ -557,10 +575,11 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
             masked_from = min(masked_from, k0 + koff);
             w.mask(s, see - k0 - koff);
         }
-        const float off = w.bound(s, a.c);
+        float scale = a.c;
+        const float off = w.bound(s, scale);
         w.scores(lds + (buf ^ 1) * kTile + koff * HD, next);
         uint32_t p[TERMS][kMine / 32][8];
-        w.weights(s, a.c, off, p);
+        w.weights(s, scale, off, p);
         w.product(lds + (2 + buf) * kTile + koff * HD, p);
     };
     if (k_lo < k_hi) {
@@ -674,7 +693,9 @@ __global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(
                 uint32_t p[TERMS][kMine / 32][8];
                 w.scores_of(lds + buf * kTile + koff * HD, walk, s);
                 if (k0 + koff + kMine > see_least) w.mask(s, see - k0 - koff);
-                w.weights(s, a.c, w.bound(s, a.c), p);
+                float scale = a.c;
+                const float off = w.bound(s, scale);
+                w.weights(s, scale, off, p);
                 w.product(lds + (2 + buf) * kTile + koff * HD, p);
             }
             if (walk != kFiniteOnly) w.take_marks(s_marks[walk - kUps] + tid);
@@ -766,9 +787,10 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
             masked_from = min(masked_from, k0);
             w.mask(s, see - k0);
         }
-        const float off = w.bound(s, a.c);
+        float scale = a.c;
+        const float off = w.bound(s, scale);
         uint32_t p[2][kStep / 32][8];
-        w.weights(s, a.c, off, p);
+        w.weights(s, scale, off, p);
         if (more) wait_for_lds_loads_but<kRequests>();     // V is there (the next K was asked for behind it)
         else wait_for_lds_loads();
         w.product(vt, p);
@@ -799,7 +821,9 @@ __global__ __launch_bounds__(kPromptThreads, HD > 64 ? 1 : 2) void attn_prompt_n
                 uint32_t p[2][kStep / 32][8];
                 w.scores_of(kt, walk, s);
                 if (k0 + kStep > see_least) w.mask(s, see - k0);
-                w.weights(s, a.c, w.bound(s, a.c), p);
+                float scale = a.c;
+                const float off = w.bound(s, scale);
+                w.weights(s, scale, off, p);
                 w.product(vt, p);
                 wait_for_lds_reads();
             }

@@ -101,3 +101,39 @@ def test_one_query_for_all_heads_or_rows(rk, n, L, heads, kvh, hd):
         rk.attn_prompt(q, k, v, out, **args)
         rk.attn_prompt(q.contiguous(), k, v, want, **args)
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n,L,heads,kvh,hd", FORMS)
+def test_scores_of_millions_and_more(rk, n, L, heads, kvh, hd, dtype):
+    """Scores of 2^28 to 2^37 whose differences, where there are any, are 2^23 and more: one key takes all weight, or those equal to it share it.
+    The output is the mean of their values, rounded: each weight is 1, up to 2 roundings of the sum and the quotient, 2^-22."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    level = torch.randperm(L, generator=g, device="cuda") // 3                     # every score three times
+    size = 60000.0 if dtype == F16 else 2.0 ** 20
+    top = (L + 2) // 3
+    k = (16 * (level - top / 2).round())[:, None, None].to(dtype).expand(L, kvh, hd).contiguous()      # (their products with q: exact in fp32)
+    level = k[:, 0, 0].double()
+    q = torch.full((n, heads, hd), size, dtype=dtype, device="cuda")
+    q[1::3] *= -1
+    q[2::3] = randn(7, 1, heads, hd, dtype=dtype)[:, :, :1] * 0.001                  # rows of ordinary scores between them
+    v = randn(8, L, kvh, hd, dtype=dtype)
+    out, lse = torch.empty_like(q), torch.empty(n, heads, device="cuda")
+    args = dict(q_start=ints([0, n]), k_start=ints([0]), k_len=ints([L]), timed=False)
+    rk.attn_prompt(q, k, v, out, lse=lse, **args)
+    vd = v.double().repeat_interleave(heads // kvh, 1)
+    u = torch.finfo(dtype).eps / 2
+    for i in sorted({0, 1, n // 2 // 3 * 3, n // 2 // 3 * 3 + 1, (n - 1) // 3 * 3, n - 1 - (n - 2) % 3}):
+        sign = -1 if i % 3 == 1 else 1
+        seen = sign * level[:L - n + 1 + i]
+        best = seen == seen.max()
+        want = vd[:L - n + 1 + i][best].mean(0)
+        assert bool(((out[i].double() - want).abs() <= u * want.abs() + 2.0 ** -20).all()), i
+        score = size * float(seen.max()) * hd ** 0.5
+        assert bool(((lse[i].double() - score - math.log(int(best.sum()))).abs() <= 2.0 ** -20 * abs(score) + 1e-5).all()), i
+    # the rows between have the bits they have among their like
+    q2, out2, lse2 = q[2::3].repeat_interleave(3, 0)[:n].contiguous(), torch.empty_like(out), torch.empty_like(lse)
+    if q2.size(0) < n:
+        q2 = torch.cat([q2, q2[-1:].expand(n - q2.size(0), heads, hd)]).contiguous()
+    rk.attn_prompt(q2, k, v, out2, lse=lse2, **args)
+    assert torch.equal(out[2::3], out2[2::3]) and torch.equal(lse[2::3], lse2[2::3])
