@@ -497,12 +497,26 @@ __global__ __launch_bounds__(64 * kKv4Waves<HD>, HD > 128 ? 2 : 4) void kv4_attn
             for (int e = 0; e < kE; e++) acc[e] *= f;
             m = up;
         }
-        const float mc = (m == -INFINITY ? 0.f : m) - kKv4WeightLog2;
+        float mc = (m == -INFINITY ? 0.f : m) - kKv4WeightLog2, scale = a.c;
+        // the bound is a rounded product, and what the rounding left a factor of all weights: within 2^(1/32) of 1 below 2^20, but up to 2^32
+        // at 2^30.  From 2^20 on the scores are multiplied and rounded as the bound was, and their differences to it taken
+        const uint32_t size = __builtin_bit_cast(uint32_t, m) & 0x7FFFFFFFu;
+        const bool far = size - 0x49800000u < 0x7F800000u - 0x49800000u;      // 2^20 <= |m| < infinity
+        if (__ballot(far)) {
+#pragma clang fp contract(off)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float product = s[j / 4][j % 4] * scale;
+                s[j / 4][j % 4] = far ? product - m : s[j / 4][j % 4];
+            }
+            scale = far ? 1.f : scale;
+            mc = far ? -kKv4WeightLog2 : mc;
+        }
         half2_t p2[4], rest[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int r = 2 * j;
-            const float x = __builtin_amdgcn_exp2f(fmaf(s[r / 4][r % 4], a.c, -mc)), y = __builtin_amdgcn_exp2f(fmaf(s[r / 4][r % 4 + 1], a.c, -mc));
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[r / 4][r % 4], scale, -mc)), y = __builtin_amdgcn_exp2f(fmaf(s[r / 4][r % 4 + 1], scale, -mc));
             l += x;
             l += y;
             const float2v_t xy = {x, y};

@@ -95,3 +95,28 @@ def test_one_key_head_in_as_many_pieces_as_are_joined(rk, hd, L):
         o, A = p @ vd, p @ vd.abs()
         E = hd ** -0.5 * (hd + 4) * 2.0 ** -24 * (qd.abs() @ kd.abs().t().contiguous()).amax(-1, keepdim=True)
         assert bool(((out[0].double() - o).abs() <= 2.0 ** -11 * o.abs() + (2.0 ** -21 + 3 * E + 2.0 ** -13) * A + 2.0 ** -25).all()), pos
+
+
+@pytest.mark.parametrize("heads,kvh,hd,n", [(4, 4, 64, 700), (32, 2, 128, 700), (8, 1, 128, 9001), (2, 2, 256, 5000), (3, 3, 32, 900)])
+def test_scores_of_millions_and_more(rk, heads, kvh, hd, n):
+    """Scores of up to 2^34, 2^23 and more apart: one position takes all weight, or those equal to it share it.  The output is the mean
+    of their values, rounded: each weight is 1, up to roundings of the sum and the quotient, 2^-20."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    level = torch.randperm(n, generator=g, device="cuda") // 3
+    k = (12 * (level - n // 6))[:, None, None].half().expand(n, kvh, hd).contiguous()       # one value a row: held exactly, as its minimum
+    level = k[:, 0, 0].double()
+    v = randn(8, n, kvh, hd)
+    kc, vc = rk.kv4_cache(1, kvh, n, hd)
+    rk.kv4_append(k, v, kc, vc, i64([0]), timed=False)
+    rk.kv4_read(kc, vc, k, v, timed=False)
+    assert torch.equal(k[:, 0, 0].double(), level)
+    q = torch.full((1, heads, hd), 60000.0, dtype=torch.float16, device="cuda")
+    q[0, 1::2] *= -1
+    for pos in (n - 1, n // 2, 40):
+        out = torch.empty_like(q)
+        rk.kv4_attn_decode(q, kc, vc, i64([pos]), out, timed=False)
+        vd = v[:pos + 1].double().repeat_interleave(heads // kvh, 1)
+        for h in range(heads):
+            seen = level[:pos + 1] * (-1 if h % 2 else 1)
+            want = vd[seen == seen.max(), h].mean(0)
+            assert bool(((out[0, h].double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -20).all()), (pos, h)
