@@ -19,7 +19,7 @@
 // V^T is read with the transposing LDS read.
 //
 // What bounds it: a SIMD's matrix and vector instructions hardly overlap (a step of 32 rows and 64 keys at hd 128: 0.47 us of one, 0.25 of
-// the other, of 0.9 together), at the clock the power leaves.  8192 causal rows of 32 / 8 heads x 128, bf16: 497 to 512 us, 1.09
+// the other, of 0.9 together), at the clock the power leaves.  8192 causal rows of 32 / 8 heads x 128, bf16: 503 to 530 us, 1.04 to 1.09
 // PFLOP/s, the matrix unit busy for 62 % of it (a library product of 8192^3 1.22 PFLOP/s).  32 rows behind 8000, 32 heads x 128: 30 us
 // for 132 MB, 4.4 TB/s, and 4 for joining the pieces.
 #include "join.hpp"
